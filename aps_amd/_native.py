@@ -5,13 +5,14 @@ The library is built ahead of time (python -m aps_amd.build).  It is NOT built o
 time: if it is missing, every call raises, loudly -- the product path has no CPU fallback.
 torch must be imported before the library is opened so that both bind the same libamdhip64.
 """
+import contextlib
 import ctypes as C
 import os
 
 import torch as th
 
 _LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc", "libaps_amd.so")
-ABI_VERSION = 58
+ABI_VERSION = 59
 
 
 class StftParams(C.Structure):
@@ -202,6 +203,16 @@ SIGNATURES = {
                                               _I64, _F, _P]),
     "aps_mvdr_covariance_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
                                                _I64, _I64, _I32, _P, _P]),
+    "aps_attention_packed": (C.c_int, [_P, _P, _P, _P, _I32, _P, _P] + [_I64] * 11 + [_I32, _I32, _F, _P]),
+    "aps_attention_packed_backward_workspace": (_I64, [_I64, _I64]),
+    "aps_attention_packed_backward": (C.c_int, [_P] * 7 + [_I32, _P, _P, _P] + [_I64] * 13 +
+                                      [_I32, _I32, _F, _P, _P]),
+    "aps_paged_append": (C.c_int, [_P] * 6 + [_I32, _P, _I32] + [_I64] * 12 + [_I32, _P]),
+    "aps_attention_paged_workspace": (_I64, [_I64] * 7 + [_I32]),
+    "aps_attention_paged": (C.c_int, [_P] * 5 + [_I32, _P, _I32, _P] + [_I64] * 11 + [_I32, _F, _I32, _P, _P]),
+    "aps_beam_select_workspace": (_I64, [_I64] * 4),
+    "aps_beam_select": (C.c_int, [_P, _I64, _P, _P, _I64, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I32, _P, _P]),
+    "aps_beam_reorder": (C.c_int, [_P, _P, _P, _P, _I64, _P, _I64, _I64, _I64, _P]),
 }
 
 _lib = None
@@ -253,6 +264,11 @@ def ptr(t):
 
 def stream_of(t: th.Tensor):
     return C.c_void_p(th.cuda.current_stream(t.device).cuda_stream)
+
+
+def on_device_of(t: th.Tensor):
+    """context in which the device of `t` is the current one (launches go to the current device)"""
+    return contextlib.nullcontext() if t.device.index == th.cuda.current_device() else th.cuda.device(t.device)
 
 
 def needs_grad(*tensors) -> bool:

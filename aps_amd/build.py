@@ -13,8 +13,10 @@ LIB = os.path.join(CSRC, "libaps_amd.so")
 OBJ_DIR = os.path.join(CSRC, "_obj")
 SOURCES = ["aps_core.hip", "stft.hip", "feats.hip", "mvdr.hip", "nn.hip", "lstm.hip", "context.hip",
            "conv.hip", "decoder.hip", "spatial.hip", "augment.hip", "grad.hip",
-           "gemm_split.hip", "gemm_fp16x2.hip", "gemm_panel.hip", "gemm_tn.hip", "conformer_mega.hip"]
+           "gemm_split.hip", "gemm_fp16x2.hip", "gemm_panel.hip", "gemm_tn.hip", "conformer_mega.hip",
+           "attention_packed.hip", "attention_paged.hip", "beam.hip"]
 HEADERS = ["common.h", "fft_core.h", "twiddles.h", "conv_core.h", "grad_core.h", "grad_api.inc",
+           "attention_tile.h", "attention_rows.h",
            os.path.join("..", "..", "include", "aps_amd.h")]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 # No packed-fp32 VALU instructions (v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32) in any kernel: round 3

@@ -1,0 +1,355 @@
+// Attention over sequences packed end to end, and its gradients:
+//   P_rj = exp(scale q_r . k_j - lse_r),  o_r = sum_j P_rj v_j                    (attention_rows.h)
+//   D_r  = do_r . o_r
+//   dS_rj = P_rj (do_r . v_j - D_r) scale
+//   dq_r = sum_j dS_rj k_j,   dk_j = sum_r dS_rj q_r,   dv_j = sum_r P_rj do_r
+// with r over the rows (token, head of the group) that see key j: the sums over a group's heads are part
+// of the same accumulation.  Two launches, neither with atomics, so the gradients are bit-reproducible:
+// the first walks the keys for a tile of rows (D_r, dq), the second walks the rows for a tile of keys
+// (dk, dv); P is formed again in each from the saved lse.
+#include "attention_rows.h"
+
+namespace aps {
+namespace att {
+
+struct GradArgs {
+  const void *q, *k, *v, *o, *go;
+  const float* lse;    // [total, Hq]
+  float* delta;        // [total, Hq]
+  void *gq, *gk, *gv;  // [total, Hq | Hkv, D]
+  Index cu;
+  int64_t total, N, tiles;
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h, go_t, go_h;
+  int32_t G, Hkv, causal;
+  float c, scale;
+};
+
+// dq: the forward kernel's walk, with V as the left operand of dP^T = V dO^T beside S^T = K Q^T and K
+// read transposed for dq^T = K^T dS^T
+template <typename T, int D>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void attention_rows_backward_kernel(GradArgs a) {
+  constexpr int BK = key_tile<T>(), E = chunk_elems<T>(), KS = 2 * E, NS = D / KS, NKB = BK / 32, NDB = D / 32;
+  constexpr int NPS = 32 / KS, TILE = BK * D * (int)sizeof(T);
+  __shared__ __align__(16) char lds[4 * TILE];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, half = lane >> 5;
+  const int h = blockIdx.x % a.Hkv;
+  const int64_t want = a.tiles - 1 - blockIdx.x / a.Hkv;
+  const SeqTile t = find_tile(a.cu, a.N, a.total, a.G, kRowTile, want, lane);
+  const int Hq = a.Hkv * a.G;
+  if (t.seq < 0) {
+    if (h == 0)
+      clear_rows<T, D>(static_cast<T*>(a.gq), a.cu, a.N, a.total, Hq, want - t.used, a.tiles - t.used);
+    return;
+  }
+  const int kv = t.len, rows = t.len * a.G;
+  const int row0 = t.tile * kRowTile + wv * 32, row = row0 + (lane & 31);
+  const bool live = row < rows;
+  const int tok = live ? row / a.G : 0, head = h * a.G + (live ? row - tok * a.G : 0);
+  const int pos = live ? (a.causal ? tok : kv - 1) : -1;
+  const int last = min(row0 + 32, rows) - 1;
+  const int end = a.causal ? (min(t.tile * kRowTile + kRowTile, rows) - 1) / a.G + 1 : kv;
+  const int wave_end = row0 >= rows ? 0 : (a.causal ? last / a.G + 1 : kv);
+  const int wave_min = a.causal ? row0 / a.G : kv - 1;
+  const int64_t at = (t.start + tok) * Hq + head;
+  const T* qp = static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + head * a.q_h;
+  const T* gp = static_cast<const T*>(a.go) + (t.start + tok) * a.go_t + head * a.go_h;
+  const T* op = static_cast<const T*>(a.o) + at * D;
+  u32x4 qf[NS], gf[NS];
+  float delta = 0.f;
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    qf[s] = gf[s] = u32x4{0, 0, 0, 0};
+    if (live) {
+      const int c = (2 * s + half) * E;
+      qf[s] = *reinterpret_cast<const u32x4*>(qp + c);
+      gf[s] = *reinterpret_cast<const u32x4*>(gp + c);
+      delta += dot_chunk<T>(gf[s], *reinterpret_cast<const u32x4*>(op + c));
+    }
+  }
+  delta += __shfl_xor(delta, 32, 64);
+  const float lse = live ? a.lse[at] : INFINITY;
+  if (live && half == 0) a.delta[at] = delta;
+
+  RowsArgs kvargs;
+  kvargs.k = a.k, kvargs.v = a.v, kvargs.k_t = a.k_t, kvargs.k_h = a.k_h, kvargs.v_t = a.v_t, kvargs.v_h = a.v_h;
+  f32x16 acc[NDB];
+#pragma unroll
+  for (int d = 0; d < NDB; ++d) acc[d] = f32x16{0};
+  const int tile_hi = (end + BK - 1) / BK;
+  KvStage<T, D, false> st;
+  st.load(kvargs, t.start, t.seq, h, 0, end);
+  st.store(lds, lds + TILE, nullptr);
+  __syncthreads();
+  for (int kt = 0; kt < tile_hi; ++kt) {
+    const char* tk = lds + (kt & 1) * 2 * TILE;
+    const char* tv = tk + TILE;
+    char* nk = lds + ((kt + 1) & 1) * 2 * TILE;
+    const bool more = kt + 1 < tile_hi;
+    if (more) st.load(kvargs, t.start, t.seq, h, (kt + 1) * BK, end);
+    const int k0 = kt * BK;
+    if (k0 < wave_end) {
+      const bool edge = k0 + BK - 1 > wave_min;
+#pragma unroll
+      for (int b = 0; b < NKB; ++b) {
+        f32x16 s = f32x16{0}, g = f32x16{0};
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+          s = mma<T>(frag<T, D>(tk, b * 32 + (lane & 31), i, half), qf[i], s);
+          g = mma<T>(frag<T, D>(tv, b * 32 + (lane & 31), i, half), gf[i], g);
+        }
+        float p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = exp2_fast(fmaf(s[i], a.c, -lse)) * (g[i] - delta);
+        if (edge) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (k0 + b * 32 + result_row(i, half) > pos) p[i] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NPS; ++i) {
+          const u32x4 pf = pack<T>(p + i * (KS / 2));
+#pragma unroll
+          for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(frag_t<T, D>(tk, b * 32, i, d, lane), pf, acc[d]);
+        }
+      }
+    }
+    if (more) st.store(nk, nk + TILE, nullptr);
+    __syncthreads();
+  }
+  if (!live) return;
+  T* po = static_cast<T*>(a.gq) + at * D;
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      store4<T>(po + d * 32 + result_row(i, half),
+                f32x4{acc[d][i] * a.scale, acc[d][i + 1] * a.scale, acc[d][i + 2] * a.scale, acc[d][i + 3] * a.scale});
+}
+
+// dk, dv: a workgroup per (tile of 128 keys, key head), a wavefront per 32 keys whose K and V rows stay
+// in registers as right operands; Q and dO go through LDS, 32 rows (64 for 16-bit types) at a time, with
+// the rows' lse, D_r and positions beside them.  S = Q K^T and dP = dO V^T have the rows in the
+// registers, so P and dS are the right operands of dv^T = dO^T P and dk^T = Q^T dS as they stand.
+template <typename T>
+constexpr int grad_rows() { return sizeof(T) == 2 ? 64 : 32; }
+
+template <typename T, int D>
+__global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention_keys_backward_kernel(GradArgs a) {
+  constexpr int BR = grad_rows<T>(), E = chunk_elems<T>(), CH = D / E, KS = 2 * E, NS = D / KS, NRB = BR / 32;
+  constexpr int NDB = D / 32, NPS = 32 / KS, TILE = BR * D * (int)sizeof(T), PER = BR * CH / 256, STEP = 256 / CH;
+  __shared__ __align__(16) char lds[4 * TILE];
+  __shared__ __align__(16) float s_lse[2][BR], s_delta[2][BR];
+  __shared__ __align__(16) int s_pos[2][BR];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, half = lane >> 5;
+  const int h = blockIdx.x % a.Hkv;
+  const int64_t want = blockIdx.x / a.Hkv;  // the first keys are seen by the most rows: they go first
+  const SeqTile t = find_tile(a.cu, a.N, a.total, 1, kRowTile, want, lane);
+  const int Hq = a.Hkv * a.G;
+  if (t.seq < 0) {
+    if (h == 0) {
+      clear_rows<T, D>(static_cast<T*>(a.gk), a.cu, a.N, a.total, a.Hkv, want - t.used, a.tiles - t.used);
+      clear_rows<T, D>(static_cast<T*>(a.gv), a.cu, a.N, a.total, a.Hkv, want - t.used, a.tiles - t.used);
+    }
+    return;
+  }
+  const int rows = t.len * a.G, tile0 = t.tile * kRowTile, key0 = tile0 + wv * 32, key = key0 + (lane & 31);
+  const bool live = key < t.len;
+  u32x4 kf[NS], vf[NS];
+  {
+    const T* kp = static_cast<const T*>(a.k) + (t.start + (live ? key : 0)) * a.k_t + h * a.k_h;
+    const T* vp = static_cast<const T*>(a.v) + (t.start + (live ? key : 0)) * a.v_t + h * a.v_h;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      kf[s] = live ? *reinterpret_cast<const u32x4*>(kp + (2 * s + half) * E) : u32x4{0, 0, 0, 0};
+      vf[s] = live ? *reinterpret_cast<const u32x4*>(vp + (2 * s + half) * E) : u32x4{0, 0, 0, 0};
+    }
+  }
+  f32x16 gk[NDB], gv[NDB];
+#pragma unroll
+  for (int d = 0; d < NDB; ++d) gk[d] = gv[d] = f32x16{0};
+
+  u32x4 qr[PER], gr[PER];
+  float r_lse = INFINITY, r_delta = 0.f;
+  int r_pos = -1;
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int row = r0 + threadIdx.x / CH + i * STEP, c = threadIdx.x % CH;
+      qr[i] = gr[i] = u32x4{0, 0, 0, 0};
+      if (row < rows) {
+        const int tok = row / a.G, head = h * a.G + row - tok * a.G;
+        qr[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + head * a.q_h + c * E);
+        gr[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.go) + (t.start + tok) * a.go_t + head * a.go_h + c * E);
+      }
+    }
+    if (threadIdx.x < BR) {
+      const int row = r0 + threadIdx.x;
+      r_lse = INFINITY, r_delta = 0.f, r_pos = -1;
+      if (row < rows) {
+        const int tok = row / a.G;
+        const int64_t at = (t.start + tok) * Hq + h * a.G + row - tok * a.G;
+        r_lse = a.lse[at], r_delta = a.delta[at], r_pos = a.causal ? tok : t.len - 1;
+      }
+    }
+  };
+  auto store = [&](int buf) {
+    char* tq = lds + buf * 2 * TILE;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = tile_at<T, D>(threadIdx.x / CH + i * STEP, threadIdx.x % CH);
+      *reinterpret_cast<u32x4*>(tq + at) = qr[i];
+      *reinterpret_cast<u32x4*>(tq + TILE + at) = gr[i];
+    }
+    if (threadIdx.x < BR)
+      s_lse[buf][threadIdx.x] = r_lse, s_delta[buf][threadIdx.x] = r_delta, s_pos[buf][threadIdx.x] = r_pos;
+  };
+  // causal: the rows before token `tile0` see none of the tile's keys
+  const int lo = a.causal ? (tile0 * a.G) / BR : 0, hi = (rows + BR - 1) / BR;
+  load(lo * BR);
+  store(0);
+  __syncthreads();
+  for (int rt = lo; rt < hi; ++rt) {
+    const int buf = (rt - lo) & 1;
+    const char* tq = lds + buf * 2 * TILE;
+    const char* tg = tq + TILE;
+    const bool more = rt + 1 < hi;
+    if (more) load((rt + 1) * BR);
+#pragma unroll 1
+    for (int b = 0; b < NRB; ++b) {
+      const int r0 = rt * BR + b * 32;
+      // rows [r0, r0 + 32): none sees this wavefront's keys / some see some of them
+      const bool none = key0 >= t.len || r0 >= rows || (a.causal && (min(r0 + 32, rows) - 1) / a.G < key0);
+      if (none) continue;
+      f32x16 s = f32x16{0}, g = f32x16{0};
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        s = mma<T>(frag<T, D>(tq, b * 32 + (lane & 31), i, half), kf[i], s);
+        g = mma<T>(frag<T, D>(tg, b * 32 + (lane & 31), i, half), vf[i], g);
+      }
+      const bool edge = r0 + 32 > rows || key0 + 32 > t.len || (a.causal && r0 / a.G < key0 + 31);
+      float p[16], ds[16];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[buf][b * 32 + j * 8 + half * 4]);
+        const f32x4 dl = *reinterpret_cast<const f32x4*>(&s_delta[buf][b * 32 + j * 8 + half * 4]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = j * 4 + e;
+          p[i] = exp2_fast(fmaf(s[i], a.c, -lse[e]));
+          ds[i] = p[i] * (g[i] - dl[e]);
+        }
+        if (edge) {
+          typedef int i32x4 __attribute__((ext_vector_type(4)));
+          const i32x4 ps = *reinterpret_cast<const i32x4*>(&s_pos[buf][b * 32 + j * 8 + half * 4]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key > ps[e] || !live) p[j * 4 + e] = 0.f, ds[j * 4 + e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NPS; ++i) {
+        const u32x4 pf = pack<T>(p + i * (KS / 2)), df = pack<T>(ds + i * (KS / 2));
+#pragma unroll
+        for (int d = 0; d < NDB; ++d) {
+          gv[d] = mma<T>(frag_t<T, D>(tg, b * 32, i, d, lane), pf, gv[d]);
+          gk[d] = mma<T>(frag_t<T, D>(tq, b * 32, i, d, lane), df, gk[d]);
+        }
+      }
+    }
+    if (more) store(buf ^ 1);
+    __syncthreads();
+  }
+  if (!live) return;
+  T* pk = static_cast<T*>(a.gk) + ((t.start + key) * a.Hkv + h) * D;
+  T* pv = static_cast<T*>(a.gv) + ((t.start + key) * a.Hkv + h) * D;
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int c = d * 32 + result_row(i, half);
+      store4<T>(pk + c, f32x4{gk[d][i] * a.scale, gk[d][i + 1] * a.scale, gk[d][i + 2] * a.scale, gk[d][i + 3] * a.scale});
+      store4<T>(pv + c, f32x4{gv[d][i], gv[d][i + 1], gv[d][i + 2], gv[d][i + 3]});
+    }
+}
+
+template <typename T, int D>
+static void launch_rows(const RowsArgs& a, unsigned grid, hipStream_t st) {
+  hipLaunchKernelGGL((attention_rows_kernel<T, D, false>), dim3(grid), dim3(256), 0, st, a);
+}
+template <typename T, int D>
+static void launch_rows_backward(const GradArgs& a, unsigned grid, hipStream_t st) {
+  hipLaunchKernelGGL((attention_rows_backward_kernel<T, D>), dim3(grid), dim3(256), 0, st, a);
+}
+template <typename T, int D>
+static void launch_keys_backward(const GradArgs& a, unsigned grid, hipStream_t st) {
+  hipLaunchKernelGGL((attention_keys_backward_kernel<T, D>), dim3(grid), dim3(256), 0, st, a);
+}
+
+}  // namespace att
+}  // namespace aps
+
+using namespace aps;
+using namespace aps::att;
+
+extern "C" int aps_attention_packed(const void* q, const void* k, const void* v, const void* cu_seqlens,
+                                    int32_t cu_wide, void* out, float* lse, int64_t total, int64_t N,
+                                    int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t q_t, int64_t q_h,
+                                    int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h, int32_t dtype,
+                                    int32_t causal, float scale, void* stream) {
+  if (total == 0) return APS_OK;
+  APS_CHECK_ARG(q && k && v && cu_seqlens && out && sizes_fit(total, N, Hq, Hkv) && scale > 0.f);
+  const int64_t e = dtype == kTypeF32 ? 4 : 8;
+  APS_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out));
+  APS_CHECK_ARG(q_t % e == 0 && q_h % e == 0 && k_t % e == 0 && k_h % e == 0 && v_t % e == 0 && v_h % e == 0);
+  RowsArgs a{};
+  a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
+  a.cu = Index{cu_seqlens, cu_wide};
+  a.total = total, a.N = N;
+  a.G = (int32_t)(Hq / Hkv), a.Hkv = (int32_t)Hkv;
+  a.tiles = (total * a.G + kRowTile - 1) / kRowTile + N + 1;
+  a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h;
+  a.causal = causal != 0, a.zero_tail = 1, a.splits = 1;
+  a.c = scale * kLog2e;
+  const unsigned grid = (unsigned)(a.tiles * Hkv);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  APS_ATT_DISPATCH(launch_rows, a, grid, st);
+  return aps_launch_status();
+}
+
+extern "C" int64_t aps_attention_packed_backward_workspace(int64_t total, int64_t Hq) {
+  return total < 0 || Hq < 1 ? -1 : total * Hq * (int64_t)sizeof(float);
+}
+
+extern "C" int aps_attention_packed_backward(const void* q, const void* k, const void* v, const void* out,
+                                             const void* g_out, const float* lse, const void* cu_seqlens,
+                                             int32_t cu_wide, void* g_q, void* g_k, void* g_v, int64_t total,
+                                             int64_t N, int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t q_t,
+                                             int64_t q_h, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h,
+                                             int64_t go_t, int64_t go_h, int32_t dtype, int32_t causal,
+                                             float scale, void* workspace, void* stream) {
+  if (total == 0) return APS_OK;
+  APS_CHECK_ARG(q && k && v && out && g_out && lse && cu_seqlens && g_q && g_k && g_v && workspace);
+  APS_CHECK_ARG(sizes_fit(total, N, Hq, Hkv) && scale > 0.f);
+  const int64_t e = dtype == kTypeF32 ? 4 : 8;
+  APS_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(g_out));
+  APS_CHECK_ARG(aligned16(g_q) && aligned16(g_k) && aligned16(g_v));
+  APS_CHECK_ARG(q_t % e == 0 && q_h % e == 0 && k_t % e == 0 && k_h % e == 0 && v_t % e == 0 && v_h % e == 0);
+  APS_CHECK_ARG(go_t % e == 0 && go_h % e == 0);
+  GradArgs a{};
+  a.q = q, a.k = k, a.v = v, a.o = out, a.go = g_out, a.lse = lse, a.delta = static_cast<float*>(workspace);
+  a.gq = g_q, a.gk = g_k, a.gv = g_v;
+  a.cu = Index{cu_seqlens, cu_wide};
+  a.total = total, a.N = N;
+  a.G = (int32_t)(Hq / Hkv), a.Hkv = (int32_t)Hkv;
+  a.q_t = q_t, a.q_h = q_h, a.k_t = k_t, a.k_h = k_h, a.v_t = v_t, a.v_h = v_h, a.go_t = go_t, a.go_h = go_h;
+  a.causal = causal != 0, a.scale = scale, a.c = scale * kLog2e;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  a.tiles = (total * a.G + kRowTile - 1) / kRowTile + N + 1;
+  unsigned grid = (unsigned)(a.tiles * Hkv);
+  APS_ATT_DISPATCH(launch_rows_backward, a, grid, st);
+  if (aps_launch_status() != APS_OK) return APS_ERR_LAUNCH;
+  a.tiles = (total + kRowTile - 1) / kRowTile + N + 1;
+  grid = (unsigned)(a.tiles * Hkv);
+  APS_ATT_DISPATCH(launch_keys_backward, a, grid, st);
+  return aps_launch_status();
+}

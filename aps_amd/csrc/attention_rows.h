@@ -1,0 +1,293 @@
+// Forward attention of a batch of packed sequences, a workgroup per (tile of 128 query rows, key head).
+//
+//   o_r = sum_j softmax_j(scale q_r . k_j) v_j,   j <= position of r (causal) or every key
+//
+// A query "row" is a (token, query head of the key head's group) pair, token-major: the G = Hq / Hkv
+// heads that share keys share the key / value tiles too, whatever G is.  Wavefront w owns rows 32 w ..
+// 32 w + 31 of the tile, one row per lane pair (l, l + 32): S^T = K Q^T leaves a row's scores in the
+// registers of its lane pair, the softmax needs one exchange between the two halves, and S^T's
+// registers are the operand of O^T = V^T P^T as they stand (attention_tile.h).  K and V go through two
+// LDS buffers, the next tile's global loads being in flight during this tile's products: one barrier
+// per tile.  Running maximum, sum and output stay in fp32; the output is rescaled only when the running
+// maximum grows by more than 2^8 (the weights are then at most 2^8, exact to the same relative error).
+#ifndef APS_AMD_ATTENTION_ROWS_H_
+#define APS_AMD_ATTENTION_ROWS_H_
+
+#include "attention_tile.h"
+
+namespace aps {
+namespace att {
+
+struct RowsArgs {
+  const void *q, *k, *v;  // packed: k, v [total, Hkv, D] by strides; paged: pages [P, page, Hkv, D]
+  void* out;              // [total, Hq, D]
+  float* lse;             // [total, Hq] log2 of the softmax sum, +inf for a row that sees nothing; or null
+  Index cu;               // [N + 1]
+  Index kv_lens;          // paged: [N] keys of each sequence, its new tokens included
+  const int32_t* table;   // paged: [N, table_stride]
+  int64_t table_stride;
+  int64_t total, N, tiles;
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h;  // strides in elements (paged: of a slot, of a head)
+  int64_t num_pages, max_keys;           // paged
+  int32_t page_shift;                    // paged: log2 of the page size
+  int32_t G, Hkv;
+  int32_t causal, zero_tail;
+  float c;                // scale * log2(e) > 0
+  // split over the keys (paged): partial results [split][total * Hq]{D floats} and {max, sum}
+  float* part_o;
+  float* part_ml;
+  int32_t splits;
+};
+
+template <typename T>
+constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
+constexpr int kRowTile = 128;
+
+// Rows of no sequence (behind the last one; before the first, if cu_seqlens does not begin at 0) are
+// cleared, by the workgroups that have no tile: number `first` of `step` of them
+template <typename T, int D>
+__device__ __forceinline__ void clear_rows(T* out, const Index& cu, int64_t N, int64_t total, int H, int64_t first,
+                                           int64_t step) {
+  int64_t lead, unused;
+  seq_range(cu, 0, total, lead, unused);
+  const int64_t tail = max(tail_of(cu, N, total), lead);
+  for (int64_t i = first; i < lead + total - tail; i += step) {
+    T* row = out + (i < lead ? i : tail + i - lead) * (int64_t)H * D;
+    for (int i = threadIdx.x; i < H * D / chunk_elems<T>(); i += blockDim.x)
+      reinterpret_cast<u32x4*>(row)[i] = u32x4{0, 0, 0, 0};
+  }
+}
+
+// one tile of keys / values on its way from global memory to LDS: thread t carries chunk t % CH of rows
+// t / CH + i * (256 / CH); rows outside [0, end) are zeros, so nothing that lies there (an unwritten
+// page, the next sequence) can reach a product
+template <typename T, int D, bool PAGED>
+struct KvStage {
+  static constexpr int CH = D / chunk_elems<T>(), BK = key_tile<T>(), PER = BK * CH / 256, STEP = 256 / CH;
+  u32x4 kr[PER], vr[PER];
+  uint32_t gone;  // paged: bit i: row i's page is outside the cache
+
+  __device__ __forceinline__ void load(const RowsArgs& a, int64_t start, int seq, int h, int key0, int end) {
+    const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+    gone = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int key = key0 + r0 + i * STEP;
+      kr[i] = u32x4{0, 0, 0, 0};
+      vr[i] = u32x4{0, 0, 0, 0};
+      if (key >= end) continue;
+      int64_t row;
+      if constexpr (PAGED) {
+        const int32_t p = a.table[(int64_t)seq * a.table_stride + (key >> a.page_shift)];
+        if (p < 0 || p >= a.num_pages) {
+          gone |= 1u << i;
+          continue;
+        }
+        row = ((int64_t)p << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+      } else {
+        row = start + key;
+      }
+      kr[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.k) + row * a.k_t + h * a.k_h +
+                                              c * chunk_elems<T>());
+      vr[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.v) + row * a.v_t + h * a.v_h +
+                                              c * chunk_elems<T>());
+    }
+  }
+  __device__ __forceinline__ void store(char* tk, char* tv, uint8_t* hidden) const {
+    const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (PAGED && c == 0) hidden[r0 + i * STEP] = (gone >> i) & 1;
+      const int at = tile_at<T, D>(r0 + i * STEP, c);
+      *reinterpret_cast<u32x4*>(tk + at) = kr[i];
+      *reinterpret_cast<u32x4*>(tv + at) = vr[i];
+    }
+  }
+};
+
+template <typename T, int D, bool PAGED>
+__global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void attention_rows_kernel(RowsArgs a) {
+  constexpr int BK = key_tile<T>(), KS = 2 * chunk_elems<T>(), NS = D / KS, NKB = BK / 32, NDB = D / 32;
+  constexpr int NPS = 32 / KS, TILE = BK * D * (int)sizeof(T);
+  __shared__ __align__(16) char lds[4 * TILE];
+  __shared__ uint8_t s_hidden[2][64];  // paged: keys without a page
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, half = lane >> 5;
+  const int h = blockIdx.x % a.Hkv;
+  // the last tiles of a sequence see the most keys: they go first
+  const int64_t want = a.tiles - 1 - blockIdx.x / a.Hkv;
+  const SeqTile t = find_tile(a.cu, a.N, a.total, a.G, kRowTile, want, lane);
+  const int Hq = a.Hkv * a.G;
+  if (t.seq < 0) {
+    if (a.zero_tail && h == 0 && blockIdx.y == 0)
+      clear_rows<T, D>(static_cast<T*>(a.out), a.cu, a.N, a.total, Hq, want - t.used, a.tiles - t.used);
+    return;
+  }
+  int kv = t.len;
+  if constexpr (PAGED) {
+    const int64_t n = a.kv_lens.at(t.seq);
+    kv = (int)(n < 0 ? 0 : (n > a.max_keys ? a.max_keys : n));
+  }
+  const int off = kv - t.len;  // position of the sequence's first query
+  const int rows = t.len * a.G;
+  const int row0 = t.tile * kRowTile + wv * 32;
+  const int row = row0 + (lane & 31);
+  const bool live = row < rows;
+  const int tok = live ? row / a.G : 0, head = h * a.G + (live ? row - tok * a.G : 0);
+  const int pos = live ? (a.causal ? off + tok : kv - 1) : -1;
+  // keys the tile / the wavefront can see; the least position in the wavefront (no mask below it)
+  const int tile_last = min(t.tile * kRowTile + kRowTile, rows) - 1;
+  const int last = min(row0 + 32, rows) - 1;
+  int end = kv, wave_end = kv, wave_min = kv - 1;
+  if (a.causal) {
+    end = min(kv, off + tile_last / a.G + 1);
+    wave_end = row0 < rows ? min(kv, off + last / a.G + 1) : 0;
+    wave_min = off + row0 / a.G;
+  } else if (row0 >= rows) {
+    wave_end = 0;
+  }
+  const T* qp = static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + head * a.q_h;
+  u32x4 qf[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s)
+    qf[s] = live ? *reinterpret_cast<const u32x4*>(qp + (2 * s + half) * chunk_elems<T>()) : u32x4{0, 0, 0, 0};
+
+  int tile_lo = 0, tile_hi = (max(end, 0) + BK - 1) / BK;
+  if constexpr (PAGED) {
+    if (a.splits > 1) {
+      const int per = (tile_hi + a.splits - 1) / a.splits;
+      tile_lo = min(tile_hi, per * (int)blockIdx.y);
+      tile_hi = min(tile_hi, tile_lo + per);
+    }
+  }
+  f32x16 acc[NDB];
+#pragma unroll
+  for (int d = 0; d < NDB; ++d) acc[d] = f32x16{0};
+  float m = -INFINITY, l = 0.f;  // m: the reference the weights are taken against, in units of log2
+
+  KvStage<T, D, PAGED> st;
+  if (tile_lo < tile_hi) {
+    st.load(a, t.start, t.seq, h, tile_lo * BK, end);
+    st.store(lds, lds + TILE, s_hidden[0]);
+  }
+  __syncthreads();
+  for (int kt = tile_lo; kt < tile_hi; ++kt) {
+    const char* tk = lds + ((kt - tile_lo) & 1) * 2 * TILE;
+    const char* tv = tk + TILE;
+    char* nk = lds + ((kt - tile_lo + 1) & 1) * 2 * TILE;
+    const bool more = kt + 1 < tile_hi;
+    if (more) st.load(a, t.start, t.seq, h, (kt + 1) * BK, end);
+    const int k0 = kt * BK;
+    if (k0 < wave_end) {
+      f32x16 s[NKB];
+#pragma unroll
+      for (int b = 0; b < NKB; ++b) s[b] = f32x16{0};
+#pragma unroll
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int b = 0; b < NKB; ++b) s[b] = mma<T>(frag<T, D>(tk, b * 32 + (lane & 31), i, half), qf[i], s[b]);
+      if (k0 + BK - 1 > wave_min) {
+#pragma unroll
+        for (int b = 0; b < NKB; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (k0 + b * 32 + result_row(i, half) > pos) s[b][i] = -INFINITY;
+      }
+      if constexpr (PAGED) {
+        const uint64_t hidden = __ballot(lane < BK && s_hidden[(kt - tile_lo) & 1][lane]);
+        if (hidden) {
+#pragma unroll
+          for (int b = 0; b < NKB; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if ((hidden >> (b * 32 + result_row(i, half))) & 1) s[b][i] = -INFINITY;
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < NKB; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+      top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
+      if (__any(top > m + 8.f)) {
+        const float to = fmaxf(m, top);
+        const float f = to == -INFINITY ? 1.f : exp2_fast(m - to);
+        m = to;
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < NDB; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[d][i] *= f;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int b = 0; b < NKB; ++b) {
+        float p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          p[i] = exp2_fast(fmaf(s[b][i], a.c, -ref));
+          l += p[i];
+        }
+#pragma unroll
+        for (int i = 0; i < NPS; ++i) {
+          const u32x4 pf = pack<T>(p + i * (KS / 2));
+#pragma unroll
+          for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(frag_t<T, D>(tv, b * 32, i, d, lane), pf, acc[d]);
+        }
+      }
+    }
+    if (more) st.store(nk, nk + TILE, s_hidden[(kt - tile_lo + 1) & 1]);
+    __syncthreads();
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!live) return;
+  const int64_t at = (t.start + tok) * Hq + head;
+  if constexpr (PAGED) {
+    if (a.splits > 1) {  // unnormalised; combined by attention_combine_kernel
+      const int64_t slot = (int64_t)blockIdx.y * a.total * Hq + at;
+      float* po = a.part_o + slot * D;
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4)
+          store4<float>(po + d * 32 + result_row(i, half), f32x4{acc[d][i], acc[d][i + 1], acc[d][i + 2], acc[d][i + 3]});
+      if (half == 0) *reinterpret_cast<float2*>(a.part_ml + slot * 2) = make_float2(m, l);
+      return;
+    }
+  }
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  T* po = static_cast<T*>(a.out) + at * D;
+#pragma unroll
+  for (int d = 0; d < NDB; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4)
+      store4<T>(po + d * 32 + result_row(i, half),
+                f32x4{acc[d][i] * inv, acc[d][i + 1] * inv, acc[d][i + 2] * inv, acc[d][i + 3] * inv});
+  if (a.lse && half == 0) a.lse[at] = l > 0.f ? m + log2_fast(l) : (l != l ? l : INFINITY);
+}
+
+// sizes every attention entry point takes: rows of a sequence are counted in 32 bits (token x head of
+// the group), the grid in 31
+static inline bool sizes_fit(int64_t total, int64_t N, int64_t Hq, int64_t Hkv) {
+  if (total < 0 || N < 1 || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq > 65536) return false;
+  if (total > (int64_t)0x7fff0000 / (Hq / Hkv)) return false;
+  return ((total * (Hq / Hkv) + kRowTile - 1) / kRowTile + N + 1) * Hkv < 0x7fffffff;
+}
+
+static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace att
+}  // namespace aps
+
+#define APS_ATT_DISPATCH(FN, ...)                                                                      \
+  if (dtype == kTypeF32 && head_dim == 32) FN<float, 32>(__VA_ARGS__);                                 \
+  else if (dtype == kTypeF32 && head_dim == 64) FN<float, 64>(__VA_ARGS__);                            \
+  else if (dtype == kTypeF32 && head_dim == 128) FN<float, 128>(__VA_ARGS__);                          \
+  else if (dtype == kTypeBf16 && head_dim == 32) FN<__bf16, 32>(__VA_ARGS__);                          \
+  else if (dtype == kTypeBf16 && head_dim == 64) FN<__bf16, 64>(__VA_ARGS__);                          \
+  else if (dtype == kTypeBf16 && head_dim == 128) FN<__bf16, 128>(__VA_ARGS__);                        \
+  else if (dtype == kTypeF16 && head_dim == 32) FN<_Float16, 32>(__VA_ARGS__);                         \
+  else if (dtype == kTypeF16 && head_dim == 64) FN<_Float16, 64>(__VA_ARGS__);                         \
+  else if (dtype == kTypeF16 && head_dim == 128) FN<_Float16, 128>(__VA_ARGS__);                       \
+  else return APS_ERR_UNSUPPORTED
+
+#endif  // APS_AMD_ATTENTION_ROWS_H_

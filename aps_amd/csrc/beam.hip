@@ -1,0 +1,461 @@
+// One step of a beam search: the best K continuations of B hypotheses over a vocabulary of V, for N
+// utterances at once, and the reordering of the decoder's states.
+//
+//   total[n, b, v] = score[n, b] + x[n, b, v] - log sum_v' exp(x[n, b, v'])
+//
+// The K largest of B V, ties to the lowest b V + v.  A hypothesis' own K largest logits hold every one
+// of its candidates that can be selected, so the logits are read ONCE: a workgroup takes up to 8 192 of a
+// row into registers, forms their maximum, their sum of exponentials and their K largest
+// (`beam_rows_kernel`); a workgroup per utterance merges the B * splits * K candidates
+// (`beam_merge_kernel`).  Sum and totals are in 64 bits: two candidates may lie closer than the
+// rounding of a 32-bit log-softmax, and the order must not depend on how the sum was cut.
+#include "common.h"
+
+namespace aps {
+namespace beam {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kThreads = 256, kPerThread = 32, kTile = kThreads * kPerThread;  // elements of a workgroup
+constexpr int kMaxBeam = 64, kCandidates = 1024;
+constexpr float kLargest = 3.4028234663852886e38f;
+
+// e^x for x <= 0 in 64 bits, relative error < 1e-12 (2^f by its series to f^10, |f| <= 1/2)
+__device__ __forceinline__ double exp64(double x) {
+  const double y = x * 1.4426950408889634074;
+  const double n = rint(y), f = y - n;
+  double p = 7.0549116208011233e-9;
+  p = fma(p, f, 1.0178086009239699e-7);
+  p = fma(p, f, 1.3215486790144309e-6);
+  p = fma(p, f, 1.5252733804059840e-5);
+  p = fma(p, f, 1.5403530393381609e-4);
+  p = fma(p, f, 1.3333558146428443e-3);
+  p = fma(p, f, 9.6181291076284772e-3);
+  p = fma(p, f, 5.5504108664821580e-2);
+  p = fma(p, f, 2.4022650695910071e-1);
+  p = fma(p, f, 6.9314718055994531e-1);
+  p = fma(p, f, 1.0);
+  return ldexp(p, n < -2000. ? -2000 : (int)n);
+}
+
+// order-preserving integers: larger value, larger integer
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float from_ordered(uint32_t u) {
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+__device__ __forceinline__ uint64_t ordered(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  return (u >> 63) ? ~u : (u | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double from_ordered(uint64_t u) {
+  return __longlong_as_double((long long)((u >> 63) ? (u & 0x7fffffffffffffffull) : ~u));
+}
+
+// the K-th largest of a wavefront's 64 values (bitonic sort, descending), K in 1 .. 64
+template <typename V>
+__device__ __forceinline__ V wave_kth(V v, int K, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 64; size <<= 1)
+#pragma unroll
+    for (int step = size >> 1; step > 0; step >>= 1) {
+      const V o = __shfl_xor(v, step, 64);
+      const bool lower = (lane & step) == 0, descending = (lane & size) == 0;
+      v = (lower == descending) ? (v > o ? v : o) : (v > o ? o : v);
+    }
+  return __shfl(v, K - 1, 64);
+}
+
+struct RowsArgs {
+  const void* x;
+  int64_t stride;          // elements between rows
+  const float* score;      // [N B]
+  const uint8_t* done;     // [N B] or null
+  uint64_t* keys;          // [N B][splits][K]: ordered(x) << 32 | ~token, 0 = none
+  float* top;              // [N B][splits]
+  double* sum;             // [N B][splits]
+  int64_t eos;
+  int32_t V, K, splits;
+};
+
+template <typename T>
+__device__ __forceinline__ void widen(u32x4 raw, float* to) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 v = __builtin_bit_cast(f32x4, raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = v[i];
+  } else if constexpr (__is_same(T, __bf16)) {
+    const bf16x8 v = __builtin_bit_cast(bf16x8, raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) to[i] = (float)v[i];
+  } else {
+    const f16x8 v = __builtin_bit_cast(f16x8, raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) to[i] = (float)v[i];
+  }
+}
+
+// NaN counts as ruled out, +inf as the largest finite value, -0 as 0 (they tie)
+__device__ __forceinline__ float tame(float x) { return x != x ? -INFINITY : fminf(x, kLargest) + 0.f; }
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
+  constexpr int VE = 16 / (int)sizeof(T), NV = kPerThread / VE;
+  __shared__ uint64_t s_cand[kCandidates];
+  __shared__ double s_sum[4];
+  __shared__ float s_top[4], s_kth[4];
+  __shared__ uint64_t s_best[4];
+  __shared__ int s_count;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int64_t row = blockIdx.x;
+  const int split = blockIdx.y, V = a.V, K = a.K;
+  uint64_t* out = a.keys + (row * a.splits + split) * K;
+  if (tid == 0) s_count = 0;
+  const bool done = a.done && a.done[row];
+  const bool dead = !(a.score[row] > -INFINITY);  // (NaN too)
+  // aligned vectors: element e0 + i of the row; the first vector may begin before the row
+  const T* base = static_cast<const T*>(a.x) + row * a.stride;
+  const int shift = (int)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
+  float x[kPerThread];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int e0 = (split * (kTile / VE) + j * kThreads + tid) * VE - shift;
+    float* to = x + j * VE;
+    if (done || dead) {
+#pragma unroll
+      for (int i = 0; i < VE; ++i) to[i] = (done && !dead && e0 + i == a.eos) ? 0.f : -INFINITY;
+    } else if (e0 >= 0 && e0 + VE <= V) {
+      widen<T>(*reinterpret_cast<const u32x4*>(base + e0), to);
+#pragma unroll
+      for (int i = 0; i < VE; ++i) to[i] = tame(to[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        to[i] = (e0 + i >= 0 && e0 + i < V) ? tame((float)base[e0 + i]) : -INFINITY;
+    }
+  }
+  float best = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < kPerThread; ++i) best = fmaxf(best, x[i]);
+  const float kth = wave_kth(best, K, lane), wtop = wave_max(best);
+  if (lane == 0) s_top[wv] = wtop, s_kth[wv] = kth;
+  __syncthreads();
+  const float top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+  // K of the threads' maxima are at least `least`, so the K largest elements are too
+  const float least = fmaxf(fmaxf(s_kth[0], s_kth[1]), fmaxf(s_kth[2], s_kth[3]));
+  double sum = 0.;
+  if (top > -INFINITY) {
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i)
+      if (x[i] > -INFINITY) sum += exp64((double)x[i] - (double)top);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  if (lane == 0) s_sum[wv] = sum;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int e0 = (split * (kTile / VE) + j * kThreads + tid) * VE - shift;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      if (x[j * VE + i] >= least && e0 + i >= 0 && e0 + i < V) {
+        const int at = atomicAdd(&s_count, 1);  // (the order of arrival does not matter: ranked below)
+        if (at < kCandidates) s_cand[at] = ((uint64_t)ordered(x[j * VE + i]) << 32) | (uint32_t)~(e0 + i);
+      }
+    }
+  }
+  __syncthreads();
+  const int count = s_count;
+  if (tid == 0) {
+    a.top[row * a.splits + split] = top;
+    a.sum[row * a.splits + split] = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+  }
+  if (count <= kCandidates) {
+    for (int c = tid; c < count; c += kThreads) {
+      const uint64_t key = s_cand[c];
+      int rank = 0;
+      for (int o = 0; o < count; ++o) rank += s_cand[o] > key;
+      if (rank < K) out[rank] = key;
+    }
+    for (int c = count + tid; c < K; c += kThreads) out[c] = 0;  // fewer elements than K
+    return;
+  }
+  // a great many equal values: K rounds of the largest key below the last
+  uint64_t last = ~0ull;
+  for (int k = 0; k < K; ++k) {
+    uint64_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int e0 = (split * (kTile / VE) + j * kThreads + tid) * VE - shift;
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        if (e0 + i < 0 || e0 + i >= V) continue;
+        const uint64_t key = ((uint64_t)ordered(x[j * VE + i]) << 32) | (uint32_t)~(e0 + i);
+        if (key < last && key > mine) mine = key;
+      }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint64_t other = __shfl_xor(mine, o, 64);
+      mine = other > mine ? other : mine;
+    }
+    if (lane == 0) s_best[wv] = mine;
+    __syncthreads();
+    last = s_best[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) last = s_best[w] > last ? s_best[w] : last;
+    if (tid == 0) out[k] = last;
+    __syncthreads();
+  }
+}
+
+struct MergeArgs {
+  const uint64_t* keys;
+  const float* top;
+  const double* sum;
+  const float* score;
+  const uint8_t* done;
+  float* new_score;     // [N, K]
+  int64_t *parent, *token;
+  uint8_t* new_done;
+  int64_t eos;
+  int32_t B, V, K, splits;
+};
+
+__global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
+  __shared__ uint64_t s_key[kCandidates];
+  __shared__ uint32_t s_flat[kCandidates];
+  __shared__ double s_add[kMaxBeam];  // score - log sum exp of a hypothesis
+  __shared__ double s_score[kMaxBeam];
+  __shared__ uint64_t s_kth[4], s_best[4];
+  __shared__ uint32_t s_best_flat[4];
+  __shared__ int s_count;
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int64_t n = blockIdx.x;
+  const int B = a.B, K = a.K, S = a.splits;
+  if (tid == 0) s_count = 0;
+  if (tid < B) {
+    const int64_t row = n * B + tid;
+    float top = -INFINITY;
+    for (int s = 0; s < S; ++s) top = fmaxf(top, a.top[row * S + s]);
+    double sum = 0.;
+    if (top > -INFINITY)
+      for (int s = 0; s < S; ++s)
+        if (a.top[row * S + s] > -INFINITY)
+          sum += a.sum[row * S + s] * exp64((double)a.top[row * S + s] - (double)top);
+    s_add[tid] = top > -INFINITY ? (double)top + log(sum) : 0.;
+    s_score[tid] = (double)tame(a.score[row]);
+  }
+  __syncthreads();
+  const uint64_t* keys = a.keys + n * B * S * K;
+  const int total = B * S * K;
+  // candidate c of the utterance: its total as an ordered integer (0: none) and its flat index
+  auto candidate = [&](int c, uint32_t& flat) -> uint64_t {
+    const uint64_t key = keys[c];
+    if (!key) return 0;
+    const int b = c / (S * K);
+    const uint32_t token = ~(uint32_t)key;
+    flat = (uint32_t)b * (uint32_t)a.V + token;
+    const float x = from_ordered((uint32_t)(key >> 32));
+    return ordered(x > -INFINITY ? s_score[b] + ((double)x - s_add[b]) + 0. : (double)-INFINITY);
+  };
+  uint64_t best = 0;
+  for (int c = tid; c < total; c += kThreads) {
+    uint32_t flat;
+    const uint64_t v = candidate(c, flat);
+    best = v > best ? v : best;
+  }
+  const uint64_t kth = wave_kth(best, K, lane);
+  if (lane == 0) s_kth[wv] = kth;
+  __syncthreads();
+  uint64_t least = s_kth[0];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) least = s_kth[w] > least ? s_kth[w] : least;
+  if (least == 0) least = 1;  // (0 is no candidate)
+  for (int c = tid; c < total; c += kThreads) {
+    uint32_t flat;
+    const uint64_t v = candidate(c, flat);
+    if (v >= least) {
+      const int at = atomicAdd(&s_count, 1);
+      if (at < kCandidates) s_key[at] = v, s_flat[at] = flat;
+    }
+  }
+  __syncthreads();
+  const int count = s_count;
+  auto put = [&](int rank, uint64_t v, uint32_t flat) {
+    const int64_t b = flat / (uint32_t)a.V, token = flat % (uint32_t)a.V;
+    const int64_t at = n * K + rank;
+    a.new_score[at] = (float)from_ordered(v);
+    a.parent[at] = b;
+    a.token[at] = token;
+    a.new_done[at] = (a.done && a.done[n * B + b]) || token == a.eos;
+  };
+  if (count <= kCandidates) {
+    for (int c = tid; c < count; c += kThreads) {
+      const uint64_t v = s_key[c];
+      const uint32_t flat = s_flat[c];
+      int rank = 0;
+      for (int o = 0; o < count; ++o) rank += s_key[o] > v || (s_key[o] == v && s_flat[o] < flat);
+      if (rank < K) put(rank, v, flat);
+    }
+    return;
+  }
+  uint64_t last = ~0ull;
+  uint32_t last_flat = 0;
+  for (int k = 0; k < K; ++k) {
+    uint64_t mine = 0;
+    uint32_t mine_flat = 0;
+    for (int c = tid; c < total; c += kThreads) {
+      uint32_t flat = 0;
+      const uint64_t v = candidate(c, flat);
+      if (!v || !(v < last || (v == last && flat > last_flat))) continue;
+      if (v > mine || (v == mine && flat < mine_flat)) mine = v, mine_flat = flat;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      const uint64_t v = __shfl_xor(mine, o, 64);
+      const uint32_t flat = __shfl_xor(mine_flat, o, 64);
+      if (v > mine || (v == mine && flat < mine_flat)) mine = v, mine_flat = flat;
+    }
+    if (lane == 0) s_best[wv] = mine, s_best_flat[wv] = mine_flat;
+    __syncthreads();
+    last = s_best[0], last_flat = s_best_flat[0];
+#pragma unroll
+    for (int w = 1; w < 4; ++w)
+      if (s_best[w] > last || (s_best[w] == last && s_best_flat[w] < last_flat)) last = s_best[w], last_flat = s_best_flat[w];
+    if (tid == 0) put(k, last, last_flat);
+    __syncthreads();
+  }
+}
+
+// ---- states: row n K + k of a result is row n B + parent[n, k] of its source, for several tensors in
+// one launch.  A tensor is [outer, rows, inner bytes]; a parent outside [0, B) gives zeros.
+constexpr int kStates = 16, kUnits = 4;  // tensors a launch, units a thread
+struct ReorderArgs {
+  const char* src[kStates];
+  char* dst[kStates];
+  uint32_t unit[kStates];    // bytes a thread moves at once: 16, 8, 4, 2 or 1
+  uint32_t inner[kStates];   // units a row
+  int64_t units[kStates];    // outer * N * K * inner
+  int64_t first[kStates];    // first block
+  const int64_t* parent;
+  uint32_t rows_in, rows_out, B, K;  // N B, N K
+  int32_t count;
+};
+
+template <typename U>
+__device__ __forceinline__ void move_units(const ReorderArgs& a, int s, int64_t i0) {
+  U v[kUnits];
+  int64_t at[kUnits];
+#pragma unroll
+  for (int j = 0; j < kUnits; ++j) {
+    const int64_t i = i0 + j * 256;
+    at[j] = i < a.units[s] ? i : -1;
+    v[j] = U{};
+    if (at[j] < 0) continue;
+    const uint64_t flat = (uint64_t)i / a.inner[s];
+    const uint32_t col = (uint32_t)((uint64_t)i - flat * a.inner[s]);
+    const uint64_t outer = flat / a.rows_out;
+    const uint32_t row = (uint32_t)(flat - outer * a.rows_out);
+    const uint32_t n = row / a.K;
+    const int64_t p = a.parent[row];
+    if (p < 0 || p >= a.B) continue;
+    v[j] = reinterpret_cast<const U*>(a.src[s])[(outer * a.rows_in + (uint64_t)n * a.B + p) * a.inner[s] + col];
+  }
+#pragma unroll
+  for (int j = 0; j < kUnits; ++j)
+    if (at[j] >= 0) reinterpret_cast<U*>(a.dst[s])[at[j]] = v[j];
+}
+
+__global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
+  int s = 0;
+  while (s + 1 < a.count && (int64_t)blockIdx.x >= a.first[s + 1]) ++s;
+  const int64_t i0 = ((int64_t)blockIdx.x - a.first[s]) * (256 * kUnits) + threadIdx.x;
+  switch (a.unit[s]) {
+    case 16: move_units<u32x4>(a, s, i0); break;
+    case 8: move_units<uint64_t>(a, s, i0); break;
+    case 4: move_units<uint32_t>(a, s, i0); break;
+    case 2: move_units<uint16_t>(a, s, i0); break;
+    default: move_units<uint8_t>(a, s, i0); break;
+  }
+}
+
+static int64_t splits_of(int64_t V, int64_t elem) { return (V + 16 / elem - 1 + kTile - 1) / kTile; }
+static bool sizes_fit(int64_t N, int64_t B, int64_t V, int64_t K) {
+  return N >= 1 && B >= 1 && B <= kMaxBeam && K >= 1 && K <= kMaxBeam && V >= 1 && V <= (1 << 24) &&
+         K <= B * V && N <= 0x7fffffff / B;
+}
+
+}  // namespace beam
+}  // namespace aps
+
+using namespace aps::beam;
+
+extern "C" int64_t aps_beam_select_workspace(int64_t N, int64_t B, int64_t V, int64_t K) {
+  if (!sizes_fit(N, B, V, K)) return -1;
+  return N * B * splits_of(V, 2) * (K * 8 + 16);  // (16-bit logits may begin a vector later: their count)
+}
+
+extern "C" int aps_beam_select(const void* logits, int64_t row_stride, const float* scores, const uint8_t* finished,
+                               int64_t eos, float* new_scores, int64_t* parent, int64_t* token,
+                               uint8_t* new_finished, int64_t N, int64_t B, int64_t V, int64_t K, int32_t dtype,
+                               void* workspace, void* stream) {
+  APS_CHECK_ARG(logits && scores && new_scores && parent && token && new_finished && workspace);
+  APS_CHECK_ARG(sizes_fit(N, B, V, K) && row_stride >= V && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
+  APS_CHECK_ARG(!finished || (eos >= 0 && eos < V));
+  if (dtype < 0 || dtype > 2) return APS_ERR_UNSUPPORTED;
+  const int64_t elem = dtype == 0 ? 4 : 2, S = splits_of(V, elem);
+  APS_CHECK_ARG((reinterpret_cast<uintptr_t>(logits) & (elem - 1)) == 0);
+  RowsArgs r{};
+  r.x = logits, r.stride = row_stride, r.score = scores, r.done = finished, r.eos = eos;
+  r.V = (int32_t)V, r.K = (int32_t)K, r.splits = (int32_t)S;
+  r.keys = static_cast<uint64_t*>(workspace);
+  r.sum = reinterpret_cast<double*>(r.keys + N * B * S * K);
+  r.top = reinterpret_cast<float*>(r.sum + N * B * S);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(N * B), (unsigned)S);
+  if (dtype == 0) hipLaunchKernelGGL(beam_rows_kernel<float>, grid, dim3(kThreads), 0, st, r);
+  else if (dtype == 1) hipLaunchKernelGGL(beam_rows_kernel<__bf16>, grid, dim3(kThreads), 0, st, r);
+  else hipLaunchKernelGGL(beam_rows_kernel<_Float16>, grid, dim3(kThreads), 0, st, r);
+  if (aps_launch_status() != APS_OK) return APS_ERR_LAUNCH;
+  MergeArgs m{};
+  m.keys = r.keys, m.top = r.top, m.sum = r.sum, m.score = scores, m.done = finished, m.eos = eos;
+  m.new_score = new_scores, m.parent = parent, m.token = token, m.new_done = new_finished;
+  m.B = (int32_t)B, m.V = (int32_t)V, m.K = (int32_t)K, m.splits = (int32_t)S;
+  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)N), dim3(kThreads), 0, st, m);
+  return aps_launch_status();
+}
+
+extern "C" int aps_beam_reorder(const void* const* src, void* const* dst, const int64_t* outer,
+                                const int64_t* inner_bytes, int64_t count, const int64_t* parent, int64_t N,
+                                int64_t K, int64_t B, void* stream) {
+  APS_CHECK_ARG(src && dst && outer && inner_bytes && parent && count >= 0 && N >= 1 && K >= 1 && B >= 1);
+  APS_CHECK_ARG(N <= 0x7fffffff / K && N <= 0x7fffffff / B);
+  for (int64_t s0 = 0; s0 < count; s0 += kStates) {
+    ReorderArgs a{};
+    int64_t blocks = 0;
+    for (int64_t s = s0; s < count && s < s0 + kStates; ++s) {
+      APS_CHECK_ARG(outer[s] >= 0 && inner_bytes[s] >= 0);
+      if (outer[s] == 0 || inner_bytes[s] == 0) continue;
+      APS_CHECK_ARG(src[s] && dst[s] && inner_bytes[s] < 0x7fffffff);
+      const uintptr_t at = reinterpret_cast<uintptr_t>(src[s]) | reinterpret_cast<uintptr_t>(dst[s]) | (uintptr_t)inner_bytes[s];
+      const int i = a.count++;
+      a.unit[i] = at & 1 ? 1 : (at & 3 ? 2 : (at & 7 ? 4 : (at & 15 ? 8 : 16)));
+      a.src[i] = static_cast<const char*>(src[s]), a.dst[i] = static_cast<char*>(dst[s]);
+      a.inner[i] = (uint32_t)(inner_bytes[s] / a.unit[i]);
+      a.units[i] = outer[s] * N * K * a.inner[i];
+      a.first[i] = blocks;
+      blocks += (a.units[i] + 256 * kUnits - 1) / (256 * kUnits);
+    }
+    if (!a.count) continue;
+    APS_CHECK_ARG(blocks < 0x7fffffff);
+    a.parent = parent, a.rows_in = (uint32_t)(N * B), a.rows_out = (uint32_t)(N * K), a.B = (uint32_t)B, a.K = (uint32_t)K;
+    hipLaunchKernelGGL(beam_reorder_kernel, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    if (aps_launch_status() != APS_OK) return APS_ERR_LAUNCH;
+  }
+  return APS_OK;
+}

@@ -618,6 +618,44 @@ class AttentionCrossFn(th.autograd.Function):
         return g_q, g_kv, None, None, None, None, None
 
 
+class AttentionPackedFn(th.autograd.Function):
+    """nn_ops.attention_packed with its adjoint (aps_attention_packed_backward): the forward keeps the
+    softmax sums, the backward forms the weights again from them, a tile at a time"""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, causal, scale):
+        from aps_amd import nn_ops
+        q, k, v = (nn_ops._strided16(t.detach()) for t in (q, k, v))
+        out, sums = nn_ops.attention_packed_forward(q, k, v, cu_seqlens, causal, scale, lse=True)
+        ctx.save_for_backward(q, k, v, out, sums, cu_seqlens)
+        ctx.cfg = (causal, scale)
+        return out
+
+    @staticmethod
+    @th.autograd.function.once_differentiable
+    def backward(ctx, g):
+        from aps_amd import nn_ops
+        q, k, v, out, sums, cu_seqlens = ctx.saved_tensors
+        causal, scale = ctx.cfg
+        lib = nat.load()
+        T, Hq, D = q.shape
+        Hkv = k.shape[1]
+        g = nn_ops._strided16(g)
+        g_q = th.empty(q.shape, device=q.device, dtype=q.dtype)
+        g_k, g_v = (th.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
+        if T:
+            ws = th.empty(lib.aps_attention_packed_backward_workspace(T, Hq), device=q.device, dtype=th.uint8)
+            with nat.on_device_of(q):
+                rc = lib.aps_attention_packed_backward(
+                    q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(), sums.data_ptr(),
+                    cu_seqlens.data_ptr(), int(cu_seqlens.dtype == th.int64), g_q.data_ptr(), g_k.data_ptr(),
+                    g_v.data_ptr(), T, cu_seqlens.shape[0] - 1, Hq, Hkv, D, q.stride(0), q.stride(1), k.stride(0),
+                    k.stride(1), v.stride(0), v.stride(1), g.stride(0), g.stride(1), nn_ops.ELEMENT_TYPES[q.dtype],
+                    int(causal), scale, ws.data_ptr(), nat.stream_of(q))
+            nat.check(rc, "aps_attention_packed_backward")
+        return g_q, g_k, g_v, None, None, None
+
+
 class EmbeddingPosencFn(th.autograd.Function):
     """table[ids] * factor + sinusoid (aps_embedding_posenc: the decoder's token embedding) with the
     adjoint w.r.t. the table: the lookups sorted by token (index plumbing: torch.sort), the rows of

@@ -2,9 +2,11 @@
 Launchers for the encoder kernels (aps_amd/csrc/nn.hip): host-side argument marshalling only.
 Activations are batch-major [N, T, D] / [rows, D], fp32, contiguous.
 """
+import math
 import os
+from ctypes import c_int64 as C_int64
 from ctypes import c_void_p as C_void_p
-from typing import Optional
+from typing import List, Optional, Sequence
 
 import torch as th
 
@@ -531,6 +533,296 @@ def attention_cross(q: th.Tensor, kv: th.Tensor, num_heads: int,
                                  D // num_heads, nat.stream_of(q))
     nat.check(rc, "aps_attention_cross")
     return ctx
+
+
+# ------------------------------------------------------------------------------------------------
+# Packed sequences, paged caches, beam search: f32 | bf16 | f16, grouped heads (aps_attention_packed,
+# aps_attention_paged, aps_beam_select)
+# ------------------------------------------------------------------------------------------------
+ELEMENT_TYPES = {th.float32: 0, th.bfloat16: 1, th.float16: 2}
+PACKED_HEAD_DIMS = (32, 64, 128)
+
+
+def _strided16(t: th.Tensor) -> th.Tensor:
+    """rows x heads x D as the kernels read it: the last axis contiguous, rows and heads anywhere on
+    16-byte boundaries (a slice of a fused projection is read in place); a copy of anything else"""
+    unit = 16 // t.element_size()
+    if t.stride(2) == 1 and t.stride(0) % unit == 0 and t.stride(1) % unit == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=th.contiguous_format)
+
+
+def _index_array(t: th.Tensor, what: str, length: Optional[int] = None) -> th.Tensor:
+    if t.dim() != 1 or t.dtype not in (th.int32, th.int64) or (length is not None and t.shape[0] != length):
+        want = "" if length is None else f" of {length}"
+        raise RuntimeError(f"{what} must be a 1-D int32 / int64 tensor{want}, got {tuple(t.shape)} {t.dtype}")
+    return t.contiguous()
+
+
+def _check_heads(what: str, q: th.Tensor, *kv: th.Tensor) -> None:
+    """q rows x Hq x D against the (rows | pages x page) x Hkv x D tensors it attends to"""
+    if q.dim() != 3 or q.dtype not in ELEMENT_TYPES:
+        raise RuntimeError(f"{what}: q must be rows x heads x head_dim in f32 / bf16 / f16, got "
+                           f"{tuple(q.shape)} {q.dtype}")
+    D = q.shape[2]
+    if D not in PACKED_HEAD_DIMS:
+        raise RuntimeError(f"{what}: head_dim {D} not in {PACKED_HEAD_DIMS}")
+    for t in kv:
+        if t.dtype != q.dtype:
+            raise RuntimeError(f"{what}: keys / values in {t.dtype}, q in {q.dtype}")
+        if t.shape != kv[0].shape or t.shape[-1] != D or t.shape[-2] < 1 or q.shape[1] < 1 or \
+                q.shape[1] % t.shape[-2]:
+            raise RuntimeError(f"{what}: keys / values {[tuple(x.shape) for x in kv]} do not fit q "
+                               f"{tuple(q.shape)} (the same head_dim, q's heads a multiple of theirs)")
+
+
+def _softmax_scale(what: str, scale: Optional[float], D: int) -> float:
+    scale = D**-0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise RuntimeError(f"{what}: scale must be positive and finite, got {scale}")
+    return scale
+
+
+def attention_packed(q: th.Tensor, k: th.Tensor, v: th.Tensor, cu_seqlens: th.Tensor, causal: bool = True,
+                     scale: Optional[float] = None) -> th.Tensor:
+    """Attention within each of N sequences packed end to end (no padding): q T x Hq x D, k / v T x Hkv x D
+    with Hq a multiple of Hkv (query head h reads key head h // (Hq // Hkv)), f32 | bf16 | f16, D 32 | 64 |
+    128 -> T x Hq x D.  cu_seqlens N + 1 (int32 | int64, on the device): sequence n is rows cu[n] ..
+    cu[n + 1] - 1; from 0, non-decreasing; rows behind cu[N] belong to no sequence and give zeros.
+    causal: a token sees its own sequence up to itself, else all of it; scale defaults to D ** -0.5.
+    q, k, v may be slices of one fused projection (read in place).  Differentiable in q, k and v
+    (aps_attention_packed_backward: the same bits on every run)."""
+    what = "attention_packed"
+    if k.dim() != 3 or v.dim() != 3 or k.shape[0] != q.shape[0]:
+        raise RuntimeError(f"{what}: k {tuple(k.shape)} / v {tuple(v.shape)} must be {q.shape[0]} x heads x head_dim")
+    _check_heads(what, q, k, v)
+    cu_seqlens = _index_array(cu_seqlens, f"{what}: cu_seqlens")
+    if cu_seqlens.shape[0] < 2:
+        raise RuntimeError(f"{what}: cu_seqlens holds the N + 1 bounds of N >= 1 sequences")
+    scale = _softmax_scale(what, scale, q.shape[2])
+    if nat.needs_grad(q, k, v):
+        from aps_amd.grad_ops import AttentionPackedFn
+        return AttentionPackedFn.apply(q, k, v, cu_seqlens, bool(causal), scale)
+    return attention_packed_forward(q, k, v, cu_seqlens, bool(causal), scale)[0]
+
+
+def attention_packed_forward(q, k, v, cu_seqlens, causal: bool, scale: float, lse: bool = False):
+    """the launch behind `attention_packed` -> (context, log2 of the softmax sums T x Hq | None)"""
+    nat.require_device(q, k, v, cu_seqlens)
+    lib = nat.load()
+    T, Hq, D = q.shape
+    q, k, v = _strided16(q), _strided16(k), _strided16(v)
+    out = th.empty(T, Hq, D, device=q.device, dtype=q.dtype)
+    sums = th.empty(T, Hq, device=q.device, dtype=th.float32) if lse else None
+    if T:
+        with nat.on_device_of(q):
+            rc = lib.aps_attention_packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(),
+                                          int(cu_seqlens.dtype == th.int64), out.data_ptr(),
+                                          None if sums is None else sums.data_ptr(), T, cu_seqlens.shape[0] - 1,
+                                          Hq, k.shape[1], D, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+                                          v.stride(0), v.stride(1), ELEMENT_TYPES[q.dtype], int(causal), scale,
+                                          nat.stream_of(q))
+        nat.check(rc, "aps_attention_packed")
+    return out, sums
+
+
+def _check_cache(what: str, rows: int, k_pages: th.Tensor, v_pages: th.Tensor, page_table: th.Tensor,
+                 cu_seqlens: th.Tensor, kv_lens: th.Tensor):
+    for t in (k_pages, v_pages):
+        if t.dim() != 4 or not t.is_contiguous() or t.data_ptr() % 16:
+            raise RuntimeError(f"{what}: a cache is a contiguous, 16-byte aligned pages x page x heads x head_dim "
+                               f"tensor, got {tuple(t.shape)} with strides {tuple(t.stride())}")
+    page = k_pages.shape[1]
+    if page < 1 or page & (page - 1) or page > 65536 or k_pages.shape[0] < 1:
+        raise RuntimeError(f"{what}: {k_pages.shape[0]} pages of {page}: the page size must be a power of two up to 65536")
+    if page_table.dim() != 2 or page_table.dtype != th.int32 or page_table.shape[1] < 1 or page_table.stride(1) != 1:
+        raise RuntimeError(f"{what}: page_table must be int32 sequences x pages, got {tuple(page_table.shape)} "
+                           f"{page_table.dtype}")
+    N = page_table.shape[0]
+    if page_table.stride(0) < page_table.shape[1]:
+        page_table = page_table.contiguous()
+    cu_seqlens = _index_array(cu_seqlens, f"{what}: cu_seqlens", N + 1)
+    kv_lens = _index_array(kv_lens, f"{what}: kv_lens", N)
+    if N < 1 and rows:
+        raise RuntimeError(f"{what}: {rows} tokens and no sequence")
+    return page_table, cu_seqlens, kv_lens
+
+
+def paged_append(k: th.Tensor, v: th.Tensor, k_pages: th.Tensor, v_pages: th.Tensor, page_table: th.Tensor,
+                 cu_seqlens: th.Tensor, kv_lens: th.Tensor) -> None:
+    """Write the keys / values of new tokens (k / v T x Hkv x D, sequence n's at rows cu_seqlens[n] ..) into
+    a paged cache: k_pages / v_pages P x page x Hkv x D (page a power of two), page_table N x W int32 (position
+    p of sequence n lies in page page_table[n, p // page]), kv_lens N: the positions of each sequence WITH its new
+    tokens, which are the last of them.  Positions without a page (an entry outside 0 .. P - 1) are not written.
+    Only the written slots change; two sequences must not write the same slot."""
+    what = "paged_append"
+    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or k.shape[2] not in PACKED_HEAD_DIMS or \
+            k.dtype not in ELEMENT_TYPES:
+        raise RuntimeError(f"{what}: k {tuple(k.shape)} {k.dtype} / v {tuple(v.shape)} {v.dtype}: tokens x heads x "
+                           f"head_dim {PACKED_HEAD_DIMS} in f32 / bf16 / f16")
+    page_table, cu_seqlens, kv_lens = _check_cache(what, k.shape[0], k_pages, v_pages, page_table, cu_seqlens, kv_lens)
+    if k_pages.shape != v_pages.shape or k_pages.shape[2:] != k.shape[1:] or k_pages.dtype != k.dtype or \
+            v_pages.dtype != k.dtype:
+        raise RuntimeError(f"{what}: cache {tuple(k_pages.shape)} {k_pages.dtype} / {tuple(v_pages.shape)} does not fit "
+                           f"k {tuple(k.shape)} {k.dtype}")
+    nat.require_device(k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens)
+    T, H, D = k.shape
+    if not T or not H:
+        return
+    k, v = _strided16(k), _strided16(v)
+    with nat.on_device_of(k):
+        rc = nat.load().aps_paged_append(
+            k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+            cu_seqlens.data_ptr(), int(cu_seqlens.dtype == th.int64), kv_lens.data_ptr(),
+            int(kv_lens.dtype == th.int64), T, page_table.shape[0], H, D, k_pages.shape[0], k_pages.shape[1],
+            page_table.shape[1], page_table.stride(0), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            ELEMENT_TYPES[k.dtype], nat.stream_of(k))
+    nat.check(rc, "aps_paged_append")
+
+
+def attention_paged(q: th.Tensor, k_pages: th.Tensor, v_pages: th.Tensor, page_table: th.Tensor,
+                    cu_seqlens: th.Tensor, kv_lens: th.Tensor, scale: Optional[float] = None,
+                    out: Optional[th.Tensor] = None) -> th.Tensor:
+    """Attention of new tokens (one a sequence, a chunk, none) over a paged cache that holds their own keys
+    already (`paged_append`, same cache arguments): q T x Hq x D -> T x Hq x D.  Token i of the L new ones of
+    sequence n sits at position kv_lens[n] - L + i and sees the positions up to there; a row that sees
+    nothing gives zeros.  Rows behind the last sequence are zeros, or left as they are in a given `out`
+    (contiguous, not overlapping the inputs).  Inference only."""
+    what = "attention_paged"
+    page_table, cu_seqlens, kv_lens = _check_cache(what, q.shape[0], k_pages, v_pages, page_table, cu_seqlens, kv_lens)
+    _check_heads(what, q, k_pages, v_pages)
+    scale = _softmax_scale(what, scale, q.shape[2])
+    nat.require_device(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, out)
+    lib = nat.load()
+    T, Hq, D = q.shape
+    keep = out is not None
+    if not keep:
+        out = th.empty(T, Hq, D, device=q.device, dtype=q.dtype)
+    else:
+        if out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
+            raise RuntimeError(f"{what}: out must be contiguous, 16-byte aligned, {tuple(q.shape)} {q.dtype}")
+        for t in (q, k_pages, v_pages):
+            if _overlap(out, t):
+                raise RuntimeError(f"{what}: out overlaps an input")
+    if not T:
+        return out
+    N, W = page_table.shape
+    P, page, Hkv, _ = k_pages.shape
+    dtype = ELEMENT_TYPES[q.dtype]
+    q = _strided16(q)
+    nbytes = lib.aps_attention_paged_workspace(T, N, Hq, Hkv, D, page, W, dtype)
+    ws = th.empty(nbytes, device=q.device, dtype=th.uint8) if nbytes > 0 else None
+    with nat.on_device_of(q):
+        rc = lib.aps_attention_paged(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), cu_seqlens.data_ptr(),
+            int(cu_seqlens.dtype == th.int64), kv_lens.data_ptr(), int(kv_lens.dtype == th.int64), out.data_ptr(), T,
+            N, Hq, Hkv, D, P, page, W, page_table.stride(0), q.stride(0), q.stride(1), dtype, scale, int(keep),
+            None if ws is None else ws.data_ptr(), nat.stream_of(q))
+    nat.check(rc, "aps_attention_paged")
+    return out
+
+
+def _extent(t: th.Tensor):
+    """first and last byte + 1 a tensor touches"""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size() if t.numel() else t.data_ptr()
+
+
+def _overlap(a: th.Tensor, b: th.Tensor) -> bool:
+    (a0, a1), (b0, b1) = _extent(a), _extent(b)
+    return a0 < b1 and b0 < a1
+
+
+BEAM_MAX = 64
+
+
+def beam_select(logits: th.Tensor, scores: th.Tensor, eos: int, finished: Optional[th.Tensor] = None,
+                beam: Optional[int] = None):
+    """One step of a beam search: logits N B x V (| N x B x V; f32 | bf16 | f16, not normalised) of B
+    hypotheses of N utterances with scores N x B (f32) -> (scores, parent, token, finished), each N x K: the K =
+    `beam` (default B) best of score + log_softmax(logits) over an utterance's B V continuations, best first,
+    ties to the lowest b V + v; parent (which of the B) and token int64, finished = the parent was, or the
+    token is `eos`.  finished N x B bool: such a hypothesis has one continuation, `eos` at its own score.
+    Ruled-out tokens are -inf logits, unused hypotheses -inf scores (the first step: B = 1, or scores 0, -inf,
+    ...); they are selected only when nothing else is left.  NaN counts as -inf.  Totals in 64 bits."""
+    what = "beam_select"
+    if scores.dim() != 2 or scores.dtype != th.float32:
+        raise RuntimeError(f"{what}: scores must be f32 utterances x hypotheses, got {tuple(scores.shape)} {scores.dtype}")
+    N, B = scores.shape
+    K = B if beam is None else int(beam)
+    V = logits.shape[-1] if logits.dim() else 0
+    if logits.dtype not in ELEMENT_TYPES or tuple(logits.shape) not in ((N * B, V), (N, B, V)):
+        raise RuntimeError(f"{what}: logits {tuple(logits.shape)} {logits.dtype} for {N} x {B} hypotheses")
+    if N < 1 or not 1 <= B <= BEAM_MAX or not 1 <= K <= BEAM_MAX or not 1 <= V <= 1 << 24 or K > B * V:
+        raise RuntimeError(f"{what}: {N} utterances, {B} hypotheses, beam {K}, vocabulary {V}: at least one utterance, "
+                           f"1 .. {BEAM_MAX} hypotheses, 1 .. 2^24 tokens, no more selected than there are")
+    eos = int(eos)
+    if not 0 <= eos < V:
+        raise RuntimeError(f"{what}: eos {eos} outside the vocabulary of {V}")
+    if finished is not None and (finished.shape != scores.shape or finished.dtype != th.bool):
+        raise RuntimeError(f"{what}: finished must be bool {tuple(scores.shape)}, got {tuple(finished.shape)} {finished.dtype}")
+    nat.require_device(logits, scores, finished)
+    lib = nat.load()
+    logits = logits.reshape(N * B, V)
+    if logits.stride(1) != 1 or (logits.stride(0) < V and N * B > 1):
+        logits = logits.contiguous()
+    scores = scores.contiguous()
+    finished = None if finished is None else finished.contiguous()
+    dev = logits.device
+    new_scores = th.empty(N, K, device=dev, dtype=th.float32)
+    parent, token = th.empty(2, N, K, device=dev, dtype=th.int64).unbind(0)
+    done = th.empty(N, K, device=dev, dtype=th.bool)
+    ws = th.empty(lib.aps_beam_select_workspace(N, B, V, K), device=dev, dtype=th.uint8)
+    with nat.on_device_of(logits):
+        rc = lib.aps_beam_select(logits.data_ptr(), max(logits.stride(0), V), scores.data_ptr(),
+                                 None if finished is None else finished.data_ptr(), eos, new_scores.data_ptr(),
+                                 parent.data_ptr(), token.data_ptr(), done.data_ptr(), N, B, V, K,
+                                 ELEMENT_TYPES[logits.dtype], ws.data_ptr(), nat.stream_of(logits))
+    nat.check(rc, "aps_beam_select")
+    return new_scores, parent, token, done
+
+
+def beam_reorder(states: Sequence[th.Tensor], parent: th.Tensor, dims: Optional[Sequence[int]] = None) -> List[th.Tensor]:
+    """States of the hypotheses that `beam_select` chose: every tensor of `states` has an axis of N B
+    hypotheses (`dims`, default the first: token histories, page tables and contexts N B x ...; 1 for the
+    L x N B x H states of nn.LSTM / nn.GRU) -> new tensors with N K there, row n K + k being row
+    n B + parent[n, k].  Any types, one launch for up to 16 tensors.  parent N x K int64, values 0 .. B - 1 (one
+    outside gives zeros).  No gradient."""
+    what = "beam_reorder"
+    if parent.dim() != 2 or parent.dtype != th.int64 or parent.numel() == 0:
+        raise RuntimeError(f"{what}: parent must be int64 utterances x beam, got {tuple(parent.shape)} {parent.dtype}")
+    states = list(states)
+    dims = [0] * len(states) if dims is None else [int(d) for d in dims]
+    if len(dims) != len(states):
+        raise RuntimeError(f"{what}: {len(states)} states, {len(dims)} dims")
+    if not states:
+        return []
+    nat.require_device(parent, *states)
+    N, K = parent.shape
+    B, src, dst, outer, inner = 0, [], [], [], []
+    for t, d in zip(states, dims):
+        if not -t.dim() <= d < t.dim():
+            raise RuntimeError(f"{what}: a state {tuple(t.shape)} has no axis {d}")
+        d %= t.dim()
+        rows = t.shape[d]
+        if rows < N or rows % N or (B and rows != N * B):
+            raise RuntimeError(f"{what}: axis {d} of {tuple(t.shape)} is not {N} x {B or 'hypotheses'}")
+        B = rows // N
+        t = t.contiguous()
+        shape = list(t.shape)
+        shape[d] = N * K
+        src.append(t)
+        dst.append(th.empty(shape, device=t.device, dtype=t.dtype))
+        outer.append(math.prod(shape[:d]))
+        inner.append(math.prod(shape[d + 1:]) * t.element_size())
+    parent = parent.contiguous()
+    n = len(src)
+    with nat.on_device_of(parent):
+        rc = nat.load().aps_beam_reorder((C_void_p * n)(*[t.data_ptr() for t in src]),
+                                         (C_void_p * n)(*[t.data_ptr() for t in dst]), (C_int64 * n)(*outer),
+                                         (C_int64 * n)(*inner), n, parent.data_ptr(), N, K, B, nat.stream_of(parent))
+    nat.check(rc, "aps_beam_reorder")
+    return dst
 
 
 def embedding_posenc(table: th.Tensor, ids: th.Tensor, div_term: th.Tensor, factor: float = 1.0,

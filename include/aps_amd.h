@@ -1045,6 +1045,82 @@ int aps_conformer_stack(float* x, const int64_t* lens, const ApsMegaLayer* layer
                         const float* rel, int64_t rel_zero, int64_t rel_len, int64_t N, int64_t T, int64_t D,
                         int64_t FF, int64_t heads, float* scratch, int32_t* wide_count, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Autoregressive decoding and training on packed sequences: attention over sequences packed end to end
+ * with its gradients, attention of new tokens over a paged cache, one step of a beam search.  These take
+ * f32, bf16 and f16 (dtype 0 / 1 / 2) and grouped heads (Hq a multiple of Hkv: query head h reads key
+ * head h / (Hq / Hkv)); head_dim in {32, 64, 128}.  Accumulation, softmax statistics and log-sum-exps
+ * are f32 or wider for every type.
+ *   cu_seqlens [N + 1] (int32, or int64 with cu_wide = 1): tokens cu[n] .. cu[n + 1] - 1 of the packed
+ *     axis are sequence n; from 0, non-decreasing, at most `total`.  Values outside that are clamped on
+ *     the device.  Rows behind the last sequence belong to none: their outputs / gradients are zeros.
+ *   strides q_t, q_h, ... in elements (token, head; the last axis is contiguous); pointers 16-byte
+ *     aligned, strides multiples of 16 bytes.
+ * ------------------------------------------------------------------------------------------- */
+
+/* out[r, h] = sum_j softmax_j(scale q[r, h] . k[j, h']) v[j, h'] over the keys of r's own sequence, those
+ * up to r if `causal`; q [total, Hq, dh], k / v [total, Hkv, dh] -> out [total, Hq, dh] contiguous.
+ * lse (or NULL) [total, Hq]: log2 of the softmax's sum, what the backward pass needs. */
+int aps_attention_packed(const void* q, const void* k, const void* v, const void* cu_seqlens, int32_t cu_wide,
+                         void* out, float* lse, int64_t total, int64_t N, int64_t Hq, int64_t Hkv,
+                         int64_t head_dim, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t v_t,
+                         int64_t v_h, int32_t dtype, int32_t causal, float scale, void* stream);
+/* its adjoint: g_out [total, Hq, dh] by strides -> g_q [total, Hq, dh], g_k / g_v [total, Hkv, dh]
+ * contiguous, the same bits on every run (no atomics).  out, lse: of the forward call.
+ * workspace: aps_attention_packed_backward_workspace bytes. */
+int64_t aps_attention_packed_backward_workspace(int64_t total, int64_t Hq);
+int aps_attention_packed_backward(const void* q, const void* k, const void* v, const void* out,
+                                  const void* g_out, const float* lse, const void* cu_seqlens,
+                                  int32_t cu_wide, void* g_q, void* g_k, void* g_v, int64_t total, int64_t N,
+                                  int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t q_t, int64_t q_h,
+                                  int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h, int64_t go_t,
+                                  int64_t go_h, int32_t dtype, int32_t causal, float scale, void* workspace,
+                                  void* stream);
+
+/* Paged cache: k_pages / v_pages [num_pages, page, Hkv, dh] contiguous, `page` a power of two up to 65536
+ * (page 1: a slot per token, so the row of a table is a history that can be copied and regrouped);
+ * page_table int32 [N, width] (row stride table_stride): position p of sequence n lies in page
+ * page_table[n, p / page]; kv_lens [N] (int32, or int64 with kv_wide = 1): positions of sequence n, the
+ * new tokens (its cu_seqlens range) being the last of them.  A position whose page is outside
+ * [0, num_pages) is hidden from the attention and not written; one before 0 (more new tokens than
+ * positions) sees nothing and is not written.
+ * aps_paged_append: k / v [total, Hkv, dh] (by strides) of the new tokens into the cache. */
+int aps_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
+                     const void* cu_seqlens, int32_t cu_wide, const void* kv_lens, int32_t kv_wide,
+                     int64_t total, int64_t N, int64_t Hkv, int64_t head_dim, int64_t num_pages, int64_t page,
+                     int64_t width, int64_t table_stride, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h,
+                     int32_t dtype, void* stream);
+/* the new tokens' attention over everything cached up to themselves; a row that sees nothing gives zeros.
+ * keep_tail = 1: rows of no sequence are left as they are instead of cleared.
+ * workspace: aps_attention_paged_workspace bytes (0: none needed). */
+int64_t aps_attention_paged_workspace(int64_t total, int64_t N, int64_t Hq, int64_t Hkv, int64_t head_dim,
+                                      int64_t page, int64_t width, int32_t dtype);
+int aps_attention_paged(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
+                        const void* cu_seqlens, int32_t cu_wide, const void* kv_lens, int32_t kv_wide, void* out,
+                        int64_t total, int64_t N, int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t num_pages,
+                        int64_t page, int64_t width, int64_t table_stride, int64_t q_t, int64_t q_h,
+                        int32_t dtype, float scale, int32_t keep_tail, void* workspace, void* stream);
+
+/* One step of a beam search over N utterances of B hypotheses each (B, K <= 64, V <= 2^24):
+ *   total[n, b, v] = scores[n, b] + logits[n B + b, v] - log sum exp logits[n B + b, :]
+ * and its K largest per utterance in descending order, ties to the lowest b V + v (among the
+ * continuations of one hypothesis: by logit, ties to the lowest token).  Totals are formed in 64 bits.
+ * finished uint8 [N, B] (or NULL): a finished hypothesis has one continuation, `eos`, at its own score.
+ * A NaN logit or score counts as -inf, +inf as the largest finite value; what is ruled out (-inf) is
+ * selected only when nothing else is left, lowest b V + v first.
+ * logits [N B, V] with row_stride elements between rows (any alignment); outputs [N, K]: new_scores f32,
+ * parent (b) and token int64, new_finished uint8 = the parent was finished or the token is eos.
+ * workspace: aps_beam_select_workspace bytes. */
+int64_t aps_beam_select_workspace(int64_t N, int64_t B, int64_t V, int64_t K);
+int aps_beam_select(const void* logits, int64_t row_stride, const float* scores, const uint8_t* finished,
+                    int64_t eos, float* new_scores, int64_t* parent, int64_t* token, uint8_t* new_finished,
+                    int64_t N, int64_t B, int64_t V, int64_t K, int32_t dtype, void* workspace, void* stream);
+/* the states of the selected hypotheses: row n K + k of dst[s] = row n B + parent[n, k] of src[s], for
+ * `count` tensors [outer[s], N B (dst: N K), inner_bytes[s]] (16 a launch); src, dst, outer, inner_bytes
+ * are host arrays.  A parent outside [0, B) gives zeros.  dst must not overlap src. */
+int aps_beam_reorder(const void* const* src, void* const* dst, const int64_t* outer, const int64_t* inner_bytes,
+                     int64_t count, const int64_t* parent, int64_t N, int64_t K, int64_t B, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,255 @@
+"""
+The decoder's operators on packed sequences, paged caches and beams (nn_ops.attention_packed,
+paged_append, attention_paged, beam_select, beam_reorder) against 64-bit definitions
+(tests/attention_reference.py: elementwise bounds derived there).
+"""
+import pytest
+import torch
+
+from tests import attention_reference as ref
+
+gpu = pytest.mark.gpu
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+DEV = "cuda:0"
+
+
+def cu_of(lens, dtype=torch.int32, device=DEV):
+    return torch.tensor([0] + list(torch.tensor(lens).cumsum(0)), dtype=dtype, device=device)
+
+
+def randn(*shape, dtype=torch.float32, seed=0, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(*shape, generator=g) * std).to(dtype).to(DEV)
+
+
+PACKED = [  # type, heads, key heads, head_dim, lengths, causal, rows behind the last sequence
+    ("f32", 1, 1, 64, [1], True, 0),
+    ("f32", 2, 2, 64, [0, 1, 0, 2, 0], True, 3),
+    ("f32", 8, 8, 64, [31, 32, 33, 5], True, 0),
+    ("f32", 4, 2, 32, [63, 64, 65, 1, 127], False, 1),
+    ("f32", 3, 1, 128, [130, 97], True, 0),
+    ("f32", 6, 2, 128, [45, 0, 33], False, 5),
+    ("bf16", 1, 1, 128, [1], False, 0),
+    ("bf16", 8, 2, 128, [64, 65, 129, 2], True, 0),
+    ("bf16", 6, 2, 64, [200, 31, 1], True, 7),
+    ("bf16", 5, 5, 32, [257, 0, 64], False, 0),
+    ("bf16", 16, 1, 64, [70, 9], True, 0),
+    ("f16", 4, 4, 64, [128, 127, 129], True, 0),
+    ("f16", 2, 1, 128, [300, 5], False, 2),
+    ("f16", 7, 1, 32, [37, 500], True, 0),
+]
+
+
+@gpu
+@pytest.mark.parametrize("kind,hq,hkv,d,lens,causal,tail", PACKED)
+def test_packed_forward(kind, hq, hkv, d, lens, causal, tail):
+    from aps_amd import nn_ops
+    t = sum(lens) + tail
+    q, k, v = (randn(t, h, d, dtype=TYPES[kind], seed=i) for i, h in enumerate((hq, hkv, hkv)))
+    with torch.no_grad():
+        out = nn_ops.attention_packed(q, k, v, cu_of(lens), causal=causal)
+    (want,), (bound,) = ref.packed(q, k, v, lens, causal)
+    ref.check(out, want, bound, "out")
+
+
+@gpu
+@pytest.mark.parametrize("kind,hq,hkv,d,lens,causal,tail", PACKED)
+def test_packed_gradients(kind, hq, hkv, d, lens, causal, tail):
+    from aps_amd import nn_ops
+    t = sum(lens) + tail
+    q, k, v = (randn(t, h, d, dtype=TYPES[kind], seed=i).requires_grad_() for i, h in enumerate((hq, hkv, hkv)))
+    g = randn(t, hq, d, dtype=TYPES[kind], seed=7)
+    out = nn_ops.attention_packed(q, k, v, cu_of(lens, torch.int64), causal=causal)
+    grads = torch.autograd.grad(out, (q, k, v), g)
+    vals, bounds = ref.packed(q, k, v, lens, causal, g=g)
+    for name, x, want, bound in zip(("out", "gq", "gk", "gv"), (out,) + grads, vals, bounds):
+        assert x.dtype == q.dtype
+        ref.check(x, want, bound, name)
+    again = torch.autograd.grad(nn_ops.attention_packed(q, k, v, cu_of(lens), causal=causal), (q, k, v), g)
+    assert all(torch.equal(a, b) for a, b in zip(grads, again))
+
+
+def paged_case(kind, hkv, d, lens, page, seed, poison=float("nan")):
+    """a cache with the old tokens of `lens` = [(new, old)] in randomly ordered pages, the rest poisoned"""
+    need = [(a + b + page - 1) // page for a, b in lens]
+    width, count = max(need + [1]) + 1, sum(need) + 2
+    g = torch.Generator().manual_seed(seed)
+    order = torch.randperm(count, generator=g)
+    table = torch.full((len(lens), width), -1, dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        table[i, :n] = order[at:at + n].int()
+        at += n
+    cache = [torch.full((count, page, hkv, d), poison).to(TYPES[kind]) for _ in range(2)]
+    old = []
+    for i, (new, had) in enumerate(lens):
+        rows = [torch.randn(had, hkv, d, generator=g).to(TYPES[kind]) for _ in range(2)]
+        for p in range(had):
+            for c, r in zip(cache, rows):
+                c[table[i, p // page], p % page] = r[p]
+        old.append(rows)
+    return table, cache, old
+
+
+PAGED = [  # type, heads, key heads, head_dim, [(new, old)], page
+    ("f32", 8, 8, 64, [(1, 0), (1, 5), (1, 200), (1, 31)], 1),
+    ("f32", 2, 1, 128, [(1, 70), (0, 9), (3, 0)], 16),
+    ("f32", 32, 1, 128, [(1, 300), (1, 63)], 32),
+    ("f32", 4, 4, 32, [(50, 20), (1, 0), (128, 3)], 8),
+    ("f32", 4, 2, 128, [(200, 77), (33, 400)], 64),
+    ("bf16", 32, 8, 128, [(1, 1000), (1, 511), (1, 0), (1, 63), (1, 64)], 64),
+    ("bf16", 4, 4, 64, [(1, 4000)], 16),
+    ("bf16", 16, 2, 64, [(4, 700), (3, 1), (0, 0), (5, 32)], 16),
+    ("bf16", 24, 1, 32, [(1, 129), (2, 300)], 128),
+    ("bf16", 8, 2, 128, [(257, 1000), (1, 3000), (64, 0)], 32),
+    ("f16", 6, 2, 64, [(1, 77), (1, 2500)], 4),
+    ("f16", 2, 2, 32, [(1, 1), (2, 2), (3, 3)], 2),
+    ("f16", 12, 3, 128, [(100, 0), (7, 650)], 1),
+]
+
+
+@gpu
+@pytest.mark.parametrize("kind,hq,hkv,d,lens,page", PAGED)
+def test_paged_step(kind, hq, hkv, d, lens, page):
+    """append + attention, the cache's unwritten slots holding NaN"""
+    from aps_amd import nn_ops
+    table, cache, old = paged_case(kind, hkv, d, lens, page, seed=len(lens))
+    new = [a for a, _ in lens]
+    total = sum(new)
+    width = (hq + 2 * hkv) * d  # slices of one projection
+    qkv = randn(total + 2, width, dtype=TYPES[kind], seed=3)
+    q = qkv[:, :hq * d].view(-1, hq, d)
+    k = qkv[:, hq * d:(hq + hkv) * d].view(-1, hkv, d)
+    v = qkv[:, (hq + hkv) * d:].view(-1, hkv, d)
+    want_k, want_v = (c.clone() for c in cache)
+    a = 0
+    for i, (n, had) in enumerate(lens):
+        for j in range(n):
+            p = had + j
+            want_k[table[i, p // page], p % page] = k[a + j].cpu()
+            want_v[table[i, p // page], p % page] = v[a + j].cpu()
+        a += n
+    kc, vc = (c.to(DEV) for c in cache)
+    args = (kc, vc, table.to(DEV), cu_of(new), torch.tensor([a + b for a, b in lens], device=DEV, dtype=torch.int32))
+    with torch.no_grad():
+        nn_ops.paged_append(k, v, *args)
+        out = nn_ops.attention_paged(q, *args)
+        kept = torch.full_like(out, 7.0)
+        assert nn_ops.attention_paged(q, *args, out=kept) is kept
+    assert torch.equal(torch.nan_to_num(kc.cpu(), nan=9.5), torch.nan_to_num(want_k, nan=9.5))
+    assert torch.equal(torch.nan_to_num(vc.cpu(), nan=9.5), torch.nan_to_num(want_v, nan=9.5))
+    assert (out[total:] == 0).all() and (kept[total:] == 7.0).all() and torch.equal(kept[:total], out[:total])
+    a = 0
+    for i, (n, had) in enumerate(lens):
+        ks = torch.cat([old[i][0], k[a:a + n].cpu()]).double()
+        vs = torch.cat([old[i][1], v[a:a + n].cpu()]).double()
+        for h in range(hq if n else 0):
+            c = h // (hq // hkv)
+            want, bound = ref.attend(q[a:a + n, h].cpu().double(), ks[:, c], vs[:, c], had, True, d**-0.5, TYPES[kind])
+            ref.check(out[a:a + n, h], want, bound, f"sequence {i} head {h}")
+        a += n
+
+
+def beam_reference(logits, scores, eos, finished, K):
+    n, b = scores.shape
+    x = logits.detach().cpu().double().view(n, b, -1)
+    x = torch.nan_to_num(x, nan=float("-inf"), posinf=torch.finfo(torch.float32).max, neginf=float("-inf"))
+    s = torch.nan_to_num(scores.detach().cpu().double(), nan=float("-inf"), posinf=torch.finfo(torch.float32).max,
+                         neginf=float("-inf"))
+    v = x.shape[-1]
+    logp = x - torch.logsumexp(x, -1, keepdim=True)
+    logp = torch.where(torch.isnan(logp), torch.full_like(logp, float("-inf")), logp)
+    fin = torch.zeros(n, b, dtype=torch.bool) if finished is None else finished.cpu()
+    only = torch.full((v,), float("-inf"), dtype=torch.float64)
+    only[eos] = 0
+    logp = torch.where(fin[..., None], only, logp)
+    total = (s[..., None] + logp).view(n, -1)
+    best, at = torch.sort(total, dim=1, descending=True, stable=True)
+    best, at = best[:, :K], at[:, :K]
+    parent, token = at // v, at % v
+    return best, parent, token, torch.gather(fin, 1, parent) | (token == eos)
+
+
+def check_beam(logits, scores, eos, finished, K):
+    from aps_amd import nn_ops
+    got = nn_ops.beam_select(logits, scores, eos, finished=finished, beam=K)
+    want = beam_reference(logits, scores, eos, finished, K)
+    assert torch.equal(got[1].cpu(), want[1]) and torch.equal(got[2].cpu(), want[2])
+    assert torch.equal(got[3].cpu(), want[3])
+    w = want[0].float()
+    close = (got[0].cpu() == w) | ((got[0].cpu() - w).abs() <= 2**-23 * w.abs())
+    assert close.all(), (got[0], w)
+
+
+BEAM = [  # type, utterances, hypotheses, vocabulary, K, finished share
+    ("f32", 1, 1, 1, 1, 0.0), ("f32", 1, 1, 7, 7, 0.0), ("f32", 2, 3, 5, 15, 0.5), ("f32", 1, 8, 4233, 8, 0.2),
+    ("f32", 3, 64, 333, 64, 0.1), ("f32", 2, 4, 8192, 4, 0.0), ("f32", 2, 4, 8193, 5, 0.0), ("f32", 5, 2, 40001, 64, 0.0),
+    ("bf16", 9, 5, 10007, 5, 0.3), ("bf16", 4, 16, 129, 16, 0.6), ("f16", 2, 10, 5003, 10, 1.0), ("f16", 1, 1, 65, 64, 0.0),
+]
+
+
+@gpu
+@pytest.mark.parametrize("kind,n,b,v,K,share", BEAM)
+def test_beam_select(kind, n, b, v, K, share):
+    logits = randn(n * b, v, dtype=TYPES[kind], seed=v, std=3.0)
+    scores = -randn(n, b, seed=1).abs() * 5
+    fin = (randn(n, b, seed=2).abs() < share * 1.5) if share else None
+    check_beam(logits, scores, v // 2, fin, K)
+    # rows that do not begin on 16 bytes, and a row stride
+    wide = torch.zeros(n * b, v + 3, dtype=TYPES[kind], device=DEV)
+    wide[:, 1:v + 1] = logits
+    check_beam(wide[:, 1:v + 1], scores, v // 2, fin, K)
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("v", [70, 3001, 20000])
+def test_beam_select_ties_and_ruled_out(kind, v):
+    """equal logits (more than fit the candidate list), whole rows ruled out, NaN, +inf, unused
+    hypotheses, fewer continuations than selected"""
+    flat = torch.zeros(2 * 3, v, dtype=TYPES[kind], device=DEV)
+    scores = torch.tensor([[-1.0, -1.0, -2.0], [-3.0, -0.5, -0.5]], device=DEV)
+    check_beam(flat, scores, 1, None, 9)
+    flat[:, ::2] = -0.0
+    check_beam(flat, scores, 1, None, 9)
+    few = torch.full((2 * 3, v), float("-inf"), dtype=TYPES[kind], device=DEV)
+    check_beam(few, scores, 1, None, 9)
+    few[1, v - 1] = 2.0
+    few[4, 5] = -4.0
+    check_beam(few, scores, 1, None, 9)
+    first = torch.tensor([[0.0, float("-inf"), float("-inf")], [float("nan"), float("-inf"), 0.0]], device=DEV)
+    x = randn(6, v, dtype=TYPES[kind], seed=5)
+    check_beam(x, first, 2, None, 9)
+    check_beam(x, first, 2, torch.tensor([[True, False, True], [False, False, False]], device=DEV), 9)
+    x[0, 3] = float("nan")
+    x[5, :4] = float("nan")
+    check_beam(x, scores, 2, None, 9)
+    x[2, 7] = float("inf")
+    x[3, 1] = x[3, 9] = float("inf")
+    from aps_amd import nn_ops
+    got = nn_ops.beam_select(x, scores, 2, beam=9)
+    assert not torch.isnan(got[0]).any()
+
+
+@gpu
+def test_beam_reorder():
+    from aps_amd import nn_ops
+    n, b, K = 3, 4, 6
+    parent = torch.tensor([[0, 1, 1, 3, 2, 0], [3, 3, 3, 3, 3, 3], [2, 0, 1, 1, 0, 2]], device=DEV)
+    rows = (parent.cpu() + b * torch.arange(n)[:, None]).reshape(-1)
+    states, dims = [], []
+    for i, (shape, dim, dtype) in enumerate([
+            ((12, 5), 0, torch.int64), ((12,), 0, torch.bool), ((2, 12, 7), 1, torch.float32),
+            ((3, 12, 33), -2, torch.bfloat16), ((12, 3), 0, torch.uint8), ((12, 64, 16), 0, torch.float16),
+            ((12, 0), 0, torch.float32), ((5, 2, 12), 2, torch.int32), ((12, 1025), 0, torch.int16)]):
+        g = torch.Generator().manual_seed(i)
+        states.append(torch.randint(0, 100, shape, generator=g).to(dtype).to(DEV))
+        dims.append(dim)
+    states = states * 3  # more than a launch takes
+    dims = dims * 3
+    out = nn_ops.beam_reorder(states, parent, dims=dims)
+    for x, s, d in zip(out, states, dims):
+        assert torch.equal(x.cpu(), s.cpu().index_select(d, rows)), (s.shape, d)
+    odd = nn_ops.beam_reorder([states[0]], parent.clone().fill_(4))[0]
+    assert (odd == 0).all()
+    assert nn_ops.beam_reorder([], parent) == []
