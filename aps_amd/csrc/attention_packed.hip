@@ -126,16 +126,22 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
                 f32x4{acc[d][i] * a.scale, acc[d][i + 1] * a.scale, acc[d][i + 2] * a.scale, acc[d][i + 3] * a.scale});
 }
 
-// dk, dv: a workgroup per (tile of 128 keys, key head), a wavefront per 32 keys whose K and V rows stay
-// in registers as right operands; Q and dO go through LDS, 32 rows (64 for 16-bit types) at a time, with
-// the rows' lse, D_r and positions beside them.  S = Q K^T and dP = dO V^T have the rows in the
-// registers, so P and dS are the right operands of dv^T = dO^T P and dk^T = Q^T dS as they stand.
-template <typename T>
-constexpr int grad_rows() { return sizeof(T) == 2 ? 64 : 32; }
+// dk, dv: a workgroup per (tile of keys, key head), a wavefront per 32 keys whose K and V rows stay in
+// registers as right operands; Q and dO go through LDS with the rows' lse, D_r and positions beside them.
+// S = Q K^T and dP = dO V^T have the rows in the registers, so P and dS are the right operands of
+// dv^T = dO^T P and dk^T = Q^T dS as they stand.  Two of the four wavefronts share 32 keys and take
+// alternate blocks of 32 rows, their sums meeting in LDS at the end: a tile of 64 keys, because the first
+// keys of a causal sequence are seen by every row of the group and the longest tile is what the launch
+// waits for (128-key tiles: %K128%; 64: %K64% on 12 sequences of 64 - 2 048 tokens, 16 / 4 heads of 128, bf16).  f32 with
+// D = 128 has no registers for the larger row tile: four times 32 keys there.
+template <typename T, int D>
+constexpr int grad_rows() { return D * sizeof(T) >= 512 ? 32 : 64; }
+template <typename T, int D>
+constexpr int grad_keys() { return 32 * 4 / (grad_rows<T, D>() / 32); }
 
 template <typename T, int D>
 __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention_keys_backward_kernel(GradArgs a) {
-  constexpr int BR = grad_rows<T>(), E = chunk_elems<T>(), CH = D / E, KS = 2 * E, NS = D / KS, NRB = BR / 32;
+  constexpr int BR = grad_rows<T, D>(), RG = BR / 32, KG = 4 / RG, E = chunk_elems<T>(), CH = D / E, KS = 2 * E, NS = D / KS;
   constexpr int NDB = D / 32, NPS = 32 / KS, TILE = BR * D * (int)sizeof(T), PER = BR * CH / 256, STEP = 256 / CH;
   __shared__ __align__(16) char lds[4 * TILE];
   __shared__ __align__(16) float s_lse[2][BR], s_delta[2][BR];
@@ -143,7 +149,7 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
   const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
   const int64_t want = blockIdx.x / a.Hkv;  // the first keys are seen by the most rows: they go first
-  const SeqTile t = find_tile(a.cu, a.N, a.total, 1, kRowTile, want, lane);
+  const SeqTile t = find_tile(a.cu, a.N, a.total, 1, grad_keys<T, D>(), want, lane);
   const int Hq = a.Hkv * a.G;
   if (t.seq < 0) {
     if (h == 0) {
@@ -152,7 +158,7 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
     }
     return;
   }
-  const int rows = t.len * a.G, tile0 = t.tile * kRowTile, key0 = tile0 + wv * 32, key = key0 + (lane & 31);
+  const int rows = t.len * a.G, tile0 = t.tile * grad_keys<T, D>(), key0 = tile0 + wv % KG * 32, key = key0 + (lane & 31);
   const bool live = key < t.len;
   u32x4 kf[NS], vf[NS];
   {
@@ -214,50 +220,69 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
     const char* tg = tq + TILE;
     const bool more = rt + 1 < hi;
     if (more) load((rt + 1) * BR);
-#pragma unroll 1
-    for (int b = 0; b < NRB; ++b) {
-      const int r0 = rt * BR + b * 32;
-      // rows [r0, r0 + 32): none sees this wavefront's keys / some see some of them
-      const bool none = key0 >= t.len || r0 >= rows || (a.causal && (min(r0 + 32, rows) - 1) / a.G < key0);
-      if (none) continue;
-      f32x16 s = f32x16{0}, g = f32x16{0};
+    const int b = wv / KG;  // this wavefront's block of 32 rows
+    const int r0 = rt * BR + b * 32;
+    // (every wavefront multiplies every block, masked ones too: a branch around the products makes the
+    // compiler move the 128 accumulators between the register files in every iteration)
+    f32x16 s = f32x16{0}, g = f32x16{0};
 #pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        s = mma<T>(frag<T, D>(tq, b * 32 + (lane & 31), i, half), kf[i], s);
-        g = mma<T>(frag<T, D>(tg, b * 32 + (lane & 31), i, half), vf[i], g);
+    for (int i = 0; i < NS; ++i) {
+      s = mma<T>(frag<T, D>(tq, b * 32 + (lane & 31), i, half), kf[i], s);
+      g = mma<T>(frag<T, D>(tg, b * 32 + (lane & 31), i, half), vf[i], g);
+    }
+    const bool edge = r0 + 32 > rows || key0 + 32 > t.len || (a.causal && r0 / a.G < key0 + 31);
+    float p[16], ds[16];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[buf][b * 32 + j * 8 + half * 4]);
+      const f32x4 dl = *reinterpret_cast<const f32x4*>(&s_delta[buf][b * 32 + j * 8 + half * 4]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = j * 4 + e;
+        p[i] = exp2_fast(fmaf(s[i], a.c, -lse[e]));
+        ds[i] = p[i] * (g[i] - dl[e]);
       }
-      const bool edge = r0 + 32 > rows || key0 + 32 > t.len || (a.causal && r0 / a.G < key0 + 31);
-      float p[16], ds[16];
+      if (edge) {
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        const i32x4 ps = *reinterpret_cast<const i32x4*>(&s_pos[buf][b * 32 + j * 8 + half * 4]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[buf][b * 32 + j * 8 + half * 4]);
-        const f32x4 dl = *reinterpret_cast<const f32x4*>(&s_delta[buf][b * 32 + j * 8 + half * 4]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int i = j * 4 + e;
-          p[i] = exp2_fast(fmaf(s[i], a.c, -lse[e]));
-          ds[i] = p[i] * (g[i] - dl[e]);
-        }
-        if (edge) {
-          typedef int i32x4 __attribute__((ext_vector_type(4)));
-          const i32x4 ps = *reinterpret_cast<const i32x4*>(&s_pos[buf][b * 32 + j * 8 + half * 4]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (key > ps[e] || !live) p[j * 4 + e] = 0.f, ds[j * 4 + e] = 0.f;
-        }
+        for (int e = 0; e < 4; ++e)
+          if (key > ps[e] || !live) p[j * 4 + e] = 0.f, ds[j * 4 + e] = 0.f;
       }
+    }
 #pragma unroll
-      for (int i = 0; i < NPS; ++i) {
-        const u32x4 pf = pack<T>(p + i * (KS / 2)), df = pack<T>(ds + i * (KS / 2));
+    for (int i = 0; i < NPS; ++i) {
+      const u32x4 pf = pack<T>(p + i * (KS / 2)), df = pack<T>(ds + i * (KS / 2));
 #pragma unroll
-        for (int d = 0; d < NDB; ++d) {
-          gv[d] = mma<T>(frag_t<T, D>(tg, b * 32, i, d, lane), pf, gv[d]);
-          gk[d] = mma<T>(frag_t<T, D>(tq, b * 32, i, d, lane), df, gk[d]);
-        }
+      for (int d = 0; d < NDB; ++d) {
+        gv[d] = mma<T>(frag_t<T, D>(tg, b * 32, i, d, lane), pf, gv[d]);
+        gk[d] = mma<T>(frag_t<T, D>(tq, b * 32, i, d, lane), df, gk[d]);
       }
     }
     if (more) store(buf ^ 1);
     __syncthreads();
+  }
+  if constexpr (RG > 1) {  // the second half of the rows joins the first (the tiles are free by now)
+    float* meet = reinterpret_cast<float*>(lds) + (int64_t)(wv % KG) * (NDB * 32 * 64) + lane;
+    static_assert(KG * NDB * 32 * 64 * 4 <= sizeof(lds), "the sums of half the wavefronts fit the tiles");
+    if (wv >= KG) {
+#pragma unroll
+      for (int d = 0; d < NDB; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          meet[(d * 32 + i) * 64] = gk[d][i];
+          meet[(d * 32 + 16 + i) * 64] = gv[d][i];
+        }
+    }
+    __syncthreads();
+    if (wv >= KG) return;
+#pragma unroll
+    for (int d = 0; d < NDB; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        gk[d][i] += meet[(d * 32 + i) * 64];
+        gv[d][i] += meet[(d * 32 + 16 + i) * 64];
+      }
   }
   if (!live) return;
   T* pk = static_cast<T*>(a.gk) + ((t.start + key) * a.Hkv + h) * D;
@@ -281,8 +306,9 @@ static void launch_rows_backward(const GradArgs& a, unsigned grid, hipStream_t s
   hipLaunchKernelGGL((attention_rows_backward_kernel<T, D>), dim3(grid), dim3(256), 0, st, a);
 }
 template <typename T, int D>
-static void launch_keys_backward(const GradArgs& a, unsigned grid, hipStream_t st) {
-  hipLaunchKernelGGL((attention_keys_backward_kernel<T, D>), dim3(grid), dim3(256), 0, st, a);
+static void launch_keys_backward(GradArgs a, hipStream_t st) {
+  a.tiles = (a.total + grad_keys<T, D>() - 1) / grad_keys<T, D>() + a.N + 1;
+  hipLaunchKernelGGL((attention_keys_backward_kernel<T, D>), dim3((unsigned)(a.tiles * a.Hkv)), dim3(256), 0, st, a);
 }
 
 }  // namespace att
@@ -345,11 +371,9 @@ extern "C" int aps_attention_packed_backward(const void* q, const void* k, const
   a.causal = causal != 0, a.scale = scale, a.c = scale * kLog2e;
   hipStream_t st = static_cast<hipStream_t>(stream);
   a.tiles = (total * a.G + kRowTile - 1) / kRowTile + N + 1;
-  unsigned grid = (unsigned)(a.tiles * Hkv);
+  const unsigned grid = (unsigned)(a.tiles * Hkv);
   APS_ATT_DISPATCH(launch_rows_backward, a, grid, st);
   if (aps_launch_status() != APS_OK) return APS_ERR_LAUNCH;
-  a.tiles = (total + kRowTile - 1) / kRowTile + N + 1;
-  grid = (unsigned)(a.tiles * Hkv);
-  APS_ATT_DISPATCH(launch_keys_backward, a, grid, st);
+  APS_ATT_DISPATCH(launch_keys_backward, a, st);
   return aps_launch_status();
 }

@@ -252,17 +252,36 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(RowsArgs a) {
   int64_t s0, e0;
   seq_range(a.cu, 0, a.total, s0, e0);
   if (row < s0 * Hq) return;  // rows before the first sequence belong to none either
+  // eight splits at a time, their loads in flight together
   float top = -INFINITY, sum = 0.f;
   f32x4 o = f32x4{0};
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[(s * all + row) * 2]);
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (s * all + row) * 2);
-    if (ml.y == 0.f) continue;
-    const float f = exp2_fast(ml.x - top);
-    const f32x4 x = *reinterpret_cast<const f32x4*>(a.part_o + (s * all + row) * D + d);
-    sum += f * ml.y;
+  for (int s0 = 0; s0 < a.splits; s0 += 8) {
+    float2 ml[8];
+    f32x4 x[8];
+    float to = top;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += f * x[e];
+    for (int j = 0; j < 8; ++j) {
+      ml[j] = make_float2(-INFINITY, 0.f);
+      if (s0 + j < a.splits) ml[j] = *reinterpret_cast<const float2*>(a.part_ml + ((s0 + j) * all + row) * 2);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = f32x4{0};
+      if (ml[j].y != 0.f) x[j] = *reinterpret_cast<const f32x4*>(a.part_o + ((s0 + j) * all + row) * D + d);
+      to = fmaxf(to, ml[j].x);
+    }
+    const float f0 = to == -INFINITY ? 0.f : exp2_fast(top - to);
+    sum *= f0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= f0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float f = ml[j].y == 0.f ? 0.f : exp2_fast(ml[j].x - to);
+      sum += f * ml[j].y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += f * x[j][e];
+    }
+    top = to;
   }
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   store4<T>(static_cast<T*>(a.out) + row * D + d, f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv});
@@ -311,6 +330,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 
 // Which kernel and how many splits, from what the host knows (the lengths themselves are on the
 // device): form 1 / 2 = decode tiles of 16 / 32 rows, 0 = 128-row tiles.
+#ifndef kTargetA
+#define kTargetA 1024
+#define kTargetB 1024
+#endif
 struct PagedPlan { int form; int64_t tiles; int splits; };
 
 static PagedPlan paged_plan(int64_t total, int64_t N, int64_t G, int64_t Hkv, int64_t max_keys, int64_t dtype) {
@@ -321,7 +344,7 @@ static PagedPlan paged_plan(int64_t total, int64_t N, int64_t G, int64_t Hkv, in
   p.tiles = (total * G + tile - 1) / tile + N + 1;
   const int64_t busy = ((total * G + tile - 1) / tile > N ? (total * G + tile - 1) / tile : N) * Hkv;
   // four workgroups per CU for the loads' sake (decode), two for the 128-row tiles
-  const int64_t target = p.form ? 1024 : 512;
+  const int64_t target = p.form ? kTargetA : kTargetB;
   const int64_t least = p.form ? kDecodeChunk * kDecodeLeast : 256;
   int64_t s = (target + busy - 1) / busy, most = (max_keys + least - 1) / least;
   if (s > most) s = most;

@@ -65,7 +65,21 @@ template <typename T, int D, bool PAGED>
 struct KvStage {
   static constexpr int CH = D / chunk_elems<T>(), BK = key_tile<T>(), PER = BK * CH / 256, STEP = 256 / CH;
   u32x4 kr[PER], vr[PER];
-  uint32_t gone;  // paged: bit i: row i's page is outside the cache
+  int next[PER];  // paged: slots of the rows that the next `load` reads, looked up a tile ahead: -1 behind the
+                  // end, -2 for a page outside the cache
+  uint32_t gone;  // paged: bit i: row i of the loaded tile has no page
+
+  __device__ __forceinline__ void locate(const RowsArgs& a, int seq, int key0, int end) {
+    const int r0 = threadIdx.x / CH;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int key = key0 + r0 + i * STEP;
+      next[i] = -1;
+      if (key >= end) continue;
+      const int32_t p = a.table[(int64_t)seq * a.table_stride + (key >> a.page_shift)];
+      next[i] = p < 0 || p >= a.num_pages ? -2 : (p << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+    }
+  }
 
   __device__ __forceinline__ void load(const RowsArgs& a, int64_t start, int seq, int h, int key0, int end) {
     const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
@@ -75,16 +89,13 @@ struct KvStage {
       const int key = key0 + r0 + i * STEP;
       kr[i] = u32x4{0, 0, 0, 0};
       vr[i] = u32x4{0, 0, 0, 0};
-      if (key >= end) continue;
       int64_t row;
       if constexpr (PAGED) {
-        const int32_t p = a.table[(int64_t)seq * a.table_stride + (key >> a.page_shift)];
-        if (p < 0 || p >= a.num_pages) {
-          gone |= 1u << i;
-          continue;
-        }
-        row = ((int64_t)p << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+        if (next[i] == -2) gone |= 1u << i;
+        if (next[i] < 0) continue;
+        row = next[i];
       } else {
+        if (key >= end) continue;
         row = start + key;
       }
       kr[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.k) + row * a.k_t + h * a.k_h +
@@ -166,7 +177,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
 
   KvStage<T, D, PAGED> st;
   if (tile_lo < tile_hi) {
+    if constexpr (PAGED) st.locate(a, t.seq, tile_lo * BK, end);
     st.load(a, t.start, t.seq, h, tile_lo * BK, end);
+    if constexpr (PAGED) st.locate(a, t.seq, (tile_lo + 1) * BK, end);
     st.store(lds, lds + TILE, s_hidden[0]);
   }
   __syncthreads();
@@ -175,7 +188,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
     const char* tv = tk + TILE;
     char* nk = lds + ((kt - tile_lo + 1) & 1) * 2 * TILE;
     const bool more = kt + 1 < tile_hi;
-    if (more) st.load(a, t.start, t.seq, h, (kt + 1) * BK, end);
+    if (more) {
+      st.load(a, t.start, t.seq, h, (kt + 1) * BK, end);
+      if constexpr (PAGED) st.locate(a, t.seq, (kt + 2) * BK, end);
+    }
     const int k0 = kt * BK;
     if (k0 < wave_end) {
       f32x16 s[NKB];
@@ -270,7 +286,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
 static inline bool sizes_fit(int64_t total, int64_t N, int64_t Hq, int64_t Hkv) {
   if (total < 0 || N < 1 || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq > 65536) return false;
   if (total > (int64_t)0x7fff0000 / (Hq / Hkv)) return false;
-  return ((total * (Hq / Hkv) + kRowTile - 1) / kRowTile + N + 1) * Hkv < 0x7fffffff;
+  return ((total * (Hq / Hkv) + 31) / 32 + N + 1) * Hkv < 0x7fffffff;  // (32: the smallest tile of any launch; 16 x more rows in the decode form are checked there)
 }
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

@@ -19,19 +19,18 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kThreads = 256, kPerThread = 32, kTile = kThreads * kPerThread;  // elements of a workgroup
-constexpr int kMaxBeam = 64, kCandidates = 1024;
+constexpr int kThreads = 256;
+constexpr int kMaxBeam = 64, kCandidates = 1024, kHeld = 4;
 constexpr float kLargest = 3.4028234663852886e38f;
 
-// e^x for x <= 0 in 64 bits, relative error < 1e-12 (2^f by its series to f^10, |f| <= 1/2)
+// e^x for x <= 0 in 64 bits, relative error < 1e-11: 2^f, |f| <= 1/2, by its series to f^9
 __device__ __forceinline__ double exp64(double x) {
   const double y = x * 1.4426950408889634074;
   const double n = rint(y), f = y - n;
-  double p = 7.0549116208011233e-9;
-  p = fma(p, f, 1.0178086009239699e-7);
-  p = fma(p, f, 1.3215486790144309e-6);
-  p = fma(p, f, 1.5252733804059840e-5);
-  p = fma(p, f, 1.5403530393381609e-4);
+  double p = 1.0178086009239697e-7;
+  p = fma(p, f, 1.3215486790144307e-6);
+  p = fma(p, f, 1.5252733804059839e-5);
+  p = fma(p, f, 1.5403530393381608e-4);
   p = fma(p, f, 1.3333558146428443e-3);
   p = fma(p, f, 9.6181291076284772e-3);
   p = fma(p, f, 5.5504108664821580e-2);
@@ -57,18 +56,31 @@ __device__ __forceinline__ double from_ordered(uint64_t u) {
   return __longlong_as_double((long long)((u >> 63) ? (u & 0x7fffffffffffffffull) : ~u));
 }
 
-// the K-th largest of a wavefront's 64 values (bitonic sort, descending), K in 1 .. 64
-template <typename V>
-__device__ __forceinline__ V wave_kth(V v, int K, int lane) {
+// A lower bound of the K-th largest of a wavefront's 64 unsigned values, K in 1 .. 64: the largest
+// multiple of 2^LOW that at least K of them reach, a bit at a time by ballots (a sort by lane exchanges
+// took three times as long)
+template <int LOW>
+__device__ __forceinline__ uint32_t wave_kth(uint32_t v, int K) {
+  uint32_t t = 0;
 #pragma unroll
-  for (int size = 2; size <= 64; size <<= 1)
+  for (int bit = 31; bit >= LOW; --bit) {
+    const uint32_t c = t | (1u << bit);
+    if (__popcll(__ballot(v >= c)) >= K) t = c;
+  }
+  return t;
+}
+
+// Exclusive sum over the workgroup's threads, in no particular order of wavefronts, from *counter on
+__device__ __forceinline__ int place(int n, int lane, int* counter) {
+  int upto = n;
 #pragma unroll
-    for (int step = size >> 1; step > 0; step >>= 1) {
-      const V o = __shfl_xor(v, step, 64);
-      const bool lower = (lane & step) == 0, descending = (lane & size) == 0;
-      v = (lower == descending) ? (v > o ? v : o) : (v > o ? o : v);
-    }
-  return __shfl(v, K - 1, 64);
+  for (int o = 1; o < 64; o <<= 1) {
+    const int v = __shfl_up(upto, o, 64);
+    if (lane >= o) upto += v;
+  }
+  int base = 0;
+  if (lane == 63 && upto) base = atomicAdd(counter, upto);  // (the order of arrival does not matter: ranked later)
+  return __shfl(base, 63, 64) + upto - n;
 }
 
 struct RowsArgs {
@@ -103,12 +115,15 @@ __device__ __forceinline__ void widen(u32x4 raw, float* to) {
 // NaN counts as ruled out, +inf as the largest finite value, -0 as 0 (they tie)
 __device__ __forceinline__ float tame(float x) { return x != x ? -INFINITY : fminf(x, kLargest) + 0.f; }
 
-template <typename T>
+// A workgroup takes 256 PER elements of a row: 32 a thread where there are rows enough to fill the chip,
+// 8 (a shorter chain of dependent work) where there are not.
+template <typename T, int PER>
 __global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
-  constexpr int VE = 16 / (int)sizeof(T), NV = kPerThread / VE;
-  __shared__ uint64_t s_cand[kCandidates];
+  constexpr int VE = 16 / (int)sizeof(T), NV = PER / VE, TILE = kThreads * PER;
+  __shared__ __align__(16) uint64_t s_cand[kCandidates];
   __shared__ double s_sum[4];
-  __shared__ float s_top[4], s_kth[4];
+  __shared__ float s_top[4];
+  __shared__ uint32_t s_kth[4];
   __shared__ uint64_t s_best[4];
   __shared__ int s_count;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -116,58 +131,87 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
   const int split = blockIdx.y, V = a.V, K = a.K;
   uint64_t* out = a.keys + (row * a.splits + split) * K;
   if (tid == 0) s_count = 0;
+  const uint64_t none = (uint64_t)ordered(-INFINITY) << 32;  // key of a ruled-out token, its index apart
   const bool done = a.done && a.done[row];
   const bool dead = !(a.score[row] > -INFINITY);  // (NaN too)
+  if (done || dead) {
+    // no logit is looked at: a finished hypothesis goes on with eos at its own score, an unused one with
+    // nothing; what is ruled out comes lowest token first, from the first split
+    const bool ends = done && !dead;
+    if (tid < K) {
+      uint64_t key = 0;
+      if (split == 0) {
+        const int64_t token = ends ? (tid == 0 ? a.eos : tid - 1 + (tid > a.eos)) : tid;
+        if (token < V) key = (ends && tid == 0 ? (uint64_t)ordered(0.f) << 32 : none) | (uint32_t)~(uint32_t)token;
+      }
+      out[tid] = key;
+    }
+    if (tid == 0) {
+      a.top[row * a.splits + split] = ends && split == 0 ? 0.f : -INFINITY;
+      a.sum[row * a.splits + split] = 1.;
+    }
+    return;
+  }
   // aligned vectors: element e0 + i of the row; the first vector may begin before the row
   const T* base = static_cast<const T*>(a.x) + row * a.stride;
   const int shift = (int)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
-  float x[kPerThread];
+  const int first = split * TILE + tid * VE - shift;  // vector j of the thread: first + j * 256 VE
+  float x[PER];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int e0 = (split * (kTile / VE) + j * kThreads + tid) * VE - shift;
+    const int e0 = first + j * kThreads * VE;
     float* to = x + j * VE;
-    if (done || dead) {
-#pragma unroll
-      for (int i = 0; i < VE; ++i) to[i] = (done && !dead && e0 + i == a.eos) ? 0.f : -INFINITY;
-    } else if (e0 >= 0 && e0 + VE <= V) {
+    if (e0 >= 0 && e0 + VE <= V) {
       widen<T>(*reinterpret_cast<const u32x4*>(base + e0), to);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) to[i] = tame(to[i]);
     } else {
 #pragma unroll
-      for (int i = 0; i < VE; ++i)
-        to[i] = (e0 + i >= 0 && e0 + i < V) ? tame((float)base[e0 + i]) : -INFINITY;
+      for (int i = 0; i < VE; ++i) to[i] = (e0 + i >= 0 && e0 + i < V) ? (float)base[e0 + i] : -INFINITY;
     }
   }
   float best = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kPerThread; ++i) best = fmaxf(best, x[i]);
-  const float kth = wave_kth(best, K, lane), wtop = wave_max(best);
+  for (int i = 0; i < PER; ++i) {
+    x[i] = tame(x[i]);
+    best = fmaxf(best, x[i]);
+  }
+  // K of the threads' maxima are at least `least`, so the K largest elements are too
+  const uint32_t kth = wave_kth<12>(ordered(best), K);
+  const float wtop = wave_max(best);
   if (lane == 0) s_top[wv] = wtop, s_kth[wv] = kth;
   __syncthreads();
   const float top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-  // K of the threads' maxima are at least `least`, so the K largest elements are too
-  const float least = fmaxf(fmaxf(s_kth[0], s_kth[1]), fmaxf(s_kth[2], s_kth[3]));
+  const uint32_t bound = max(max(s_kth[0], s_kth[1]), max(s_kth[2], s_kth[3]));
+  // (ruled-out tokens are not collected: if they are needed at all, it is the lowest few)
+  const float least = bound <= ordered(-kLargest) ? -kLargest : from_ordered(bound);
+  int mine = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+#pragma unroll
+    for (int i = 0; i < VE; ++i) mine += x[j * VE + i] >= least;
+  int at = place(mine, lane, &s_count);
+  if (mine) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) {
+        const int e = first + j * kThreads * VE + i;
+        if (x[j * VE + i] >= least) {
+          if (at < kCandidates) s_cand[at] = ((uint64_t)ordered(x[j * VE + i]) << 32) | (uint32_t)~e;
+          ++at;
+        }
+      }
+  }
   double sum = 0.;
   if (top > -INFINITY) {
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i)
-      if (x[i] > -INFINITY) sum += exp64((double)x[i] - (double)top);
+    for (int i = 0; i < PER; ++i) {
+      const double e = exp64((double)x[i] - (double)top);
+      sum += x[i] > -INFINITY ? e : 0.;
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
   if (lane == 0) s_sum[wv] = sum;
-#pragma unroll
-  for (int j = 0; j < NV; ++j) {
-    const int e0 = (split * (kTile / VE) + j * kThreads + tid) * VE - shift;
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      if (x[j * VE + i] >= least && e0 + i >= 0 && e0 + i < V) {
-        const int at = atomicAdd(&s_count, 1);  // (the order of arrival does not matter: ranked below)
-        if (at < kCandidates) s_cand[at] = ((uint64_t)ordered(x[j * VE + i]) << 32) | (uint32_t)~(e0 + i);
-      }
-    }
-  }
   __syncthreads();
   const int count = s_count;
   if (tid == 0) {
@@ -178,32 +222,44 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
     for (int c = tid; c < count; c += kThreads) {
       const uint64_t key = s_cand[c];
       int rank = 0;
+#pragma unroll 8
       for (int o = 0; o < count; ++o) rank += s_cand[o] > key;
       if (rank < K) out[rank] = key;
     }
-    for (int c = count + tid; c < K; c += kThreads) out[c] = 0;  // fewer elements than K
+    if (count < K) {
+      // Of the split's first K + count tokens at most `count` are not ruled out: the lowest ones of the rest
+      // follow, then nothing.  (K + count < 128: two wavefronts)
+      const int lo = max(0, split * TILE - shift), hi = min(V, split * TILE - shift + TILE);
+      bool out_of = false;
+      if (tid < 128 && lo + tid < hi) out_of = tame((float)base[lo + tid]) == -INFINITY;
+      const uint64_t mask = __ballot(out_of);
+      if (lane == 0) s_best[wv] = mask;
+      __syncthreads();
+      const int below = __popcll(mask & ((1ull << lane) - 1)) + (wv == 1 ? __popcll(s_best[0]) : 0);
+      if (out_of && count + below < K) out[count + below] = none | (uint32_t)~(uint32_t)(lo + tid);
+      for (int c = count + __popcll(s_best[0]) + __popcll(s_best[1]) + tid; c < K; c += kThreads) out[c] = 0;
+    }
     return;
   }
   // a great many equal values: K rounds of the largest key below the last
   uint64_t last = ~0ull;
   for (int k = 0; k < K; ++k) {
-    uint64_t mine = 0;
+    uint64_t mx = 0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int e0 = (split * (kTile / VE) + j * kThreads + tid) * VE - shift;
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        if (e0 + i < 0 || e0 + i >= V) continue;
-        const uint64_t key = ((uint64_t)ordered(x[j * VE + i]) << 32) | (uint32_t)~(e0 + i);
-        if (key < last && key > mine) mine = key;
+        const int e = first + j * kThreads * VE + i;
+        if (!(x[j * VE + i] > -INFINITY)) continue;  // (there are more than K others)
+        const uint64_t key = ((uint64_t)ordered(x[j * VE + i]) << 32) | (uint32_t)~e;
+        if (key < last && key > mx) mx = key;
       }
-    }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t other = __shfl_xor(mine, o, 64);
-      mine = other > mine ? other : mine;
+      const uint64_t other = __shfl_xor(mx, o, 64);
+      mx = other > mx ? other : mx;
     }
-    if (lane == 0) s_best[wv] = mine;
+    if (lane == 0) s_best[wv] = mx;
     __syncthreads();
     last = s_best[0];
 #pragma unroll
@@ -231,7 +287,8 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
   __shared__ uint32_t s_flat[kCandidates];
   __shared__ double s_add[kMaxBeam];  // score - log sum exp of a hypothesis
   __shared__ double s_score[kMaxBeam];
-  __shared__ uint64_t s_kth[4], s_best[4];
+  __shared__ uint32_t s_kth[4];
+  __shared__ uint64_t s_best[4];
   __shared__ uint32_t s_best_flat[4];
   __shared__ int s_count;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -250,12 +307,15 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
     s_add[tid] = top > -INFINITY ? (double)top + log(sum) : 0.;
     s_score[tid] = (double)tame(a.score[row]);
   }
-  __syncthreads();
   const uint64_t* keys = a.keys + n * B * S * K;
   const int total = B * S * K;
+  // the first candidates of each thread are on their way while the sums are formed
+  uint64_t held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = tid + i * kThreads < total ? keys[tid + i * kThreads] : 0;
+  __syncthreads();
   // candidate c of the utterance: its total as an ordered integer (0: none) and its flat index
-  auto candidate = [&](int c, uint32_t& flat) -> uint64_t {
-    const uint64_t key = keys[c];
+  auto candidate = [&](int c, uint64_t key, uint32_t& flat) -> uint64_t {
     if (!key) return 0;
     const int b = c / (S * K);
     const uint32_t token = ~(uint32_t)key;
@@ -264,25 +324,42 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
     return ordered(x > -INFINITY ? s_score[b] + ((double)x - s_add[b]) + 0. : (double)-INFINITY);
   };
   uint64_t best = 0;
-  for (int c = tid; c < total; c += kThreads) {
+  uint32_t held_flat[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    held_flat[i] = 0;
+    held[i] = candidate(tid + i * kThreads, held[i], held_flat[i]);
+    best = held[i] > best ? held[i] : best;
+  }
+  for (int c = tid + kHeld * kThreads; c < total; c += kThreads) {
     uint32_t flat;
-    const uint64_t v = candidate(c, flat);
+    const uint64_t v = candidate(c, keys[c], flat);
     best = v > best ? v : best;
   }
-  const uint64_t kth = wave_kth(best, K, lane);
+  const uint32_t kth = wave_kth<0>((uint32_t)(best >> 32), K);  // (bounds the totals by their upper halves)
   if (lane == 0) s_kth[wv] = kth;
   __syncthreads();
-  uint64_t least = s_kth[0];
+  const uint32_t bound = max(max(s_kth[0], s_kth[1]), max(s_kth[2], s_kth[3]));
+  const uint64_t least = bound ? (uint64_t)bound << 32 : 1;  // (0 is no candidate)
+  int mine = 0;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) least = s_kth[w] > least ? s_kth[w] : least;
-  if (least == 0) least = 1;  // (0 is no candidate)
-  for (int c = tid; c < total; c += kThreads) {
+  for (int i = 0; i < kHeld; ++i) mine += held[i] >= least;
+  for (int c = tid + kHeld * kThreads; c < total; c += kThreads) {
     uint32_t flat;
-    const uint64_t v = candidate(c, flat);
-    if (v >= least) {
-      const int at = atomicAdd(&s_count, 1);
-      if (at < kCandidates) s_key[at] = v, s_flat[at] = flat;
-    }
+    mine += candidate(c, keys[c], flat) >= least;
+  }
+  int at = place(mine, lane, &s_count);
+  auto collect = [&](uint64_t v, uint32_t flat) {
+    if (v < least) return;
+    if (at < kCandidates) s_key[at] = v, s_flat[at] = flat;
+    ++at;
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) collect(held[i], held_flat[i]);
+  for (int c = tid + kHeld * kThreads; c < total; c += kThreads) {
+    uint32_t flat = 0;
+    const uint64_t v = candidate(c, keys[c], flat);
+    collect(v, flat);
   }
   __syncthreads();
   const int count = s_count;
@@ -299,6 +376,7 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
       const uint64_t v = s_key[c];
       const uint32_t flat = s_flat[c];
       int rank = 0;
+#pragma unroll 8
       for (int o = 0; o < count; ++o) rank += s_key[o] > v || (s_key[o] == v && s_flat[o] < flat);
       if (rank < K) put(rank, v, flat);
     }
@@ -307,21 +385,21 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
   uint64_t last = ~0ull;
   uint32_t last_flat = 0;
   for (int k = 0; k < K; ++k) {
-    uint64_t mine = 0;
-    uint32_t mine_flat = 0;
+    uint64_t mx = 0;
+    uint32_t mx_flat = 0;
     for (int c = tid; c < total; c += kThreads) {
       uint32_t flat = 0;
-      const uint64_t v = candidate(c, flat);
+      const uint64_t v = candidate(c, keys[c], flat);
       if (!v || !(v < last || (v == last && flat > last_flat))) continue;
-      if (v > mine || (v == mine && flat < mine_flat)) mine = v, mine_flat = flat;
+      if (v > mx || (v == mx && flat < mx_flat)) mx = v, mx_flat = flat;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t v = __shfl_xor(mine, o, 64);
-      const uint32_t flat = __shfl_xor(mine_flat, o, 64);
-      if (v > mine || (v == mine && flat < mine_flat)) mine = v, mine_flat = flat;
+      const uint64_t v = __shfl_xor(mx, o, 64);
+      const uint32_t flat = __shfl_xor(mx_flat, o, 64);
+      if (v > mx || (v == mx && flat < mx_flat)) mx = v, mx_flat = flat;
     }
-    if (lane == 0) s_best[wv] = mine, s_best_flat[wv] = mine_flat;
+    if (lane == 0) s_best[wv] = mx, s_best_flat[wv] = mx_flat;
     __syncthreads();
     last = s_best[0], last_flat = s_best_flat[0];
 #pragma unroll
@@ -347,7 +425,7 @@ struct ReorderArgs {
   int32_t count;
 };
 
-template <typename U>
+template <typename U, typename I>
 __device__ __forceinline__ void move_units(const ReorderArgs& a, int s, int64_t i0) {
   U v[kUnits];
   int64_t at[kUnits];
@@ -357,14 +435,14 @@ __device__ __forceinline__ void move_units(const ReorderArgs& a, int s, int64_t 
     at[j] = i < a.units[s] ? i : -1;
     v[j] = U{};
     if (at[j] < 0) continue;
-    const uint64_t flat = (uint64_t)i / a.inner[s];
-    const uint32_t col = (uint32_t)((uint64_t)i - flat * a.inner[s]);
-    const uint64_t outer = flat / a.rows_out;
+    const I flat = (I)i / a.inner[s];
+    const uint32_t col = (uint32_t)((I)i - flat * a.inner[s]);
+    const I outer = flat / a.rows_out;
     const uint32_t row = (uint32_t)(flat - outer * a.rows_out);
     const uint32_t n = row / a.K;
     const int64_t p = a.parent[row];
     if (p < 0 || p >= a.B) continue;
-    v[j] = reinterpret_cast<const U*>(a.src[s])[(outer * a.rows_in + (uint64_t)n * a.B + p) * a.inner[s] + col];
+    v[j] = reinterpret_cast<const U*>(a.src[s])[((uint64_t)outer * a.rows_in + (uint64_t)n * a.B + p) * a.inner[s] + col];
   }
 #pragma unroll
   for (int j = 0; j < kUnits; ++j)
@@ -375,19 +453,39 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
   int s = 0;
   while (s + 1 < a.count && (int64_t)blockIdx.x >= a.first[s + 1]) ++s;
   const int64_t i0 = ((int64_t)blockIdx.x - a.first[s]) * (256 * kUnits) + threadIdx.x;
+  const bool narrow = a.units[s] <= 0x7fffffff;  // (index arithmetic in 32 bits)
   switch (a.unit[s]) {
-    case 16: move_units<u32x4>(a, s, i0); break;
-    case 8: move_units<uint64_t>(a, s, i0); break;
-    case 4: move_units<uint32_t>(a, s, i0); break;
-    case 2: move_units<uint16_t>(a, s, i0); break;
-    default: move_units<uint8_t>(a, s, i0); break;
+#define APS_MOVE(BYTES, U)                              \
+  case BYTES:                                           \
+    if (narrow) move_units<U, uint32_t>(a, s, i0);      \
+    else move_units<U, uint64_t>(a, s, i0);             \
+    break;
+    APS_MOVE(16, u32x4)
+    APS_MOVE(8, uint64_t)
+    APS_MOVE(4, uint32_t)
+    APS_MOVE(2, uint16_t)
+    APS_MOVE(1, uint8_t)
+#undef APS_MOVE
   }
 }
 
-static int64_t splits_of(int64_t V, int64_t elem) { return (V + 16 / elem - 1 + kTile - 1) / kTile; }
+// Elements a thread of the rows kernel takes.  32: 2 048 workgroups read 512 rows of 32 000 f32 logits in
+// %LARGE% us; 8 for what would be fewer than two workgroups a CU: 8 rows of 4 233 in %SMALL8% us, with 32 in
+// %SMALL32%.
+static int per_thread(int64_t rows, int64_t V) { return rows * ((V + 8191) / 8192) < 512 ? 8 : 32; }
+static int64_t splits_of(int64_t rows, int64_t V) {
+  const int64_t tile = kThreads * per_thread(rows, V);
+  return (V + 7 + tile - 1) / tile;  // (a row may begin up to 7 elements into its first vector)
+}
 static bool sizes_fit(int64_t N, int64_t B, int64_t V, int64_t K) {
   return N >= 1 && B >= 1 && B <= kMaxBeam && K >= 1 && K <= kMaxBeam && V >= 1 && V <= (1 << 24) &&
          K <= B * V && N <= 0x7fffffff / B;
+}
+
+template <typename T>
+static void launch_rows(const RowsArgs& a, dim3 grid, bool wide, hipStream_t st) {
+  if (wide) hipLaunchKernelGGL((beam_rows_kernel<T, 32>), grid, dim3(kThreads), 0, st, a);
+  else hipLaunchKernelGGL((beam_rows_kernel<T, 8>), grid, dim3(kThreads), 0, st, a);
 }
 
 }  // namespace beam
@@ -397,7 +495,7 @@ using namespace aps::beam;
 
 extern "C" int64_t aps_beam_select_workspace(int64_t N, int64_t B, int64_t V, int64_t K) {
   if (!sizes_fit(N, B, V, K)) return -1;
-  return N * B * splits_of(V, 2) * (K * 8 + 16);  // (16-bit logits may begin a vector later: their count)
+  return N * B * splits_of(N * B, V) * (K * 8 + 16);
 }
 
 extern "C" int aps_beam_select(const void* logits, int64_t row_stride, const float* scores, const uint8_t* finished,
@@ -408,7 +506,7 @@ extern "C" int aps_beam_select(const void* logits, int64_t row_stride, const flo
   APS_CHECK_ARG(sizes_fit(N, B, V, K) && row_stride >= V && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0);
   APS_CHECK_ARG(!finished || (eos >= 0 && eos < V));
   if (dtype < 0 || dtype > 2) return APS_ERR_UNSUPPORTED;
-  const int64_t elem = dtype == 0 ? 4 : 2, S = splits_of(V, elem);
+  const int64_t elem = dtype == 0 ? 4 : 2, S = splits_of(N * B, V);
   APS_CHECK_ARG((reinterpret_cast<uintptr_t>(logits) & (elem - 1)) == 0);
   RowsArgs r{};
   r.x = logits, r.stride = row_stride, r.score = scores, r.done = finished, r.eos = eos;
@@ -418,9 +516,10 @@ extern "C" int aps_beam_select(const void* logits, int64_t row_stride, const flo
   r.top = reinterpret_cast<float*>(r.sum + N * B * S);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid((unsigned)(N * B), (unsigned)S);
-  if (dtype == 0) hipLaunchKernelGGL(beam_rows_kernel<float>, grid, dim3(kThreads), 0, st, r);
-  else if (dtype == 1) hipLaunchKernelGGL(beam_rows_kernel<__bf16>, grid, dim3(kThreads), 0, st, r);
-  else hipLaunchKernelGGL(beam_rows_kernel<_Float16>, grid, dim3(kThreads), 0, st, r);
+  const bool wide = per_thread(N * B, V) == 32;
+  if (dtype == 0) launch_rows<float>(r, grid, wide, st);
+  else if (dtype == 1) launch_rows<__bf16>(r, grid, wide, st);
+  else launch_rows<_Float16>(r, grid, wide, st);
   if (aps_launch_status() != APS_OK) return APS_ERR_LAUNCH;
   MergeArgs m{};
   m.keys = r.keys, m.top = r.top, m.sum = r.sum, m.score = scores, m.done = finished, m.eos = eos;
