@@ -70,50 +70,62 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   const float lse = live ? a.lse[at] : INFINITY;
   if (live && half == 0) a.delta[at] = delta;
 
-  RowsArgs kvargs;
-  kvargs.k = a.k, kvargs.v = a.v, kvargs.k_t = a.k_t, kvargs.k_h = a.k_h, kvargs.v_t = a.v_t, kvargs.v_h = a.v_h;
   f32x16 acc[NDB];
 #pragma unroll
   for (int d = 0; d < NDB; ++d) acc[d] = f32x16{0};
   const int tile_hi = (end + BK - 1) / BK;
+  const T* kb = static_cast<const T*>(a.k) + h * a.k_h + t.start * a.k_t;
+  const T* vb = static_cast<const T*>(a.v) + h * a.v_h + t.start * a.v_t;
   KvStage<T, D, false> st;
-  st.load(kvargs, t.start, t.seq, h, 0, end);
-  st.store(lds, lds + TILE, nullptr);
+  st.load(kb, a.k_t, 0, end);
+  st.store(lds);
+  st.load(vb, a.v_t, 0, end);
+  st.store(lds + TILE);
   __syncthreads();
   for (int kt = 0; kt < tile_hi; ++kt) {
     const char* tk = lds + (kt & 1) * 2 * TILE;
     const char* tv = tk + TILE;
     char* nk = lds + ((kt + 1) & 1) * 2 * TILE;
     const bool more = kt + 1 < tile_hi;
-    if (more) st.load(kvargs, t.start, t.seq, h, (kt + 1) * BK, end);
     const int k0 = kt * BK;
-    if (k0 < wave_end) {
-      const bool edge = k0 + BK - 1 > wave_min;
+    const bool sees = k0 < wave_end, edge = k0 + BK - 1 > wave_min;
+    // 32 keys at a time; the next tile's keys are in flight during the first half, its values during the second
+    if (more) st.load(kb, a.k_t, k0 + BK, end);
 #pragma unroll
-      for (int b = 0; b < NKB; ++b) {
-        f32x16 s = f32x16{0}, g = f32x16{0};
+    for (int b = 0; b < NKB; ++b) {
+      if (b == 1 && more) {
+        st.store(nk);
+        st.load(vb, a.v_t, k0 + BK, end);
+      }
+      f32x16 s = f32x16{0}, g = f32x16{0};
+      if (sees) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
           s = mma<T>(frag<T, D>(tk, b * 32 + (lane & 31), i, half), qf[i], s);
           g = mma<T>(frag<T, D>(tv, b * 32 + (lane & 31), i, half), gf[i], g);
         }
-        float p[16];
+      }
+      if (NKB == 1 && more) {  // (a single half: the values follow behind the first two products)
+        st.store(nk);
+        st.load(vb, a.v_t, k0 + BK, end);
+      }
+      if (!sees) continue;
+      float p[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = exp2_fast(fmaf(s[i], a.c, -lse)) * (g[i] - delta);
-        if (edge) {
+      for (int i = 0; i < 16; ++i) p[i] = exp2_fast(fmaf(s[i], a.c, -lse)) * (g[i] - delta);
+      if (edge) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (k0 + b * 32 + result_row(i, half) > pos) p[i] = 0.f;
-        }
+        for (int i = 0; i < 16; ++i)
+          if (k0 + b * 32 + result_row(i, half) > pos) p[i] = 0.f;
+      }
 #pragma unroll
-        for (int i = 0; i < NPS; ++i) {
-          const u32x4 pf = pack<T>(p + i * (KS / 2));
+      for (int i = 0; i < NPS; ++i) {
+        const u32x4 pf = pack<T>(p + i * (KS / 2));
 #pragma unroll
-          for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(frag_t<T, D>(tk, b * 32, i, d, lane), pf, acc[d]);
-        }
+        for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(frag_t<T, D>(tk, b * 32, i, d, lane), pf, acc[d]);
       }
     }
-    if (more) st.store(nk, nk + TILE, nullptr);
+    if (more) st.store(nk + TILE);
     __syncthreads();
   }
   if (!live) return;
@@ -177,26 +189,50 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
   u32x4 qr[PER], gr[PER];
   float r_lse = INFINITY, r_delta = 0.f;
   int r_pos = -1;
-  auto load = [&](int r0) {
+  // causal: the rows before token `tile0` see none of the tile's keys
+  const int lo = a.causal ? (tile0 * a.G) / BR : 0, hi = (rows + BR - 1) / BR;
+  // row i of the thread, and the row whose statistics it carries, as (token, head of the group) with the
+  // offsets they stand for; BR rows on: two additions instead of a division and four products
+  const int step_tok = BR / a.G, step_head = BR - step_tok * a.G;
+  const int64_t q_step = step_tok * a.q_t + step_head * a.q_h, q_wrap = a.q_t - a.G * a.q_h;
+  const int64_t g_step = step_tok * a.go_t + step_head * a.go_h, g_wrap = a.go_t - a.G * a.go_h;
+  const T* qp[PER];
+  const T* gp[PER];
+  int row_head[PER], row_at = lo * BR, s_head, s_tok;
+  {
+    const int c = threadIdx.x % CH;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int row = r0 + threadIdx.x / CH + i * STEP, c = threadIdx.x % CH;
+      const int row = row_at + threadIdx.x / CH + i * STEP, tok = row / a.G;
+      row_head[i] = row - tok * a.G;
+      qp[i] = static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + (h * a.G + row_head[i]) * a.q_h + c * E;
+      gp[i] = static_cast<const T*>(a.go) + (t.start + tok) * a.go_t + (h * a.G + row_head[i]) * a.go_h + c * E;
+    }
+    const int row = row_at + (threadIdx.x & (BR - 1));
+    s_tok = row / a.G, s_head = row - s_tok * a.G;
+  }
+  auto load = [&]() {  // the next BR rows
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
       qr[i] = gr[i] = u32x4{0, 0, 0, 0};
-      if (row < rows) {
-        const int tok = row / a.G, head = h * a.G + row - tok * a.G;
-        qr[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + head * a.q_h + c * E);
-        gr[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.go) + (t.start + tok) * a.go_t + head * a.go_h + c * E);
+      if (row_at + (int)threadIdx.x / CH + i * STEP < rows) {
+        qr[i] = *reinterpret_cast<const u32x4*>(qp[i]);
+        gr[i] = *reinterpret_cast<const u32x4*>(gp[i]);
       }
+      row_head[i] += step_head;
+      qp[i] += q_step, gp[i] += g_step;
+      if (row_head[i] >= a.G) row_head[i] -= a.G, qp[i] += q_wrap, gp[i] += g_wrap;
     }
     if (threadIdx.x < BR) {
-      const int row = r0 + threadIdx.x;
       r_lse = INFINITY, r_delta = 0.f, r_pos = -1;
-      if (row < rows) {
-        const int tok = row / a.G;
-        const int64_t at = (t.start + tok) * Hq + h * a.G + row - tok * a.G;
-        r_lse = a.lse[at], r_delta = a.delta[at], r_pos = a.causal ? tok : t.len - 1;
+      if (row_at + (int)threadIdx.x < rows) {
+        const int64_t at = (t.start + s_tok) * Hq + h * a.G + s_head;
+        r_lse = a.lse[at], r_delta = a.delta[at], r_pos = a.causal ? s_tok : t.len - 1;
       }
+      s_head += step_head, s_tok += step_tok;
+      if (s_head >= a.G) s_head -= a.G, ++s_tok;
     }
+    row_at += BR;
   };
   auto store = [&](int buf) {
     char* tq = lds + buf * 2 * TILE;
@@ -209,9 +245,7 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
     if (threadIdx.x < BR)
       s_lse[buf][threadIdx.x] = r_lse, s_delta[buf][threadIdx.x] = r_delta, s_pos[buf][threadIdx.x] = r_pos;
   };
-  // causal: the rows before token `tile0` see none of the tile's keys
-  const int lo = a.causal ? (tile0 * a.G) / BR : 0, hi = (rows + BR - 1) / BR;
-  load(lo * BR);
+  load();
   store(0);
   __syncthreads();
   for (int rt = lo; rt < hi; ++rt) {
@@ -219,7 +253,7 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
     const char* tq = lds + buf * 2 * TILE;
     const char* tg = tq + TILE;
     const bool more = rt + 1 < hi;
-    if (more) load((rt + 1) * BR);
+    if (more) load();
     const int b = wv / KG;  // this wavefront's block of 32 rows
     const int r0 = rt * BR + b * 32;
     // (every wavefront multiplies every block, masked ones too: a branch around the products makes the

@@ -58,60 +58,52 @@ __device__ __forceinline__ void clear_rows(T* out, const Index& cu, int64_t N, i
   }
 }
 
-// one tile of keys / values on its way from global memory to LDS: thread t carries chunk t % CH of rows
-// t / CH + i * (256 / CH); rows outside [0, end) are zeros, so nothing that lies there (an unwritten
-// page, the next sequence) can reach a product
+// The next tile of keys (then of values, in the same registers) on its way from global memory to LDS:
+// thread t carries chunk t % CH of rows t / CH + i * (256 / CH).  Rows outside [0, end) are zeros, so nothing
+// that lies there (an unwritten page, the next sequence) can reach a product.  Keys are in flight during a
+// tile's scores and values during its second product: half the registers of both at once, which is
+// what keeps D = 128 in 256 of them (a spilled register's reload waits for every load issued before it).
 template <typename T, int D, bool PAGED>
 struct KvStage {
   static constexpr int CH = D / chunk_elems<T>(), BK = key_tile<T>(), PER = BK * CH / 256, STEP = 256 / CH;
-  u32x4 kr[PER], vr[PER];
-  int next[PER];  // paged: slots of the rows that the next `load` reads, looked up a tile ahead: -1 behind the
-                  // end, -2 for a page outside the cache
-  uint32_t gone;  // paged: bit i: row i of the loaded tile has no page
+  u32x4 r[PER];
+  int slot[PER];  // paged: slots of the tile's rows, looked up a tile ahead of the loads: -1 behind the end, -2
+                  // for a page outside the cache
 
   __device__ __forceinline__ void locate(const RowsArgs& a, int seq, int key0, int end) {
-    const int r0 = threadIdx.x / CH;
+    if constexpr (PAGED) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int key = key0 + r0 + i * STEP;
-      next[i] = -1;
-      if (key >= end) continue;
-      const int32_t p = a.table[(int64_t)seq * a.table_stride + (key >> a.page_shift)];
-      next[i] = p < 0 || p >= a.num_pages ? -2 : (p << a.page_shift) + (key & ((1 << a.page_shift) - 1));
-    }
-  }
-
-  __device__ __forceinline__ void load(const RowsArgs& a, int64_t start, int seq, int h, int key0, int end) {
-    const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
-    gone = 0;
-#pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int key = key0 + r0 + i * STEP;
-      kr[i] = u32x4{0, 0, 0, 0};
-      vr[i] = u32x4{0, 0, 0, 0};
-      int64_t row;
-      if constexpr (PAGED) {
-        if (next[i] == -2) gone |= 1u << i;
-        if (next[i] < 0) continue;
-        row = next[i];
-      } else {
+      for (int i = 0; i < PER; ++i) {
+        const int key = key0 + (int)threadIdx.x / CH + i * STEP;
+        slot[i] = -1;
         if (key >= end) continue;
-        row = start + key;
+        const int32_t p = a.table[(int64_t)seq * a.table_stride + (key >> a.page_shift)];
+        slot[i] = p < 0 || p >= a.num_pages ? -2 : (p << a.page_shift) + (key & ((1 << a.page_shift) - 1));
       }
-      kr[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.k) + row * a.k_t + h * a.k_h +
-                                              c * chunk_elems<T>());
-      vr[i] = *reinterpret_cast<const u32x4*>(static_cast<const T*>(a.v) + row * a.v_t + h * a.v_h +
-                                              c * chunk_elems<T>());
     }
   }
-  __device__ __forceinline__ void store(char* tk, char* tv, uint8_t* hidden) const {
+  // base: the key head's row 0 (packed: of the sequence); row_stride in elements
+  __device__ __forceinline__ void load(const T* base, int64_t row_stride, int key0, int end) {
     const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if (PAGED && c == 0) hidden[r0 + i * STEP] = (gone >> i) & 1;
-      const int at = tile_at<T, D>(r0 + i * STEP, c);
-      *reinterpret_cast<u32x4*>(tk + at) = kr[i];
-      *reinterpret_cast<u32x4*>(tv + at) = vr[i];
+      const int row = PAGED ? slot[i] : key0 + r0 + i * STEP;
+      r[i] = u32x4{0, 0, 0, 0};
+      if (PAGED ? row >= 0 : row < end)
+        r[i] = *reinterpret_cast<const u32x4*>(base + row * row_stride + c * chunk_elems<T>());
+    }
+  }
+  __device__ __forceinline__ void store(char* tile) const {
+    const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) *reinterpret_cast<u32x4*>(tile + tile_at<T, D>(r0 + i * STEP, c)) = r[i];
+  }
+  __device__ __forceinline__ void mark(uint8_t* hidden) const {
+    if constexpr (PAGED) {
+      if (threadIdx.x % CH == 0) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) hidden[threadIdx.x / CH + i * STEP] = slot[i] == -2;
+      }
     }
   }
 };
@@ -175,25 +167,30 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   for (int d = 0; d < NDB; ++d) acc[d] = f32x16{0};
   float m = -INFINITY, l = 0.f;  // m: the reference the weights are taken against, in units of log2
 
+  const T* kb = static_cast<const T*>(a.k) + h * a.k_h + (PAGED ? 0 : t.start * a.k_t);
+  const T* vb = static_cast<const T*>(a.v) + h * a.v_h + (PAGED ? 0 : t.start * a.v_t);
   KvStage<T, D, PAGED> st;
   if (tile_lo < tile_hi) {
-    if constexpr (PAGED) st.locate(a, t.seq, tile_lo * BK, end);
-    st.load(a, t.start, t.seq, h, tile_lo * BK, end);
-    if constexpr (PAGED) st.locate(a, t.seq, (tile_lo + 1) * BK, end);
-    st.store(lds, lds + TILE, s_hidden[0]);
+    st.locate(a, t.seq, tile_lo * BK, end);
+    st.load(kb, a.k_t, tile_lo * BK, end);
+    st.store(lds);
+    st.mark(s_hidden[0]);
+    st.load(vb, a.v_t, tile_lo * BK, end);
+    st.locate(a, t.seq, (tile_lo + 1) * BK, end);
+    st.store(lds + TILE);
   }
   __syncthreads();
   for (int kt = tile_lo; kt < tile_hi; ++kt) {
-    const char* tk = lds + ((kt - tile_lo) & 1) * 2 * TILE;
+    const int buf = (kt - tile_lo) & 1;
+    const char* tk = lds + buf * 2 * TILE;
     const char* tv = tk + TILE;
-    char* nk = lds + ((kt - tile_lo + 1) & 1) * 2 * TILE;
+    char* nk = lds + (buf ^ 1) * 2 * TILE;
     const bool more = kt + 1 < tile_hi;
-    if (more) {
-      st.load(a, t.start, t.seq, h, (kt + 1) * BK, end);
-      if constexpr (PAGED) st.locate(a, t.seq, (kt + 2) * BK, end);
-    }
     const int k0 = kt * BK;
-    if (k0 < wave_end) {
+    const bool sees = k0 < wave_end;
+    u32x4 pf[NKB * NPS];
+    if (more) st.load(kb, a.k_t, k0 + BK, end);
+    if (sees) {
       f32x16 s[NKB];
 #pragma unroll
       for (int b = 0; b < NKB; ++b) s[b] = f32x16{0};
@@ -209,7 +206,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
             if (k0 + b * 32 + result_row(i, half) > pos) s[b][i] = -INFINITY;
       }
       if constexpr (PAGED) {
-        const uint64_t hidden = __ballot(lane < BK && s_hidden[(kt - tile_lo) & 1][lane]);
+        const uint64_t hidden = __ballot(lane < BK && s_hidden[buf][lane]);
         if (hidden) {
 #pragma unroll
           for (int b = 0; b < NKB; ++b)
@@ -244,14 +241,24 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
           l += p[i];
         }
 #pragma unroll
-        for (int i = 0; i < NPS; ++i) {
-          const u32x4 pf = pack<T>(p + i * (KS / 2));
-#pragma unroll
-          for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(frag_t<T, D>(tv, b * 32, i, d, lane), pf, acc[d]);
-        }
+        for (int i = 0; i < NPS; ++i) pf[b * NPS + i] = pack<T>(p + i * (KS / 2));
       }
     }
-    if (more) st.store(nk, nk + TILE, s_hidden[(kt - tile_lo + 1) & 1]);
+    if (more) {
+      st.store(nk);
+      st.mark(s_hidden[buf ^ 1]);
+      st.load(vb, a.v_t, k0 + BK, end);
+      st.locate(a, t.seq, k0 + 2 * BK, end);
+    }
+    if (sees) {
+#pragma unroll
+      for (int b = 0; b < NKB; ++b)
+#pragma unroll
+        for (int i = 0; i < NPS; ++i)
+#pragma unroll
+          for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(frag_t<T, D>(tv, b * 32, i, d, lane), pf[b * NPS + i], acc[d]);
+    }
+    if (more) st.store(nk + TILE);
     __syncthreads();
   }
   l += __shfl_xor(l, 32, 64);
