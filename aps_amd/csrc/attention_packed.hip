@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   constexpr int BK = key_tile<T>(), E = chunk_elems<T>(), KS = 2 * E, NS = D / KS, NKB = BK / 32, NDB = D / 32;
   constexpr int NPS = 32 / KS, TILE = BK * D * (int)sizeof(T);
   __shared__ __align__(16) char lds[4 * TILE];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
   const int64_t want = a.tiles - 1 - blockIdx.x / a.Hkv;
   const SeqTile t = find_tile(a.cu, a.N, a.total, a.G, kRowTile, want, lane);
@@ -82,10 +82,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   st.load(vb, a.v_t, 0, end);
   st.store(lds + TILE);
   __syncthreads();
-  for (int kt = 0; kt < tile_hi; ++kt) {
-    const char* tk = lds + (kt & 1) * 2 * TILE;
+  const LaneAt<T, D> at_lane(lane);
+  auto step = [&](int kt, int buf) __attribute__((always_inline)) {
+    const char* tk = lds + buf * 2 * TILE;
     const char* tv = tk + TILE;
-    char* nk = lds + ((kt + 1) & 1) * 2 * TILE;
+    char* nk = lds + (buf ^ 1) * 2 * TILE;
     const bool more = kt + 1 < tile_hi;
     const int k0 = kt * BK;
     const bool sees = k0 < wave_end, edge = k0 + BK - 1 > wave_min;
@@ -101,8 +102,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
       if (sees) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-          s = mma<T>(frag<T, D>(tk, b * 32 + (lane & 31), i, half), qf[i], s);
-          g = mma<T>(frag<T, D>(tv, b * 32 + (lane & 31), i, half), gf[i], g);
+          s = mma<T>(at_lane.frag(tk, b * 32, i), qf[i], s);
+          g = mma<T>(at_lane.frag(tv, b * 32, i), gf[i], g);
         }
       }
       if (NKB == 1 && more) {  // (a single half: the values follow behind the first two products)
@@ -114,6 +115,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[i] = exp2_fast(fmaf(s[i], a.c, -lse)) * (g[i] - delta);
       if (edge) {
+        rare();
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (k0 + b * 32 + result_row(i, half) > pos) p[i] = 0.f;
@@ -122,12 +124,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
       for (int i = 0; i < NPS; ++i) {
         const u32x4 pf = pack<T>(p + i * (KS / 2));
 #pragma unroll
-        for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(frag_t<T, D>(tk, b * 32, i, d, lane), pf, acc[d]);
+        for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(at_lane.frag_t(tk, b * 32, i, d), pf, acc[d]);
       }
     }
     if (more) st.store(nk + TILE);
     __syncthreads();
-  }
+  };
+  for (int kt = 0; kt < tile_hi; ++kt) step(kt, kt & 1);
   if (!live) return;
   T* po = static_cast<T*>(a.gq) + at * D;
 #pragma unroll
@@ -158,7 +161,7 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
   __shared__ __align__(16) char lds[4 * TILE];
   __shared__ __align__(16) float s_lse[2][BR], s_delta[2][BR];
   __shared__ __align__(16) int s_pos[2][BR];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
   const int64_t want = blockIdx.x / a.Hkv;  // the first keys are seen by the most rows: they go first
   const SeqTile t = find_tile(a.cu, a.N, a.total, 1, grad_keys<T, D>(), want, lane);
@@ -248,21 +251,21 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
   load();
   store(0);
   __syncthreads();
-  for (int rt = lo; rt < hi; ++rt) {
-    const int buf = (rt - lo) & 1;
+  const int b = wv / KG, own = b * 32 * D * (int)sizeof(T);  // this wavefront's block of 32 rows of a tile
+  const LaneAt<T, D> at_lane(lane);
+  auto step = [&](int rt, int buf) __attribute__((always_inline)) {
     const char* tq = lds + buf * 2 * TILE;
     const char* tg = tq + TILE;
     const bool more = rt + 1 < hi;
     if (more) load();
-    const int b = wv / KG;  // this wavefront's block of 32 rows
     const int r0 = rt * BR + b * 32;
     // (every wavefront multiplies every block, masked ones too: a branch around the products makes the
     // compiler move the 128 accumulators between the register files in every iteration)
     f32x16 s = f32x16{0}, g = f32x16{0};
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-      s = mma<T>(frag<T, D>(tq, b * 32 + (lane & 31), i, half), kf[i], s);
-      g = mma<T>(frag<T, D>(tg, b * 32 + (lane & 31), i, half), vf[i], g);
+      s = mma<T>(at_lane.frag(tq + own, 0, i), kf[i], s);
+      g = mma<T>(at_lane.frag(tg + own, 0, i), vf[i], g);
     }
     const bool edge = r0 + 32 > rows || key0 + 32 > t.len || (a.causal && r0 / a.G < key0 + 31);
     float p[16], ds[16];
@@ -276,26 +279,26 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
         p[i] = exp2_fast(fmaf(s[i], a.c, -lse[e]));
         ds[i] = p[i] * (g[i] - dl[e]);
       }
-      if (edge) {
-        typedef int i32x4 __attribute__((ext_vector_type(4)));
-        const i32x4 ps = *reinterpret_cast<const i32x4*>(&s_pos[buf][b * 32 + j * 8 + half * 4]);
+    }
+    if (edge) {
+      rare();
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (key > ps[e] || !live) p[j * 4 + e] = 0.f, ds[j * 4 + e] = 0.f;
-      }
+      for (int i = 0; i < 16; ++i)
+        if (key > s_pos[buf][b * 32 + result_row(i, half)] || !live) p[i] = 0.f, ds[i] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < NPS; ++i) {
       const u32x4 pf = pack<T>(p + i * (KS / 2)), df = pack<T>(ds + i * (KS / 2));
 #pragma unroll
       for (int d = 0; d < NDB; ++d) {
-        gv[d] = mma<T>(frag_t<T, D>(tg, b * 32, i, d, lane), pf, gv[d]);
-        gk[d] = mma<T>(frag_t<T, D>(tq, b * 32, i, d, lane), df, gk[d]);
+        gv[d] = mma<T>(at_lane.frag_t(tg + own, 0, i, d), pf, gv[d]);
+        gk[d] = mma<T>(at_lane.frag_t(tq + own, 0, i, d), df, gk[d]);
       }
     }
     if (more) store(buf ^ 1);
     __syncthreads();
-  }
+  };
+  for (int rt = lo; rt < hi; ++rt) step(rt, (rt - lo) & 1);
   if constexpr (RG > 1) {  // the second half of the rows joins the first (the tiles are free by now)
     float* meet = reinterpret_cast<float*>(lds) + (int64_t)(wv % KG) * (NDB * 32 * 64) + lane;
     static_assert(KG * NDB * 32 * 64 * 4 <= sizeof(lds), "the sums of half the wavefronts fit the tiles");

@@ -49,7 +49,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void atte
   constexpr int ROWS = 16 * R;
   __shared__ __align__(16) float s_o[4][ROWS][D + 4];
   __shared__ float s_m[4][ROWS], s_l[4][ROWS];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
   const int h = blockIdx.x % a.Hkv;
   const int64_t want = blockIdx.x / a.Hkv;
   const SeqTile t = find_tile(a.cu, a.N, a.total, a.G, ROWS, want, lane);

@@ -114,7 +114,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   constexpr int NPS = 32 / KS, TILE = BK * D * (int)sizeof(T);
   __shared__ __align__(16) char lds[4 * TILE];
   __shared__ uint8_t s_hidden[2][64];  // paged: keys without a page
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, half = lane >> 5;
+  const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
   // the last tiles of a sequence see the most keys: they go first
   const int64_t want = a.tiles - 1 - blockIdx.x / a.Hkv;
@@ -180,8 +180,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
     st.store(lds + TILE);
   }
   __syncthreads();
-  for (int kt = tile_lo; kt < tile_hi; ++kt) {
-    const int buf = (kt - tile_lo) & 1;
+  const LaneAt<T, D> at_lane(lane);
+  // one tile out of buffer `which`
+  auto step = [&](int kt, int buf) __attribute__((always_inline)) {
     const char* tk = lds + buf * 2 * TILE;
     const char* tv = tk + TILE;
     char* nk = lds + (buf ^ 1) * 2 * TILE;
@@ -197,8 +198,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int b = 0; b < NKB; ++b) s[b] = mma<T>(frag<T, D>(tk, b * 32 + (lane & 31), i, half), qf[i], s[b]);
+        for (int b = 0; b < NKB; ++b) s[b] = mma<T>(at_lane.frag(tk, b * 32, i), qf[i], s[b]);
       if (k0 + BK - 1 > wave_min) {
+        rare();
 #pragma unroll
         for (int b = 0; b < NKB; ++b)
 #pragma unroll
@@ -208,6 +210,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
       if constexpr (PAGED) {
         const uint64_t hidden = __ballot(lane < BK && s_hidden[buf][lane]);
         if (hidden) {
+          rare();
 #pragma unroll
           for (int b = 0; b < NKB; ++b)
 #pragma unroll
@@ -222,6 +225,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
       top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
       if (__any(top > m + 8.f)) {
+        rare();
         const float to = fmaxf(m, top);
         const float f = to == -INFINITY ? 1.f : exp2_fast(m - to);
         m = to;
@@ -256,11 +260,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
 #pragma unroll
         for (int i = 0; i < NPS; ++i)
 #pragma unroll
-          for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(frag_t<T, D>(tv, b * 32, i, d, lane), pf[b * NPS + i], acc[d]);
+          for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(at_lane.frag_t(tv, b * 32, i, d), pf[b * NPS + i], acc[d]);
     }
     if (more) st.store(nk + TILE);
     __syncthreads();
-  }
+  };
+  for (int kt = tile_lo; kt < tile_hi; ++kt) step(kt, (kt - tile_lo) & 1);
   l += __shfl_xor(l, 32, 64);
   if (!live) return;
   const int64_t at = (t.start + tok) * Hq + head;

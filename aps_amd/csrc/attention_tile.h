@@ -15,6 +15,8 @@
 
 #include "common.h"
 
+#include <type_traits>
+
 namespace aps {
 namespace att {
 
@@ -134,39 +136,58 @@ __device__ __forceinline__ int tile_at(int r, int c) {
   return r * (D * (int)sizeof(T)) + ((c ^ swizzle<T, D>(r)) << 4);
 }
 
-// row fragment: row `r` (per lane), step s
+// Where a lane's fragments lie, from a tile's first byte.  The swizzle depends on a row's last four bits, so
+// 32 rows (16 for the 16-bit transposing read) further on is a constant to the instruction's offset, and so
+// is the other buffer: the loops below run over both buffers in turn, unrolled, and add nothing per read.
+//   row fragment, step s:         row lane % 32, chunk 2 s + lane / 32
+//   transposed fragment (16-bit): ds_read_b64_tr_b16: within 16 lanes, lane j points at 4 elements of row
+//                                 j / 4 and receives column j of the 4 x 16 block
 template <typename T, int D>
-__device__ __forceinline__ u32x4 frag(const char* tile, int r, int s, int half) {
-  return *reinterpret_cast<const u32x4*>(tile + tile_at<T, D>(r, 2 * s + half));
-}
+struct LaneAt {
+  static constexpr int NS = D / (2 * chunk_elems<T>()), NDB = D / 32, PITCH = D * (int)sizeof(T);
+  int f[NS], t[sizeof(T) == 2 ? NDB : 1][2], lane;
 
-// transposed fragment: column db * 32 + lane % 32 of the KS rows that registers s * KS / 2 .. of a
-// 32x32 result stand for, rows counted from `row0`
-template <typename T, int D>
-__device__ __forceinline__ u32x4 frag_t(const char* tile, int row0, int s, int db, int lane) {
-  const int half = lane >> 5;
-  if constexpr (sizeof(T) == 2) {
-    // ds_read_b64_tr_b16: within 16 lanes, lane j points at 4 elements of row j / 4 and receives
-    // column j of the 4 x 16 block
-    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-    const int c = db * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
-    const int r = row0 + s * 16 + half * 4 + ((lane & 15) >> 2);
-    const int sub = (lane & 1) * 8;
-    s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + tile_at<T, D>(r, c) + sub));
-    s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(tile + tile_at<T, D>(r + 8, c) + sub));
-    const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
-    return u32x4{a.x, a.y, b.x, b.y};
-  } else {
-    const int d = db * 32 + (lane & 31);
-    u32x4 v;
+  __device__ __forceinline__ explicit LaneAt(int l) : lane(l) {
+    const int half = l >> 5;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = row0 + s * 8 + half * 4 + e;
-      v[e] = *reinterpret_cast<const uint32_t*>(tile + tile_at<T, D>(r, d >> 2) + (d & 3) * 4);
+    for (int s = 0; s < NS; ++s) f[s] = tile_at<T, D>(l & 31, 2 * s + half);
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int db = 0; db < NDB; ++db)
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi)
+          t[db][hi] = tile_at<T, D>(half * 4 + ((l & 15) >> 2) + hi * 8, db * 4 + ((l >> 4) & 1) * 2 + ((l & 3) >> 1)) +
+                      (l & 1) * 8;
     }
-    return v;
   }
-}
+  // rows row0 .. row0 + 31 (a multiple of 32)
+  __device__ __forceinline__ u32x4 frag(const char* tile, int row0, int s) const {
+    return *reinterpret_cast<const u32x4*>(tile + row0 * PITCH + f[s]);
+  }
+  // column db * 32 + lane % 32 of the KS rows that registers s * KS / 2 .. of a 32x32 result stand for
+  __device__ __forceinline__ u32x4 frag_t(const char* tile, int row0, int s, int db) const {
+    if constexpr (sizeof(T) == 2) {
+      typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+      const char* p = tile + (row0 + s * 16) * PITCH;
+      const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + t[db][0])));
+      const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + t[db][1])));
+      return u32x4{a.x, a.y, b.x, b.y};
+    } else {
+      const int d = db * 32 + (lane & 31);
+      u32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = row0 + s * 8 + (lane >> 5) * 4 + e;
+        v[e] = *reinterpret_cast<const uint32_t*>(tile + tile_at<T, D>(r, d >> 2) + (d & 3) * 4);
+      }
+      return v;
+    }
+  }
+};
+
+// In a branch that few tiles take: keeps the compiler from turning it into selects that all of them pay for
+// (a third of the forward kernel's vector instructions)
+__device__ __forceinline__ void rare() { asm volatile(""); }
 
 // row of a 32x32 result that register i of a lane holds
 __device__ __forceinline__ int result_row(int i, int half) { return (i >> 2) * 8 + half * 4 + (i & 3); }
