@@ -83,13 +83,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   st.store(lds + TILE);
   __syncthreads();
   const LaneAt<T, D> at_lane(lane);
-  auto step = [&](int kt, int buf) __attribute__((always_inline)) {
+  auto step = [&](int kt, int buf, auto masked) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(masked)::value;
     const char* tk = lds + buf * 2 * TILE;
     const char* tv = tk + TILE;
     char* nk = lds + (buf ^ 1) * 2 * TILE;
     const bool more = kt + 1 < tile_hi;
     const int k0 = kt * BK;
-    const bool sees = k0 < wave_end, edge = k0 + BK - 1 > wave_min;
+    const bool sees = !EDGE || k0 < wave_end;
     // 32 keys at a time; the next tile's keys are in flight during the first half, its values during the second
     if (more) st.load(kb, a.k_t, k0 + BK, end);
 #pragma unroll
@@ -114,8 +115,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
       float p[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) p[i] = exp2_fast(fmaf(s[i], a.c, -lse)) * (g[i] - delta);
-      if (edge) {
-        rare();
+      if (EDGE && k0 + BK - 1 > wave_min) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (k0 + b * 32 + result_row(i, half) > pos) p[i] = 0.f;
@@ -130,7 +130,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
     if (more) st.store(nk + TILE);
     __syncthreads();
   };
-  for (int kt = 0; kt < tile_hi; ++kt) step(kt, kt & 1);
+  // tiles that every row of the workgroup sees whole, without a mask or a branch; then the others
+  const int clear = min(tile_hi, ((a.causal ? t.tile * kRowTile / a.G : kv - 1) + 1) / BK);
+  int kt = 0;
+  for (; kt < clear; ++kt) step(kt, kt & 1, std::false_type());
+  for (; kt < tile_hi; ++kt) step(kt, kt & 1, std::true_type());
   if (!live) return;
   T* po = static_cast<T*>(a.gq) + at * D;
 #pragma unroll
@@ -253,7 +257,8 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
   __syncthreads();
   const int b = wv / KG, own = b * 32 * D * (int)sizeof(T);  // this wavefront's block of 32 rows of a tile
   const LaneAt<T, D> at_lane(lane);
-  auto step = [&](int rt, int buf) __attribute__((always_inline)) {
+  auto step = [&](int rt, int buf, auto masked) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(masked)::value;
     const char* tq = lds + buf * 2 * TILE;
     const char* tg = tq + TILE;
     const bool more = rt + 1 < hi;
@@ -267,7 +272,6 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
       s = mma<T>(at_lane.frag(tq + own, 0, i), kf[i], s);
       g = mma<T>(at_lane.frag(tg + own, 0, i), vf[i], g);
     }
-    const bool edge = r0 + 32 > rows || key0 + 32 > t.len || (a.causal && r0 / a.G < key0 + 31);
     float p[16], ds[16];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -280,11 +284,10 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
         ds[i] = p[i] * (g[i] - dl[e]);
       }
     }
-    if (edge) {
-      rare();
+    if (EDGE) {
 #pragma unroll
       for (int i = 0; i < 16; ++i)
-        if (key > s_pos[buf][b * 32 + result_row(i, half)] || !live) p[i] = 0.f, ds[i] = 0.f;
+        if (key > s_pos[buf][b * 32 + result_row(i, half)]) p[i] = 0.f, ds[i] = 0.f;
     }
 #pragma unroll
     for (int i = 0; i < NPS; ++i) {
@@ -298,7 +301,12 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
     if (more) store(buf ^ 1);
     __syncthreads();
   };
-  for (int rt = lo; rt < hi; ++rt) step(rt, (rt - lo) & 1);
+  // Only the first row tiles of a causal sequence need a mask: a row behind the last one has lse = inf, so
+  // its weights are zeros, and a column behind the last key is not stored.
+  const int masked = a.causal ? min(hi, ((tile0 + grad_keys<T, D>() - 1) * a.G + BR - 1) / BR) : lo;
+  int rt = lo;
+  for (; rt < masked; ++rt) step(rt, (rt - lo) & 1, std::true_type());
+  for (; rt < hi; ++rt) step(rt, (rt - lo) & 1, std::false_type());
   if constexpr (RG > 1) {  // the second half of the rows joins the first (the tiles are free by now)
     float* meet = reinterpret_cast<float*>(lds) + (int64_t)(wv % KG) * (NDB * 32 * 64) + lane;
     static_assert(KG * NDB * 32 * 64 * 4 <= sizeof(lds), "the sums of half the wavefronts fit the tiles");

@@ -182,13 +182,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   __syncthreads();
   const LaneAt<T, D> at_lane(lane);
   // one tile out of buffer `which`
-  auto step = [&](int kt, int buf) __attribute__((always_inline)) {
+  auto step = [&](int kt, int buf, auto edge) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge)::value;
     const char* tk = lds + buf * 2 * TILE;
     const char* tv = tk + TILE;
     char* nk = lds + (buf ^ 1) * 2 * TILE;
     const bool more = kt + 1 < tile_hi;
     const int k0 = kt * BK;
-    const bool sees = k0 < wave_end;
+    const bool sees = !EDGE || k0 < wave_end;
     u32x4 pf[NKB * NPS];
     if (more) st.load(kb, a.k_t, k0 + BK, end);
     if (sees) {
@@ -199,8 +200,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
       for (int i = 0; i < NS; ++i)
 #pragma unroll
         for (int b = 0; b < NKB; ++b) s[b] = mma<T>(at_lane.frag(tk, b * 32, i), qf[i], s[b]);
-      if (k0 + BK - 1 > wave_min) {
-        rare();
+      if (EDGE && k0 + BK - 1 > wave_min) {
 #pragma unroll
         for (int b = 0; b < NKB; ++b)
 #pragma unroll
@@ -210,8 +210,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
       if constexpr (PAGED) {
         const uint64_t hidden = __ballot(lane < BK && s_hidden[buf][lane]);
         if (hidden) {
-          rare();
-#pragma unroll
+  #pragma unroll
           for (int b = 0; b < NKB; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
@@ -225,7 +224,6 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
       top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
       if (__any(top > m + 8.f)) {
-        rare();
         const float to = fmaxf(m, top);
         const float f = to == -INFINITY ? 1.f : exp2_fast(m - to);
         m = to;
@@ -265,7 +263,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
     if (more) st.store(nk + TILE);
     __syncthreads();
   };
-  for (int kt = tile_lo; kt < tile_hi; ++kt) step(kt, (kt - tile_lo) & 1);
+  // tiles that every row of the workgroup sees whole, without a mask or a branch; then the others
+  const int block_min = a.causal ? off + t.tile * kRowTile / a.G : kv - 1;
+  const int clear = min(tile_hi, (block_min + 1) / BK);
+  int kt = tile_lo;
+  for (; kt < clear; ++kt) step(kt, (kt - tile_lo) & 1, std::false_type());
+  for (; kt < tile_hi; ++kt) step(kt, (kt - tile_lo) & 1, std::true_type());
   l += __shfl_xor(l, 32, 64);
   if (!live) return;
   const int64_t at = (t.start + tok) * Hq + head;

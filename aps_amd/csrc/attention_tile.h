@@ -185,10 +185,6 @@ struct LaneAt {
   }
 };
 
-// In a branch that few tiles take: keeps the compiler from turning it into selects that all of them pay for
-// (a third of the forward kernel's vector instructions)
-__device__ __forceinline__ void rare() { asm volatile(""); }
-
 // row of a 32x32 result that register i of a lane holds
 __device__ __forceinline__ int result_row(int i, int half) { return (i >> 2) * 8 + half * 4 + (i & 3); }
 
