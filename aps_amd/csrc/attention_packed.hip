@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
     }
     return;
   }
-  const int rows = t.len * a.G, tile0 = t.tile * grad_keys<T, D>(), key0 = tile0 + wv % KG * 32, key = key0 + (lane & 31);
+  const int tile0 = t.tile * grad_keys<T, D>(), key0 = tile0 + wv % KG * 32, key = key0 + (lane & 31);
   const bool live = key < t.len;
   u32x4 kf[NS], vf[NS];
   {
@@ -193,53 +193,53 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
 #pragma unroll
   for (int d = 0; d < NDB; ++d) gk[d] = gv[d] = f32x16{0};
 
+  // Row tiles: `toks` whole tokens of G <= BR heads each, or BR heads of one token.  A thread's place in a
+  // tile is then the same in every tile, and a tile's place is a scalar: no division in the loop.  (BR % G
+  // rows of a tile stay empty: none for the usual groups of 1, 2, 4, 8; 1 of 64 for 3, 4 of 64 for 5.)
+  const int toks = a.G <= BR ? BR / a.G : 1, segs = a.G <= BR ? 1 : (a.G + BR - 1) / BR;
+  const int lo = a.causal ? tile0 / toks * segs : 0, hi = (t.len + toks - 1) / toks * segs;
+  const int span = a.G <= BR ? a.G : BR;  // heads of a token in a tile
+  auto place = [&](int j, int& tok, int& head) {
+    tok = j / span, head = j - tok * span;
+    if (tok >= toks) tok = 1 << 30;  // an empty row
+  };
+  uint32_t q_at[PER], g_at[PER];
+  int tok_i[PER], head_i[PER], tok_s, head_s;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    place(threadIdx.x / CH + i * STEP, tok_i[i], head_i[i]);
+    const int tk = min(tok_i[i], BR);
+    q_at[i] = (uint32_t)((tk * (int)a.q_t + head_i[i] * (int)a.q_h) * (int)sizeof(T) + threadIdx.x % CH * 16);
+    g_at[i] = (uint32_t)((tk * (int)a.go_t + head_i[i] * (int)a.go_h) * (int)sizeof(T) + threadIdx.x % CH * 16);
+  }
+  place(threadIdx.x & (BR - 1), tok_s, head_s);
+  const char* qb = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + t.start * a.q_t + (int64_t)h * a.G * a.q_h);
+  const char* gb = reinterpret_cast<const char*>(static_cast<const T*>(a.go) + t.start * a.go_t + (int64_t)h * a.G * a.go_h);
   u32x4 qr[PER], gr[PER];
   float r_lse = INFINITY, r_delta = 0.f;
   int r_pos = -1;
-  // causal: the rows before token `tile0` see none of the tile's keys
-  const int lo = a.causal ? (tile0 * a.G) / BR : 0, hi = (rows + BR - 1) / BR;
-  // row i of the thread, and the row whose statistics it carries, as (token, head of the group) with the
-  // offsets they stand for; BR rows on: two additions instead of a division and four products
-  const int step_tok = BR / a.G, step_head = BR - step_tok * a.G;
-  const int64_t q_step = step_tok * a.q_t + step_head * a.q_h, q_wrap = a.q_t - a.G * a.q_h;
-  const int64_t g_step = step_tok * a.go_t + step_head * a.go_h, g_wrap = a.go_t - a.G * a.go_h;
-  const T* qp[PER];
-  const T* gp[PER];
-  int row_head[PER], row_at = lo * BR, s_head, s_tok;
-  {
-    const int c = threadIdx.x % CH;
+  auto load = [&](int rt) {
+    const int tok0 = segs == 1 ? rt * toks : rt / segs, head0 = segs == 1 ? 0 : (rt - tok0 * segs) * BR;
+    const char* q0 = qb + (tok0 * a.q_t + head0 * a.q_h) * (int)sizeof(T);
+    const char* g0 = gb + (tok0 * a.go_t + head0 * a.go_h) * (int)sizeof(T);
+    if (toks * span == BR && tok0 + toks <= t.len && head0 + span <= a.G) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int row = row_at + threadIdx.x / CH + i * STEP, tok = row / a.G;
-      row_head[i] = row - tok * a.G;
-      qp[i] = static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + (h * a.G + row_head[i]) * a.q_h + c * E;
-      gp[i] = static_cast<const T*>(a.go) + (t.start + tok) * a.go_t + (h * a.G + row_head[i]) * a.go_h + c * E;
-    }
-    const int row = row_at + (threadIdx.x & (BR - 1));
-    s_tok = row / a.G, s_head = row - s_tok * a.G;
-  }
-  auto load = [&]() {  // the next BR rows
+      for (int i = 0; i < PER; ++i) qr[i] = load_chunk(q0, q_at[i]), gr[i] = load_chunk(g0, g_at[i]);
+    } else {
+      rare();
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      qr[i] = gr[i] = u32x4{0, 0, 0, 0};
-      if (row_at + (int)threadIdx.x / CH + i * STEP < rows) {
-        qr[i] = *reinterpret_cast<const u32x4*>(qp[i]);
-        gr[i] = *reinterpret_cast<const u32x4*>(gp[i]);
+      for (int i = 0; i < PER; ++i) {
+        qr[i] = gr[i] = u32x4{0, 0, 0, 0};
+        if (tok_i[i] < t.len - tok0 && head0 + head_i[i] < a.G) qr[i] = load_chunk(q0, q_at[i]), gr[i] = load_chunk(g0, g_at[i]);
       }
-      row_head[i] += step_head;
-      qp[i] += q_step, gp[i] += g_step;
-      if (row_head[i] >= a.G) row_head[i] -= a.G, qp[i] += q_wrap, gp[i] += g_wrap;
     }
     if (threadIdx.x < BR) {
       r_lse = INFINITY, r_delta = 0.f, r_pos = -1;
-      if (row_at + (int)threadIdx.x < rows) {
-        const int64_t at = (t.start + s_tok) * Hq + h * a.G + s_head;
-        r_lse = a.lse[at], r_delta = a.delta[at], r_pos = a.causal ? s_tok : t.len - 1;
+      if (tok_s < t.len - tok0 && head0 + head_s < a.G) {
+        const int64_t at = (t.start + tok0 + tok_s) * Hq + h * a.G + head0 + head_s;
+        r_lse = a.lse[at], r_delta = a.delta[at], r_pos = a.causal ? tok0 + tok_s : t.len - 1;
       }
-      s_head += step_head, s_tok += step_tok;
-      if (s_head >= a.G) s_head -= a.G, ++s_tok;
     }
-    row_at += BR;
   };
   auto store = [&](int buf) {
     char* tq = lds + buf * 2 * TILE;
@@ -252,7 +252,7 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
     if (threadIdx.x < BR)
       s_lse[buf][threadIdx.x] = r_lse, s_delta[buf][threadIdx.x] = r_delta, s_pos[buf][threadIdx.x] = r_pos;
   };
-  load();
+  load(lo);
   store(0);
   __syncthreads();
   const int b = wv / KG, own = b * 32 * D * (int)sizeof(T);  // this wavefront's block of 32 rows of a tile
@@ -262,8 +262,7 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
     const char* tq = lds + buf * 2 * TILE;
     const char* tg = tq + TILE;
     const bool more = rt + 1 < hi;
-    if (more) load();
-    const int r0 = rt * BR + b * 32;
+    if (more) load(rt + 1);
     // (every wavefront multiplies every block, masked ones too: a branch around the products makes the
     // compiler move the 128 accumulators between the register files in every iteration)
     f32x16 s = f32x16{0}, g = f32x16{0};
@@ -303,7 +302,7 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
   };
   // Only the first row tiles of a causal sequence need a mask: a row behind the last one has lse = inf, so
   // its weights are zeros, and a column behind the last key is not stored.
-  const int masked = a.causal ? min(hi, ((tile0 + grad_keys<T, D>() - 1) * a.G + BR - 1) / BR) : lo;
+  const int masked = a.causal ? min(hi, (tile0 + grad_keys<T, D>() - 2 + toks) / toks * segs) : lo;
   int rt = lo;
   for (; rt < masked; ++rt) step(rt, (rt - lo) & 1, std::true_type());
   for (; rt < hi; ++rt) step(rt, (rt - lo) & 1, std::false_type());
@@ -371,7 +370,7 @@ extern "C" int aps_attention_packed(const void* q, const void* k, const void* v,
   APS_CHECK_ARG(q && k && v && cu_seqlens && out && sizes_fit(total, N, Hq, Hkv) && scale > 0.f);
   const int64_t e = dtype == kTypeF32 ? 4 : 8;
   APS_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out));
-  APS_CHECK_ARG(q_t % e == 0 && q_h % e == 0 && k_t % e == 0 && k_h % e == 0 && v_t % e == 0 && v_h % e == 0);
+  APS_CHECK_ARG(strides_fit(q_t, q_h, e) && strides_fit(k_t, k_h, e) && strides_fit(v_t, v_h, e));
   RowsArgs a{};
   a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
   a.cu = Index{cu_seqlens, cu_wide};
@@ -404,8 +403,8 @@ extern "C" int aps_attention_packed_backward(const void* q, const void* k, const
   const int64_t e = dtype == kTypeF32 ? 4 : 8;
   APS_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(g_out));
   APS_CHECK_ARG(aligned16(g_q) && aligned16(g_k) && aligned16(g_v));
-  APS_CHECK_ARG(q_t % e == 0 && q_h % e == 0 && k_t % e == 0 && k_h % e == 0 && v_t % e == 0 && v_h % e == 0);
-  APS_CHECK_ARG(go_t % e == 0 && go_h % e == 0);
+  APS_CHECK_ARG(strides_fit(q_t, q_h, e) && strides_fit(k_t, k_h, e) && strides_fit(v_t, v_h, e));
+  APS_CHECK_ARG(strides_fit(go_t, go_h, e));
   GradArgs a{};
   a.q = q, a.k = k, a.v = v, a.o = out, a.go = g_out, a.lse = lse, a.delta = static_cast<float*>(workspace);
   a.gq = g_q, a.gk = g_k, a.gv = g_v;

@@ -398,7 +398,7 @@ extern "C" int aps_attention_paged(const void* q, const void* k_pages, const voi
   APS_CHECK_ARG(paged_sizes_fit(total, N, Hq, Hkv, num_pages, page, width) && table_stride >= width);
   const int64_t e = dtype == kTypeF32 ? 4 : 8;
   APS_CHECK_ARG(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out));
-  APS_CHECK_ARG(q_t % e == 0 && q_h % e == 0);
+  APS_CHECK_ARG(strides_fit(q_t, q_h, e));
   RowsArgs a{};
   a.q = q, a.k = k_pages, a.v = v_pages, a.out = out;
   a.cu = Index{cu_seqlens, cu_wide}, a.kv_lens = Index{kv_lens, kv_wide};
@@ -434,7 +434,7 @@ extern "C" int aps_paged_append(const void* k, const void* v, void* k_pages, voi
     return APS_ERR_UNSUPPORTED;
   const int64_t e = dtype == kTypeF32 ? 4 : 8;
   APS_CHECK_ARG(aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages));
-  APS_CHECK_ARG(k_t % e == 0 && k_h % e == 0 && v_t % e == 0 && v_h % e == 0);
+  APS_CHECK_ARG(strides_fit(k_t, k_h, e) && strides_fit(v_t, v_h, e));
   AppendArgs a{};
   a.k = k, a.v = v, a.k_pages = k_pages, a.v_pages = v_pages;
   a.cu = Index{cu_seqlens, cu_wide}, a.kv_lens = Index{kv_lens, kv_wide};

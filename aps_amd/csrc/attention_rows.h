@@ -85,12 +85,28 @@ struct KvStage {
   // base: the key head's row 0 (packed: of the sequence); row_stride in elements
   __device__ __forceinline__ void load(const T* base, int64_t row_stride, int key0, int end) {
     const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
+    if constexpr (PAGED) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int row = PAGED ? slot[i] : key0 + r0 + i * STEP;
-      r[i] = u32x4{0, 0, 0, 0};
-      if (PAGED ? row >= 0 : row < end)
-        r[i] = *reinterpret_cast<const u32x4*>(base + row * row_stride + c * chunk_elems<T>());
+      for (int i = 0; i < PER; ++i) {
+        r[i] = u32x4{0, 0, 0, 0};
+        if (slot[i] >= 0)
+          r[i] = *reinterpret_cast<const u32x4*>(base + slot[i] * row_stride + c * chunk_elems<T>());
+      }
+    } else {
+      const char* at = reinterpret_cast<const char*>(base + key0 * row_stride);
+      const uint32_t lane_at = (uint32_t)(r0 * (int)row_stride * (int)sizeof(T) + c * 16);
+      const int64_t step = row_stride * (STEP * (int)sizeof(T));
+      if (key0 + BK <= end) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) r[i] = load_chunk(at + i * step, lane_at);
+      } else {
+        rare();
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          r[i] = u32x4{0, 0, 0, 0};
+          if (key0 + r0 + i * STEP < end) r[i] = load_chunk(at + i * step, lane_at);
+        }
+      }
     }
   }
   __device__ __forceinline__ void store(char* tile) const {
@@ -224,6 +240,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
       top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
       if (__any(top > m + 8.f)) {
+        rare();
         const float to = fmaxf(m, top);
         const float f = to == -INFINITY ? 1.f : exp2_fast(m - to);
         m = to;
@@ -302,6 +319,12 @@ static inline bool sizes_fit(int64_t total, int64_t N, int64_t Hq, int64_t Hkv) 
   if (total < 0 || N < 1 || Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq > 65536) return false;
   if (total > (int64_t)0x7fff0000 / (Hq / Hkv)) return false;
   return ((total * (Hq / Hkv) + 31) / 32 + N + 1) * Hkv < 0x7fffffff;  // (32: the smallest tile of any launch; 16 x more rows in the decode form are checked there)
+}
+
+// strides of a 16-byte-chunked tensor: whole chunks, and small enough for 32-bit offsets within a tile
+static inline bool strides_fit(int64_t t, int64_t h, int64_t e) {
+  const int64_t most = kMaxStride / (16 / e);
+  return t % e == 0 && h % e == 0 && t >= 0 && t <= most && h >= 0 && h <= most;
 }
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

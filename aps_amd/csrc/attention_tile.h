@@ -185,6 +185,17 @@ struct LaneAt {
   }
 };
 
+// In a branch that is seldom taken: keeps the compiler from turning it into selects that every tile pays for
+__device__ __forceinline__ void rare() { asm volatile(""); }
+
+// A chunk at a byte offset from a base that is the same for the whole wavefront: the load takes the base
+// from scalar registers, and a loop that steps the base adds nothing per lane.  (Strides are at most
+// kMaxStride bytes, so 128 rows stay within the 32-bit offset.)
+constexpr int64_t kMaxStride = 1 << 23;
+__device__ __forceinline__ u32x4 load_chunk(const char* base, uint32_t offset) {
+  return *reinterpret_cast<const u32x4*>(base + offset);
+}
+
 // row of a 32x32 result that register i of a lane holds
 __device__ __forceinline__ int result_row(int i, int half) { return (i >> 2) * 8 + half * 4 + (i & 3); }
 

@@ -545,9 +545,11 @@ PACKED_HEAD_DIMS = (32, 64, 128)
 
 def _strided16(t: th.Tensor) -> th.Tensor:
     """rows x heads x D as the kernels read it: the last axis contiguous, rows and heads anywhere on
-    16-byte boundaries (a slice of a fused projection is read in place); a copy of anything else"""
-    unit = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % unit == 0 and t.stride(1) % unit == 0 and t.data_ptr() % 16 == 0:
+    16-byte boundaries up to 8 MB apart (a slice of a fused projection is read in place); a copy of
+    anything else"""
+    size = t.element_size()
+    a, b, c = t.stride()
+    if c == 1 and not (a * size | b * size | t.data_ptr()) & 15 and a * size <= 1 << 23 and b * size <= 1 << 23:
         return t
     return t.clone(memory_format=th.contiguous_format)
 
