@@ -262,13 +262,23 @@ def ptr(t):
     return None if t is None else C.c_void_p(t.data_ptr())
 
 
+try:  # the handle itself, without a torch.cuda.Stream object around it (2 us of every launch)
+    _raw_stream = th._C._cuda_getCurrentRawStream
+except AttributeError:
+    def _raw_stream(index: int) -> int:
+        return th.cuda.current_stream(index).cuda_stream
+
+
 def stream_of(t: th.Tensor):
-    return C.c_void_p(th.cuda.current_stream(t.device).cuda_stream)
+    return C.c_void_p(_raw_stream(t.device.index))
+
+
+_HERE = contextlib.nullcontext()
 
 
 def on_device_of(t: th.Tensor):
     """context in which the device of `t` is the current one (launches go to the current device)"""
-    return contextlib.nullcontext() if t.device.index == th.cuda.current_device() else th.cuda.device(t.device)
+    return _HERE if t.get_device() == th.cuda.current_device() else th.cuda.device(t.device)
 
 
 def needs_grad(*tensors) -> bool:

@@ -4,6 +4,7 @@ Activations are batch-major [N, T, D] / [rows, D], fp32, contiguous.
 """
 import math
 import os
+from ctypes import addressof as C_addressof
 from ctypes import c_int64 as C_int64
 from ctypes import c_void_p as C_void_p
 from typing import List, Optional, Sequence
@@ -561,21 +562,20 @@ def _index_array(t: th.Tensor, what: str, length: Optional[int] = None) -> th.Te
     return t.contiguous()
 
 
-def _check_heads(what: str, q: th.Tensor, *kv: th.Tensor) -> None:
+def _check_heads(what: str, q: th.Tensor, k: th.Tensor, v: th.Tensor) -> None:
     """q rows x Hq x D against the (rows | pages x page) x Hkv x D tensors it attends to"""
-    if q.dim() != 3 or q.dtype not in ELEMENT_TYPES:
+    shape, dtype = k.shape, q.dtype
+    if q.dim() != 3 or dtype not in ELEMENT_TYPES:
         raise RuntimeError(f"{what}: q must be rows x heads x head_dim in f32 / bf16 / f16, got "
-                           f"{tuple(q.shape)} {q.dtype}")
-    D = q.shape[2]
+                           f"{tuple(q.shape)} {dtype}")
+    _, H, D = q.shape
     if D not in PACKED_HEAD_DIMS:
         raise RuntimeError(f"{what}: head_dim {D} not in {PACKED_HEAD_DIMS}")
-    for t in kv:
-        if t.dtype != q.dtype:
-            raise RuntimeError(f"{what}: keys / values in {t.dtype}, q in {q.dtype}")
-        if t.shape != kv[0].shape or t.shape[-1] != D or t.shape[-2] < 1 or q.shape[1] < 1 or \
-                q.shape[1] % t.shape[-2]:
-            raise RuntimeError(f"{what}: keys / values {[tuple(x.shape) for x in kv]} do not fit q "
-                               f"{tuple(q.shape)} (the same head_dim, q's heads a multiple of theirs)")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise RuntimeError(f"{what}: keys / values in {k.dtype} / {v.dtype}, q in {dtype}")
+    if v.shape != shape or shape[-1] != D or shape[-2] < 1 or H < 1 or H % shape[-2]:
+        raise RuntimeError(f"{what}: keys {tuple(shape)} / values {tuple(v.shape)} do not fit q {tuple(q.shape)} "
+                           f"(the same head_dim, q's heads a multiple of theirs)")
 
 
 def _softmax_scale(what: str, scale: Optional[float], D: int) -> float:
@@ -752,9 +752,10 @@ def beam_select(logits: th.Tensor, scores: th.Tensor, eos: int, finished: Option
         raise RuntimeError(f"{what}: scores must be f32 utterances x hypotheses, got {tuple(scores.shape)} {scores.dtype}")
     N, B = scores.shape
     K = B if beam is None else int(beam)
-    V = logits.shape[-1] if logits.dim() else 0
-    if logits.dtype not in ELEMENT_TYPES or tuple(logits.shape) not in ((N * B, V), (N, B, V)):
-        raise RuntimeError(f"{what}: logits {tuple(logits.shape)} {logits.dtype} for {N} x {B} hypotheses")
+    shape = logits.shape
+    V = shape[-1] if len(shape) else 0
+    if logits.dtype not in ELEMENT_TYPES or shape[:-1] not in ((N * B,), (N, B)):
+        raise RuntimeError(f"{what}: logits {tuple(shape)} {logits.dtype} for {N} x {B} hypotheses")
     if N < 1 or not 1 <= B <= BEAM_MAX or not 1 <= K <= BEAM_MAX or not 1 <= V <= 1 << 24 or K > B * V:
         raise RuntimeError(f"{what}: {N} utterances, {B} hypotheses, beam {K}, vocabulary {V}: at least one utterance, "
                            f"1 .. {BEAM_MAX} hypotheses, 1 .. 2^24 tokens, no more selected than there are")
@@ -763,16 +764,17 @@ def beam_select(logits: th.Tensor, scores: th.Tensor, eos: int, finished: Option
         raise RuntimeError(f"{what}: eos {eos} outside the vocabulary of {V}")
     if finished is not None and (finished.shape != scores.shape or finished.dtype != th.bool):
         raise RuntimeError(f"{what}: finished must be bool {tuple(scores.shape)}, got {tuple(finished.shape)} {finished.dtype}")
-    nat.require_device(logits, scores, finished)
+    dev = nat.require_device(logits, scores, finished)
     lib = nat.load()
-    logits = logits.reshape(N * B, V)
+    if len(shape) == 3:
+        logits = logits.reshape(N * B, V)
     if logits.stride(1) != 1 or (logits.stride(0) < V and N * B > 1):
         logits = logits.contiguous()
     scores = scores.contiguous()
     finished = None if finished is None else finished.contiguous()
-    dev = logits.device
     new_scores = th.empty(N, K, device=dev, dtype=th.float32)
-    parent, token = th.empty(2, N, K, device=dev, dtype=th.int64).unbind(0)
+    parent = th.empty(N, K, device=dev, dtype=th.int64)
+    token = th.empty_like(parent)
     done = th.empty(N, K, device=dev, dtype=th.bool)
     ws = th.empty(lib.aps_beam_select_workspace(N, B, V, K), device=dev, dtype=th.uint8)
     with nat.on_device_of(logits):
@@ -811,18 +813,22 @@ def beam_reorder(states: Sequence[th.Tensor], parent: th.Tensor, dims: Optional[
             raise RuntimeError(f"{what}: axis {d} of {tuple(t.shape)} is not {N} x {B or 'hypotheses'}")
         B = rows // N
         t = t.contiguous()
-        shape = list(t.shape)
-        shape[d] = N * K
+        shape = t.shape
         src.append(t)
-        dst.append(th.empty(shape, device=t.device, dtype=t.dtype))
+        if B == K:
+            dst.append(th.empty_like(t))
+        else:
+            dst.append(th.empty(*shape[:d], N * K, *shape[d + 1:], device=t.device, dtype=t.dtype))
         outer.append(math.prod(shape[:d]))
         inner.append(math.prod(shape[d + 1:]) * t.element_size())
     parent = parent.contiguous()
     n = len(src)
+    # the call's four host arrays, one behind the other
+    table = (C_int64 * (4 * n))(*[t.data_ptr() for t in src], *[t.data_ptr() for t in dst], *outer, *inner)
+    at = C_addressof(table)
     with nat.on_device_of(parent):
-        rc = nat.load().aps_beam_reorder((C_void_p * n)(*[t.data_ptr() for t in src]),
-                                         (C_void_p * n)(*[t.data_ptr() for t in dst]), (C_int64 * n)(*outer),
-                                         (C_int64 * n)(*inner), n, parent.data_ptr(), N, K, B, nat.stream_of(parent))
+        rc = nat.load().aps_beam_reorder(at, at + 8 * n, at + 16 * n, at + 24 * n, n, parent.data_ptr(), N, K, B,
+                                         nat.stream_of(parent))
     nat.check(rc, "aps_beam_reorder")
     return dst
 
