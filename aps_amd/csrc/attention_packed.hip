@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   __shared__ __align__(16) char lds[4 * TILE];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
-  const int64_t want = a.tiles - 1 - blockIdx.x / a.Hkv;
+  const int want = (int)a.tiles - 1 - blockIdx.x / a.Hkv;
   const SeqTile t = find_tile(a.cu, a.N, a.total, a.G, kRowTile, want, lane);
   const int Hq = a.Hkv * a.G;
   if (t.seq < 0) {
@@ -77,10 +77,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   const T* kb = static_cast<const T*>(a.k) + h * a.k_h + t.start * a.k_t;
   const T* vb = static_cast<const T*>(a.v) + h * a.v_h + t.start * a.v_t;
   KvStage<T, D, false> st;
-  st.load(kb, a.k_t, 0, end);
-  st.store(lds);
-  st.load(vb, a.v_t, 0, end);
-  st.store(lds + TILE);
+  st.template load<0>(kb, a.k_t, 0, end);
+  st.template store<0>(lds);
+  st.template load<1>(vb, a.v_t, 0, end);
+  st.template store<1>(lds + TILE);
   __syncthreads();
   const LaneAt<T, D> at_lane(lane);
   auto step = [&](int kt, int buf, auto masked) __attribute__((always_inline)) {
@@ -92,12 +92,16 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
     const int k0 = kt * BK;
     const bool sees = !EDGE || k0 < wave_end;
     // 32 keys at a time; the next tile's keys are in flight during the first half, its values during the second
-    if (more) st.load(kb, a.k_t, k0 + BK, end);
+    constexpr bool TURNS = KvStage<T, D, false>::TURNS;
+    if (more) {
+      st.template load<0>(kb, a.k_t, k0 + BK, end);
+      if (!TURNS) st.template load<1>(vb, a.v_t, k0 + BK, end);
+    }
 #pragma unroll
     for (int b = 0; b < NKB; ++b) {
-      if (b == 1 && more) {
-        st.store(nk);
-        st.load(vb, a.v_t, k0 + BK, end);
+      if (TURNS && b == 1 && more) {
+        st.template store<0>(nk);
+        st.template load<1>(vb, a.v_t, k0 + BK, end);
       }
       f32x16 s = f32x16{0}, g = f32x16{0};
       if (sees) {
@@ -107,9 +111,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
           g = mma<T>(at_lane.frag(tv, b * 32, i), gf[i], g);
         }
       }
-      if (NKB == 1 && more) {  // (a single half: the values follow behind the first two products)
-        st.store(nk);
-        st.load(vb, a.v_t, k0 + BK, end);
+      if (TURNS && NKB == 1 && more) {  // (a single half: the values follow behind the first two products)
+        st.template store<0>(nk);
+        st.template load<1>(vb, a.v_t, k0 + BK, end);
       }
       if (!sees) continue;
       float p[16];
@@ -127,7 +131,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
         for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(at_lane.frag_t(tk, b * 32, i, d), pf, acc[d]);
       }
     }
-    if (more) st.store(nk + TILE);
+    if (more) {
+      if (!TURNS) st.template store<0>(nk);
+      st.template store<1>(nk + TILE);
+    }
     __syncthreads();
   };
   // tiles that every row of the workgroup sees whole, without a mask or a branch; then the others
@@ -167,7 +174,7 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
   __shared__ __align__(16) int s_pos[2][BR];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
-  const int64_t want = blockIdx.x / a.Hkv;  // the first keys are seen by the most rows: they go first
+  const int want = blockIdx.x / a.Hkv;  // the first keys are seen by the most rows: they go first
   const SeqTile t = find_tile(a.cu, a.N, a.total, 1, grad_keys<T, D>(), want, lane);
   const int Hq = a.Hkv * a.G;
   if (t.seq < 0) {

@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void atte
   __shared__ float s_m[4][ROWS], s_l[4][ROWS];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, c = lane & 15;
   const int h = blockIdx.x % a.Hkv;
-  const int64_t want = blockIdx.x / a.Hkv;
+  const int want = blockIdx.x / a.Hkv;
   const SeqTile t = find_tile(a.cu, a.N, a.total, a.G, ROWS, want, lane);
   const int Hq = a.Hkv * a.G;
   if (t.seq < 0) {
@@ -249,9 +249,9 @@ __global__ __launch_bounds__(256) void attention_combine_kernel(RowsArgs a) {
   const int Hq = a.Hkv * a.G, d = (threadIdx.x % PER) * 4;
   const int64_t row = (int64_t)blockIdx.x * (256 / PER) + threadIdx.x / PER, all = a.total * Hq;
   if (row >= tail_of(a.cu, a.N, a.total) * Hq) return;
-  int64_t s0, e0;
+  int s0, e0;
   seq_range(a.cu, 0, a.total, s0, e0);
-  if (row < s0 * Hq) return;  // rows before the first sequence belong to none either
+  if (row < (int64_t)s0 * Hq) return;  // rows before the first sequence belong to none either
   // eight splits at a time, their loads in flight together
   float top = -INFINITY, sum = 0.f;
   f32x4 o = f32x4{0};
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
     if (a.cu.at(mid) <= tok) lo = mid;
     else hi = mid;
   }
-  int64_t start, end;
+  int start, end;
   seq_range(a.cu, lo, a.total, start, end);
   if (tok < start || tok >= end) return;
   int64_t kv = a.kv_lens.at(lo);
@@ -330,10 +330,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 
 // Which kernel and how many splits, from what the host knows (the lengths themselves are on the
 // device): form 1 / 2 = decode tiles of 16 / 32 rows, 0 = 128-row tiles.
-#ifndef kTargetA
-#define kTargetA 1024
-#define kTargetB 1024
-#endif
 struct PagedPlan { int form; int64_t tiles; int splits; };
 
 static PagedPlan paged_plan(int64_t total, int64_t N, int64_t G, int64_t Hkv, int64_t max_keys, int64_t dtype) {
@@ -343,8 +339,10 @@ static PagedPlan paged_plan(int64_t total, int64_t N, int64_t G, int64_t Hkv, in
   const int64_t tile = p.form == 1 ? 16 : (p.form == 2 ? 32 : kRowTile);
   p.tiles = (total * G + tile - 1) / tile + N + 1;
   const int64_t busy = ((total * G + tile - 1) / tile > N ? (total * G + tile - 1) / tile : N) * Hkv;
-  // four workgroups per CU for the loads' sake (decode), two for the 128-row tiles
-  const int64_t target = p.form ? kTargetA : kTargetB;
+  // Workgroups to aim for.  Decode: the lengths differ, so twice what the chip holds evens them out (16 contexts of
+  // 1 367 - 16 000 keys, 8 key heads of 128, bf16: 131 us with 1 024, 126 with 2 048, 125 with 4 096 and 4 us
+  // more in the second launch).  128-row tiles: 1 024 (8 chunks over up to 4 096 keys: 68 us with 256).
+  const int64_t target = p.form ? 2048 : 1024;
   const int64_t least = p.form ? kDecodeChunk * kDecodeLeast : 256;
   int64_t s = (target + busy - 1) / busy, most = (max_keys + least - 1) / least;
   if (s > most) s = most;

@@ -48,9 +48,9 @@ constexpr int kRowTile = 128;
 template <typename T, int D>
 __device__ __forceinline__ void clear_rows(T* out, const Index& cu, int64_t N, int64_t total, int H, int64_t first,
                                            int64_t step) {
-  int64_t lead, unused;
+  int lead, unused;
   seq_range(cu, 0, total, lead, unused);
-  const int64_t tail = max(tail_of(cu, N, total), lead);
+  const int64_t tail = max(tail_of(cu, N, total), (int64_t)lead);
   for (int64_t i = first; i < lead + total - tail; i += step) {
     T* row = out + (i < lead ? i : tail + i - lead) * (int64_t)H * D;
     for (int i = threadIdx.x; i < H * D / chunk_elems<T>(); i += blockDim.x)
@@ -60,13 +60,15 @@ __device__ __forceinline__ void clear_rows(T* out, const Index& cu, int64_t N, i
 
 // The next tile of keys (then of values, in the same registers) on its way from global memory to LDS:
 // thread t carries chunk t % CH of rows t / CH + i * (256 / CH).  Rows outside [0, end) are zeros, so nothing
-// that lies there (an unwritten page, the next sequence) can reach a product.  Keys are in flight during a
-// tile's scores and values during its second product: half the registers of both at once, which is
-// what keeps D = 128 in 256 of them (a spilled register's reload waits for every load issued before it).
+// that lies there (an unwritten page, the next sequence) can reach a product.  Rows of 256 bytes and more (D = 128):
+// the keys are in flight during a tile's scores and the values, in the same registers, during its second
+// product, which is what keeps the kernel in 256 registers (a spilled register's reload waits for every load
+// issued before it).  Shorter rows: both are in flight during the whole tile.
 template <typename T, int D, bool PAGED>
 struct KvStage {
   static constexpr int CH = D / chunk_elems<T>(), BK = key_tile<T>(), PER = BK * CH / 256, STEP = 256 / CH;
-  u32x4 r[PER];
+  static constexpr bool TURNS = D * sizeof(T) >= 256;  // keys, then values
+  u32x4 r[TURNS ? PER : 2 * PER];
   int slot[PER];  // paged: slots of the tile's rows, looked up a tile ahead of the loads: -1 behind the end, -2
                   // for a page outside the cache
 
@@ -83,7 +85,9 @@ struct KvStage {
     }
   }
   // base: the key head's row 0 (packed: of the sequence); row_stride in elements
+  template <int WHICH>  // 0 keys, 1 values
   __device__ __forceinline__ void load(const T* base, int64_t row_stride, int key0, int end) {
+    u32x4* r = this->r + (TURNS ? 0 : WHICH * PER);
     const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
     if constexpr (PAGED) {
 #pragma unroll
@@ -109,7 +113,9 @@ struct KvStage {
       }
     }
   }
+  template <int WHICH>
   __device__ __forceinline__ void store(char* tile) const {
+    const u32x4* r = this->r + (TURNS ? 0 : WHICH * PER);
     const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
 #pragma unroll
     for (int i = 0; i < PER; ++i) *reinterpret_cast<u32x4*>(tile + tile_at<T, D>(r0 + i * STEP, c)) = r[i];
@@ -133,7 +139,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
   // the last tiles of a sequence see the most keys: they go first
-  const int64_t want = a.tiles - 1 - blockIdx.x / a.Hkv;
+  const int want = (int)a.tiles - 1 - blockIdx.x / a.Hkv;
   const SeqTile t = find_tile(a.cu, a.N, a.total, a.G, kRowTile, want, lane);
   const int Hq = a.Hkv * a.G;
   if (t.seq < 0) {
@@ -188,12 +194,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   KvStage<T, D, PAGED> st;
   if (tile_lo < tile_hi) {
     st.locate(a, t.seq, tile_lo * BK, end);
-    st.load(kb, a.k_t, tile_lo * BK, end);
-    st.store(lds);
+    st.template load<0>(kb, a.k_t, tile_lo * BK, end);
+    st.template store<0>(lds);
     st.mark(s_hidden[0]);
-    st.load(vb, a.v_t, tile_lo * BK, end);
+    st.template load<1>(vb, a.v_t, tile_lo * BK, end);
     st.locate(a, t.seq, (tile_lo + 1) * BK, end);
-    st.store(lds + TILE);
+    st.template store<1>(lds + TILE);
   }
   __syncthreads();
   const LaneAt<T, D> at_lane(lane);
@@ -207,7 +213,15 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
     const int k0 = kt * BK;
     const bool sees = !EDGE || k0 < wave_end;
     u32x4 pf[NKB * NPS];
-    if (more) st.load(kb, a.k_t, k0 + BK, end);
+    constexpr bool TURNS = KvStage<T, D, PAGED>::TURNS;
+    if (more) {
+      st.template load<0>(kb, a.k_t, k0 + BK, end);
+      if (!TURNS) {
+        st.template load<1>(vb, a.v_t, k0 + BK, end);
+        st.mark(s_hidden[buf ^ 1]);
+        st.locate(a, t.seq, k0 + 2 * BK, end);
+      }
+    }
     if (sees) {
       f32x16 s[NKB];
 #pragma unroll
@@ -263,10 +277,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
         for (int i = 0; i < NPS; ++i) pf[b * NPS + i] = pack<T>(p + i * (KS / 2));
       }
     }
-    if (more) {
-      st.store(nk);
+    if (TURNS && more) {
+      st.template store<0>(nk);
       st.mark(s_hidden[buf ^ 1]);
-      st.load(vb, a.v_t, k0 + BK, end);
+      st.template load<1>(vb, a.v_t, k0 + BK, end);
       st.locate(a, t.seq, k0 + 2 * BK, end);
     }
     if (sees) {
@@ -277,7 +291,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
 #pragma unroll
           for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(at_lane.frag_t(tv, b * 32, i, d), pf[b * NPS + i], acc[d]);
     }
-    if (more) st.store(nk + TILE);
+    if (more) {
+      if (!TURNS) st.template store<0>(nk);
+      st.template store<1>(nk + TILE);
+    }
     __syncthreads();
   };
   // tiles that every row of the workgroup sees whole, without a mask or a branch; then the others

@@ -213,49 +213,45 @@ struct SeqTile {
   int tile;       // tile within the sequence
   int64_t start;  // first token of the sequence
   int len;        // its tokens
-  int64_t used;   // seq == -1: tiles there are in all
+  int used;       // seq == -1: tiles there are in all
 };
 
-// tokens [start, end) of sequence n, whatever the array holds: inside [0, total), never negative
-__device__ __forceinline__ void seq_range(const Index& cu, int64_t n, int64_t total, int64_t& start,
-                                          int64_t& end) {
+// tokens [start, end) of sequence n, whatever the array holds: inside [0, total), never negative (token
+// numbers fit 31 bits: sizes_fit)
+__device__ __forceinline__ void seq_range(const Index& cu, int64_t n, int64_t total, int& start, int& end) {
   const int64_t a = cu.at(n), b = cu.at(n + 1);
-  start = a < 0 ? 0 : (a > total ? total : a);
-  end = b < start ? start : (b > total ? total : b);
+  start = (int)(a < 0 ? 0 : (a > total ? total : a));
+  end = b < start ? start : (int)(b > total ? total : b);
 }
 
 // Tile number `want` of the batch: every sequence of L tokens has ceil(L * per / rows) tiles.  Each
 // wavefront scans the lengths 64 at a time (no shared memory, no barrier); the whole block gets the
 // same answer.
 __device__ __forceinline__ SeqTile find_tile(const Index& cu, int64_t N, int64_t total, int per, int rows,
-                                             int64_t want, int lane) {
-  int64_t base = 0;
+                                             int want, int lane) {
+  int base = 0;
   for (int64_t n0 = 0; n0 < N; n0 += 64) {
-    int64_t s = 0, e = 0;
+    int s = 0, e = 0;
     if (n0 + lane < N) seq_range(cu, n0 + lane, total, s, e);
-    const int len = (int)(e - s);
-    const int64_t tiles = ((int64_t)len * per + rows - 1) / rows;
-    int64_t upto = tiles;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t v = __shfl_up(upto, o, 64);
+    const int len = e - s, tiles = (int)(((uint32_t)len * (uint32_t)per + rows - 1) / (uint32_t)rows);
+    int upto = tiles;
+    const int most = N - n0 < 64 ? (int)(N - n0) : 64;
+    for (int o = 1; o < most; o <<= 1) {
+      const int v = __shfl_up(upto, o, 64);
       if (lane >= o) upto += v;
     }
-    const uint64_t beyond = __ballot(base + upto > want);
+    const uint64_t beyond = __ballot(base + upto > want && tiles > 0);
     if (beyond) {
       const int at = __builtin_ctzll(beyond);
       SeqTile t;
-      t.seq = __builtin_amdgcn_readfirstlane((int)(n0 + at));
-      const int64_t before = __shfl(upto - tiles, at, 64);
-      t.tile = __builtin_amdgcn_readfirstlane((int)(want - base - before));
-      t.len = __builtin_amdgcn_readfirstlane(__shfl(len, at, 64));
-      const int64_t st = __shfl(s, at, 64);
-      t.start = ((int64_t)__builtin_amdgcn_readfirstlane((int)(st >> 32)) << 32) |
-                (uint32_t)__builtin_amdgcn_readfirstlane((int)st);
+      t.seq = (int)n0 + at;
+      t.tile = want - base - __builtin_amdgcn_readlane(upto - tiles, at);
+      t.len = __builtin_amdgcn_readlane(len, at);
+      t.start = __builtin_amdgcn_readlane(s, at);
       t.used = 0;
       return t;
     }
-    base += __shfl(upto, 63, 64);
+    base += __builtin_amdgcn_readlane(upto, 63 < most - 1 ? 63 : most - 1);
   }
   return SeqTile{-1, 0, 0, 0, base};
 }
