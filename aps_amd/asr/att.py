@@ -1,8 +1,7 @@
 """
 Encoder-decoder acoustic models: `asr@att` (attention + RNN decoder) and `asr@xfmr` (Transformer
 decoder) of aps/asr/att.py:20-274 (forward path: asr_transform -> encoder -> [CTC branch] ->
-teacher-forced decoder).  Beam / greedy search and rescoring are decoding-side control flow
-outside the hot path (SURVEY.md 8 "out of scope").
+teacher-forced decoder; `XfmrASR.beam_search` runs the decoder over a key / value cache).
 """
 from typing import Dict, Optional
 
@@ -87,3 +86,11 @@ class XfmrASR(ASREncoderDecoderBase):
         enc_out, enc_ctc, enc_len = self._training_prep(x_pad, x_len)
         dec_out = self.decoder(enc_out, enc_len, y_pad, y_len)
         return dec_out, enc_ctc, enc_len
+
+    @th.no_grad()
+    def beam_search(self, x_pad: th.Tensor, x_len: NoneOrTensor = None, beam: int = 8, max_len: int = 100):
+        """x_pad N x Ti x D | N x S -> (tokens N x beam x L, scores N x beam, lengths N x beam), best first:
+        TorchTransformerDecoder.beam_search behind `sos`"""
+        enc_out, _, enc_len = self._training_prep(x_pad, x_len)
+        prompt = th.full((enc_out.shape[0], 1), self.sos, dtype=th.int64, device=enc_out.device)
+        return self.decoder.beam_search(enc_out, enc_len, prompt, self.eos, beam=beam, max_len=max_len)

@@ -13,7 +13,7 @@ of the general attention adjoint), the attention over the encoder output (aps_at
 the token embedding, and every dropout of the reference's layer -- on the attention weights, behind
 the two attentions and inside / behind the feed-forward -- as counter-based masks.
 """
-from typing import Dict, Optional, Tuple
+from typing import Callable, Dict, Optional, Tuple
 
 import torch as th
 import torch.nn as nn
@@ -22,8 +22,9 @@ from torch.nn import MultiheadAttention
 from aps_amd.asr.transformer.impl import _check_activation, get_activation_fn
 from aps_amd.grad_ops import ScaleAddFn, dropout, dropout_active
 from aps_amd.asr.transformer.pose import get_xfmr_pose
-from aps_amd.nn_ops import (attention_core, attention_cross, embedding_posenc, layernorm, linear,
-                            posenc_add)
+from aps_amd.nn_ops import (PACKED_HEAD_DIMS, attention_core, attention_cross, attention_packed,
+                            attention_paged, beam_reorder, beam_select, embedding_posenc, layernorm, linear,
+                            paged_append, posenc_add)
 
 
 class TransformerDncoderLayer(nn.Module):
@@ -60,8 +61,12 @@ class TransformerDncoderLayer(nn.Module):
         return linear(memory, att.in_proj_weight[D:], att.in_proj_bias[D:])
 
     def run(self, tgt: th.Tensor, memory: th.Tensor, tgt_len: Optional[th.Tensor],
-            mem_len: Optional[th.Tensor], memory_mask: Optional[th.Tensor] = None) -> th.Tensor:
-        """batch-major: tgt N x T x D, memory N x S x D -> N x T x D; memory_mask T x S additive"""
+            mem_len: Optional[th.Tensor], memory_mask: Optional[th.Tensor] = None,
+            self_attend: Optional[Callable[[th.Tensor], th.Tensor]] = None,
+            memory_kv: Optional[th.Tensor] = None) -> th.Tensor:
+        """batch-major: tgt N x T x D, memory N x S x D -> N x T x D; memory_mask T x S additive.
+        self_attend: what takes the place of the causal self attention over tgt itself (N x T x 3D -> N x T x D,
+        the attention over a cache); memory_kv: memory_kv(memory), formed once for many calls"""
         sa, ca = self.self_attn, self.multihead_attn
         D = sa.embed_dim
         n1, n2, n3 = self.norm1, self.norm2, self.norm3
@@ -79,13 +84,16 @@ class TransformerDncoderLayer(nn.Module):
 
         # self attention under the sub-sequence mask (prep_sub_mask): key j <= query i
         qkv = linear(tgt, sa.in_proj_weight, sa.in_proj_bias, ln=n1 if pre else None)
-        ctx = attention_core(qkv, self.nhead, tgt_len, chunk_size=1, lctx=-1, rctx=0,
-                             dropout=self.self_attn_drop)
+        if self_attend is not None:
+            ctx = self_attend(qkv)
+        else:
+            ctx = attention_core(qkv, self.nhead, tgt_len, chunk_size=1, lctx=-1, rctx=0,
+                                 dropout=self.self_attn_drop)
         tgt = post(out_proj(ctx, sa.out_proj, tgt, self.dropout1), n1)
         # attention over the encoder output
         q = linear(tgt, ca.in_proj_weight[:D], ca.in_proj_bias[:D], ln=n2 if pre else None)
-        ctx = attention_cross(q, self.memory_kv(memory), self.nhead, mem_len, memory_mask,
-                              dropout=self.cross_attn_drop)
+        ctx = attention_cross(q, self.memory_kv(memory) if memory_kv is None else memory_kv, self.nhead, mem_len,
+                              memory_mask, dropout=self.cross_attn_drop)
         tgt = post(out_proj(ctx, ca.out_proj, tgt, self.dropout2), n2)
         # feed-forward: Linear - activation - Dropout - Linear - Dropout
         up, down = self.feedforward[0], self.feedforward[3]
@@ -170,3 +178,75 @@ class TorchTransformerDecoder(nn.Module):
         """enc_out N x T x D, tgt_pad N x To -> N x To x V (decoder.py:168-186)"""
         dec_out, _ = self.step(enc_out.transpose(0, 1), tgt_pad, enc_len=enc_len, tgt_len=tgt_len)
         return dec_out.transpose(0, 1)
+
+    @th.no_grad()
+    def beam_search(self, enc_out: th.Tensor, enc_len: Optional[th.Tensor], prompt: th.Tensor, eos: int,
+                    beam: int = 8, max_len: int = 100) -> Tuple[th.Tensor, th.Tensor, th.Tensor]:
+        """Search over a key / value cache: enc_out N x T x D, prompt N x P tokens every hypothesis begins with (sos,
+        ...) -> (tokens N x beam x L, scores N x beam, lengths N x beam): the tokens behind the prompt, best
+        hypothesis first, score = the sum of their log-probabilities, eos included in tokens and lengths
+        (`max_len` tokens without one if none came); behind it eos.
+
+        The prompt goes through `attention_packed` and into a paged cache; then a step is one token a
+        hypothesis: `paged_append`, `attention_paged`, `beam_select`, `beam_reorder`.  A page holds one token,
+        so a hypothesis' past is a row of slot numbers: taking over another's past copies that row, no
+        keys or values.  The module must be in eval() mode (no dropout)."""
+        if self.training:
+            raise RuntimeError("beam_search: put the decoder into eval() mode")
+        N, P = prompt.shape
+        dev, dim = enc_out.device, self.vocab_embed.embedding_dim
+        layers = list(self.decoder.layers)
+        heads = layers[0].nhead
+        head_dim = dim // heads
+        if head_dim not in PACKED_HEAD_DIMS:
+            raise NotImplementedError(f"beam_search: heads of {head_dim}, the cache's attention takes {PACKED_HEAD_DIMS}")
+        if P < 1 or max_len < 1 or not 1 <= beam <= self.vocab_size:
+            raise RuntimeError(f"beam_search: prompt of {P} tokens, {max_len} more, {beam} of {self.vocab_size} tokens")
+        pose = self.abs_pos_enc
+        memory = enc_out.contiguous()
+        kvs = [layer.memory_kv(memory) for layer in layers]
+        caches = [th.empty(2, N * P + N * beam * max_len, 1, heads, head_dim, device=dev) for _ in layers]
+
+        def forward(tokens: th.Tensor, at: int, table: th.Tensor, cu: th.Tensor, lens: th.Tensor) -> th.Tensor:
+            """tokens N x rows x new (their positions at, at + 1, ...) -> logits of the last, N rows x V"""
+            _, rows, new = tokens.shape
+            x = embedding_posenc(self.vocab_embed.weight, tokens.reshape(N * rows, new), pose.div_term,
+                                 float(pose.factor), at).view(N, rows * new, dim)
+            for layer, kv, cache in zip(layers, kvs, caches):
+                def attend(qkv: th.Tensor) -> th.Tensor:
+                    q, k, v = qkv.view(-1, 3, heads, head_dim).unbind(1)
+                    paged_append(k, v, cache[0], cache[1], table, cu, lens)
+                    ctx = attention_packed(q, k, v, cu) if at == 0 else \
+                        attention_paged(q, cache[0], cache[1], table, cu, lens)
+                    return ctx.view(N, rows * new, dim)
+
+                x = layer.run(x, memory, None, enc_len, self_attend=attend, memory_kv=kv)
+            x = x.view(N * rows, new, dim)[:, -1]
+            return linear(x, self.output.weight, None, ln=self.decoder.norm)
+
+        # the prompt: one row of slots an utterance
+        table = th.zeros(N, P + max_len, dtype=th.int32, device=dev)
+        table[:, :P] = th.arange(N * P, dtype=th.int32, device=dev).view(N, P)
+        cu = th.arange(0, N * P + 1, P, dtype=th.int32, device=dev)
+        logits = forward(prompt.view(N, 1, P), 0, table, cu, th.full((N,), P, dtype=th.int32, device=dev))
+        scores, parent, token, done = beam_select(logits, th.zeros(N, 1, device=dev), eos, beam=beam)
+        (table,) = beam_reorder([table], parent)
+        tokens = th.full((N * beam, max_len), eos, dtype=th.int64, device=dev)
+        tokens[:, 0] = token.view(-1)
+        lengths = th.ones(N * beam, dtype=th.int64, device=dev)
+        cu = th.arange(N * beam + 1, dtype=th.int32, device=dev)
+        lens = th.full((N * beam,), P, dtype=th.int32, device=dev)
+        slots = N * P + th.arange(N * beam, dtype=th.int32, device=dev)
+        for t in range(1, max_len):
+            if t % 8 == 0 and bool(done.all()):  # (a look at the device every eighth step)
+                break
+            lens += 1
+            table[:, P + t - 1] = slots + N * beam * (t - 1)
+            logits = forward(token.view(N, beam, 1), P + t - 1, table, cu, lens)
+            scores, parent, token, done_next = beam_select(logits, scores, eos, finished=done)
+            table, tokens, lengths, done = beam_reorder([table, tokens, lengths, done.view(-1)], parent)
+            tokens[:, t] = token.view(-1)
+            lengths += ~done
+            done = done_next
+        tokens = tokens[:, :int(lengths.max())]
+        return tokens.view(N, beam, -1), scores, lengths.view(N, beam)

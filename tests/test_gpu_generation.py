@@ -253,3 +253,144 @@ def test_beam_reorder():
     odd = nn_ops.beam_reorder([states[0]], parent.clone().fill_(4))[0]
     assert (odd == 0).all()
     assert nn_ops.beam_reorder([], parent) == []
+
+
+# ---- together ------------------------------------------------------------------------------------
+
+def search_reference(step, n, prompt, eos, beam, max_len):
+    """beam search by running the whole prefix again at every step; step(tokens R x L, utterance of each row) ->
+    logits R x V in 64 bits"""
+    out = []
+    for i in range(n):
+        hyps = [(0.0, [], False)]
+        for t in range(max_len):
+            found = []
+            for b, (score, toks, done) in enumerate(hyps):
+                if done:
+                    found.append((-score, b, eos, toks, True))
+                    continue
+                logp = torch.log_softmax(step(torch.tensor([prompt[i] + toks]), [i])[0], 0)
+                for v, x in enumerate(logp.tolist()):
+                    found.append((-(score + x), b, v, toks + [v], v == eos))
+            found.sort(key=lambda f: f[:3])
+            hyps = [(-f[0], f[3], f[4]) for f in found[:beam]]
+        out.append(hyps)
+    return out
+
+
+@gpu
+@pytest.mark.parametrize("pre_norm,prompt_len", [(True, 1), (False, 3)])
+def test_beam_search_equals_the_whole_prefix(pre_norm, prompt_len):
+    """the decoder's search over the cache against a search that runs the decoder's teacher-forced forward over
+    every prefix: the same hypotheses, scores to f32 rounding"""
+    from aps_amd.asr.transformer.decoder import TorchTransformerDecoder
+    torch.manual_seed(11)
+    V, n, beam, max_len, eos = 23, 3, 4, 7, 2
+    dec = TorchTransformerDecoder(V, pose_kwargs={"dropout": 0}, num_layers=2,
+                                  arch_kwargs={"att_dim": 64, "nhead": 2, "feedforward_dim": 128, "pre_norm": pre_norm,
+                                               "att_dropout": 0, "ffn_dropout": 0}).eval().to(DEV)
+    with torch.no_grad():
+        dec.output.weight.mul_(3.0)  # confident enough that hypotheses end
+    enc = randn(n, 19, 64, seed=3)
+    enc_len = torch.tensor([19, 11, 5], device=DEV)
+    prompt = torch.randint(3, V, (n, prompt_len), generator=torch.Generator().manual_seed(5))
+    tokens, scores, lengths = dec.beam_search(enc, enc_len, prompt.to(DEV), eos, beam=beam, max_len=max_len)
+
+    def step(toks, rows):
+        with torch.no_grad():
+            return dec(enc[rows], enc_len[rows], toks.to(DEV), None)[:, -1].double().cpu()
+
+    want = search_reference(step, n, prompt.tolist(), eos, beam, max_len)
+    for i in range(n):
+        for b in range(beam):
+            score, toks, done = want[i][b]
+            assert lengths[i, b].item() == len(toks)
+            assert tokens[i, b, :len(toks)].tolist() == toks
+            assert (tokens[i, b, len(toks):] == eos).all()
+            assert abs(scores[i, b].item() - score) < 1e-4 * max(1.0, abs(score))
+
+
+@gpu
+def test_serving_run_with_grouped_heads():
+    """prompts packed -> cache -> chunks and single tokens of it, in bf16 with grouped heads, captured: every
+    token's attention equals the packed attention over the whole sequence"""
+    from aps_amd import nn_ops
+    hq, hkv, d, page = 8, 2, 64, 16
+    lens = [70, 1, 33]
+    total = sum(lens)
+    q, k, v = (randn(total, h, d, dtype=torch.bfloat16, seed=i) for i, h in enumerate((hq, hkv, hkv)))
+    (want,), (bound,) = ref.packed(q, k, v, lens, True)
+    width = 6
+    table = torch.randperm(3 * width, generator=torch.Generator().manual_seed(1)).view(3, width).int().to(DEV)
+    kc, vc = (torch.full((3 * width, page, hkv, d), float("nan"), dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    starts = [0, 70, 71]
+    got = torch.zeros_like(q)
+    done = [0, 0, 0]
+    for chunk in ([17, 0, 1], [1, 1, 30], [40, 0, 1], [12, 0, 1]):
+        rows = [starts[i] + done[i] + j for i in range(3) for j in range(chunk[i])]
+        done = [a + b for a, b in zip(done, chunk)]
+        rows = torch.tensor(rows, device=DEV)
+        args = (kc, vc, table, cu_of(chunk), torch.tensor(done, device=DEV))
+        nn_ops.paged_append(k[rows], v[rows], *args)
+        got[rows] = nn_ops.attention_paged(q[rows], *args)
+    assert done == lens
+    ref.check(got, want, bound, "chunks")
+
+
+@gpu
+def test_captured_step_replays():
+    """append + attention + selection + reordering captured once; replays with other contents, eager work in
+    between, equal the eager calls bit for bit"""
+    from aps_amd import nn_ops
+    n, b, h, d, V, T = 2, 3, 4, 64, 501, 50
+    q, k, v = (randn(n * b, h, d, seed=i) for i in range(3))
+    kc, vc = (torch.zeros(n * b * T, 1, h, d, device=DEV) for _ in range(2))
+    table = torch.arange(n * b * T, dtype=torch.int32, device=DEV).view(n * b, T)
+    lens = torch.full((n * b,), 1, dtype=torch.int32, device=DEV)
+    cu = torch.arange(n * b + 1, dtype=torch.int32, device=DEV)
+    logits, scores = randn(n * b, V, seed=4), randn(n, b, seed=5)
+
+    def step():
+        nn_ops.paged_append(k, v, kc, vc, table, cu, lens)
+        ctx = nn_ops.attention_paged(q, kc, vc, table, cu, lens)
+        sel = nn_ops.beam_select(logits, scores, 1)
+        return [ctx, *sel] + nn_ops.beam_reorder([table, ctx], sel[1])
+
+    with torch.no_grad():
+        step()
+        torch.cuda.synchronize()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = step()
+        for i in range(4):
+            lens.fill_(1 + 11 * i)
+            for j, x in enumerate((q, k, v, logits)):
+                x.copy_(randn(*x.shape, seed=100 * i + j))
+            graph.replay()
+            torch.cuda.synchronize()
+            first = [x.clone() for x in held]
+            again = step()
+            assert all(torch.equal(x, y) for x, y in zip(first, again)), i
+
+
+@gpu
+def test_other_streams_and_repeat():
+    """two streams at once, each with its own call: the same bits as one after the other"""
+    from aps_amd import nn_ops
+    lens = [300, 45, 128]
+    cases = [[randn(sum(lens), h, 64, dtype=torch.float16, seed=10 * s + i) for i, h in enumerate((6, 3, 3))] for s in range(2)]
+    cu = cu_of(lens)
+    with torch.no_grad():
+        want = [nn_ops.attention_packed(*c, cu) for c in cases]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in cases]
+        for _ in range(3):
+            got = []
+            for s, c in zip(streams, cases):
+                s.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(s):
+                    got.append(nn_ops.attention_packed(*c, cu))
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
