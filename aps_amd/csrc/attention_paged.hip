@@ -31,6 +31,13 @@ __device__ __forceinline__ f32x4 mma16<float>(u32x4 a, u32x4 b, f32x4 c) {
   return c;
 }
 
+// element e of a run of values held as 32-bit words
+template <typename T>
+__device__ __forceinline__ float value_at(const uint32_t* w, int e) {
+  if constexpr (sizeof(T) == 4) return __uint_as_float(w[e]);
+  else return (float)__builtin_bit_cast(T, (uint16_t)((e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xffff));
+}
+
 // A workgroup owns 16 R rows of one (sequence, key head) and a range of its keys; each of its four
 // wavefronts walks that range in chunks of 32 keys with a softmax of its own, straight from global
 // memory to the matrix operands: no LDS, no barrier until the four meet at the end.
@@ -134,6 +141,40 @@ __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void atte
         vr[j][0] = row >= 0 ? *reinterpret_cast<const uint32_t*>(vp) : 0u;
       }
     }
+    const int k0 = ch * kDecodeChunk;
+    // (a chunk past `end` or with a missing page is masked, so its zeros carry no weight)
+    const bool mask = k0 + kDecodeChunk - 1 > least || __any(slot < 0);
+    if (mask) {
+      // Some row may not see all of the chunk, and 0 * infinity is not 0: a non-finite value is taken out of the
+      // products and added to the rows that see it (element c VE + e belongs to lanes 4 g + i = c)
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int e = 0; e < VE; ++e) bad |= !finite(value_at<T>(vr[j], e));
+      if (__any(bad)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int e = 0; e < VE; ++e) {
+            const float x = value_at<T>(vr[j], e);
+            if (!finite(x)) {
+              if constexpr (sizeof(T) == 2) vr[j][e >> 1] &= (e & 1) ? 0xffffu : 0xffff0000u;
+              else vr[j][e] = 0;
+            }
+            for (uint64_t left = __ballot(!finite(x)); left; left &= left - 1) {
+              const int from = __builtin_ctzll(left), fg = from >> 4, fc = from & 15;
+              const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), from));
+              const int key = k0 + (j >> 2) * 16 + fg * 4 + (j & 3);
+#pragma unroll
+              for (int r = 0; r < R; ++r)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (g * 4 + i == fc && key <= pos[r]) acc[r][e][i] += v;
+            }
+          }
+      }
+    }
     // V by element: 16-bit, va[e] = element e of the 8 keys
     u32x4 va[VE];
     if constexpr (sizeof(T) == 2) {
@@ -145,9 +186,6 @@ __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void atte
           va[e][j] = (e & 1) ? __builtin_amdgcn_perm(y, x, 0x07060302) : __builtin_amdgcn_perm(y, x, 0x05040100);
         }
     }
-    const int k0 = ch * kDecodeChunk;
-    // (a chunk past `end` or with a missing page is masked, so its zeros carry no weight)
-    const bool mask = k0 + kDecodeChunk - 1 > least || __any(slot < 0);
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       f32x4 s[2] = {f32x4{0}, f32x4{0}};
@@ -172,8 +210,8 @@ __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void atte
       top = fmaxf(top, __shfl_xor(top, 16, 64));
       top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
       if (__any(top > m[r] + 8.f)) {
-        const float to = fmaxf(m[r], top);
-        const float f = to == -INFINITY ? 1.f : exp2_fast(m[r] - to);
+        const float to = top > m[r] + 8.f ? top : m[r];
+        const float f = m[r] == -INFINITY ? 1.f : exp2_fast(m[r] - to);
         m[r] = to;
         l[r] *= f;
 #pragma unroll

@@ -120,6 +120,16 @@ struct KvStage {
 #pragma unroll
     for (int i = 0; i < PER; ++i) *reinterpret_cast<u32x4*>(tile + tile_at<T, D>(r0 + i * STEP, c)) = r[i];
   }
+  // Values on their way to a tile that some row sees only in part: 0 * infinity is not 0, so a non-finite
+  // value would reach the rows it is hidden from.  It goes to LDS as 0 and is added to the rows that see it
+  // in the end (`add_non_finite`).  True if there was one.
+  __device__ __forceinline__ bool sanitize() {
+    u32x4* v = r + (TURNS ? 0 : PER);
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) v[i] = only_finite<T>(v[i], any);
+    return any;
+  }
   __device__ __forceinline__ void mark(uint8_t* hidden) const {
     if constexpr (PAGED) {
       if (threadIdx.x % CH == 0) {
@@ -130,8 +140,34 @@ struct KvStage {
   }
 };
 
+// the non-finite values of keys [from, to) to the rows that see them (seldom: straight from global memory)
 template <typename T, int D, bool PAGED>
-__global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void attention_rows_kernel(RowsArgs a) {
+__device__ __forceinline__ void add_non_finite(const RowsArgs& a, const T* base, int seq, int from, int to, int pos,
+                                               int half, f32x16* acc) {
+  for (int key = from; key < to; ++key) {
+    int64_t row = key;
+    if constexpr (PAGED) {
+      const int32_t p = a.table[(int64_t)seq * a.table_stride + (key >> a.page_shift)];
+      if (p < 0 || p >= a.num_pages) continue;
+      row = ((int64_t)p << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+    }
+    if (key > pos) continue;
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float x = (float)base[row * a.v_t + d * 32 + result_row(i, half)];
+        acc[d][i] += finite(x) ? 0.f : x;
+      }
+  }
+}
+
+// wavefronts a SIMD has registers for
+template <typename T, int D>
+constexpr int rows_waves(bool paged) { return D * sizeof(T) >= 512 ? 1 : (D * sizeof(T) >= 256 || paged ? 2 : 3); }
+
+template <typename T, int D, bool PAGED>
+__global__ __launch_bounds__(256, (rows_waves<T, D>(PAGED))) void attention_rows_kernel(RowsArgs a) {
   constexpr int BK = key_tile<T>(), KS = 2 * chunk_elems<T>(), NS = D / KS, NKB = BK / 32, NDB = D / 32;
   constexpr int NPS = 32 / KS, TILE = BK * D * (int)sizeof(T);
   __shared__ __align__(16) char lds[4 * TILE];
@@ -192,6 +228,10 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   const T* kb = static_cast<const T*>(a.k) + h * a.k_h + (PAGED ? 0 : t.start * a.k_t);
   const T* vb = static_cast<const T*>(a.v) + h * a.v_h + (PAGED ? 0 : t.start * a.v_t);
   KvStage<T, D, PAGED> st;
+  bool bad = false;  // a non-finite value in a tile that some row sees only in part
+  // tiles that every row of the workgroup sees whole: no mask, no branch; then the others
+  const int block_min = a.causal ? off + t.tile * kRowTile / a.G : kv - 1;
+  const int clear = min(tile_hi, (block_min + 1) / BK);
   if (tile_lo < tile_hi) {
     st.locate(a, t.seq, tile_lo * BK, end);
     st.template load<0>(kb, a.k_t, tile_lo * BK, end);
@@ -199,6 +239,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
     st.mark(s_hidden[0]);
     st.template load<1>(vb, a.v_t, tile_lo * BK, end);
     st.locate(a, t.seq, (tile_lo + 1) * BK, end);
+    if (tile_lo >= clear) bad |= st.sanitize();
     st.template store<1>(lds + TILE);
   }
   __syncthreads();
@@ -255,8 +296,9 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
       top = fmaxf(top, __shfl_xor(top, 32, 64)) * a.c;
       if (__any(top > m + 8.f)) {
         rare();
-        const float to = fmaxf(m, top);
-        const float f = to == -INFINITY ? 1.f : exp2_fast(m - to);
+        // (lane by lane: what a row comes to does not depend on the rows beside it)
+        const float to = top > m + 8.f ? top : m;
+        const float f = m == -INFINITY ? 1.f : exp2_fast(m - to);
         m = to;
         l *= f;
 #pragma unroll
@@ -293,17 +335,22 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
     }
     if (more) {
       if (!TURNS) st.template store<0>(nk);
+      if (EDGE || kt + 1 >= clear) {
+        rare();
+        bad |= st.sanitize();
+      }
       st.template store<1>(nk + TILE);
     }
     __syncthreads();
   };
-  // tiles that every row of the workgroup sees whole, without a mask or a branch; then the others
-  const int block_min = a.causal ? off + t.tile * kRowTile / a.G : kv - 1;
-  const int clear = min(tile_hi, (block_min + 1) / BK);
   int kt = tile_lo;
   for (; kt < clear; ++kt) step(kt, (kt - tile_lo) & 1, std::false_type());
   for (; kt < tile_hi; ++kt) step(kt, (kt - tile_lo) & 1, std::true_type());
   l += __shfl_xor(l, 32, 64);
+  if (clear < tile_hi && __syncthreads_or(bad)) {
+    rare();
+    add_non_finite<T, D, PAGED>(a, vb, t.seq, max(clear, tile_lo) * BK, min(end, tile_hi * BK), pos, half, acc);
+  }
   if (!live) return;
   const int64_t at = (t.start + tok) * Hq + head;
   if constexpr (PAGED) {

@@ -111,6 +111,30 @@ __device__ __forceinline__ float dot_chunk(u32x4 a, u32x4 b) {
   return s;
 }
 
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234663852886e38f; }
+
+// element e of a chunk / the chunk with its non-finite elements zeroed (`any` set if there were some)
+template <typename T>
+__device__ __forceinline__ float chunk_at(u32x4 v, int e) {
+  if constexpr (sizeof(T) == 2) return (float)__builtin_bit_cast(typename Vec<T>::v8, v)[e];
+  else return __builtin_bit_cast(f32x4, v)[e];
+}
+template <typename T>
+__device__ __forceinline__ u32x4 only_finite(u32x4 v, bool& any) {
+  // an exponent of ones: infinity or NaN
+  constexpr uint32_t one = sizeof(T) == 4 ? 0x7f800000u : (__is_same(T, __bf16) ? 0x7f80u : 0x7c00u);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if constexpr (sizeof(T) == 4) {
+      if ((v[w] & one) == one) v[w] = 0, any = true;
+    } else {
+      if ((v[w] & one) == one) v[w] &= 0xffff0000u, any = true;
+      if ((v[w] & (one << 16)) == one << 16) v[w] &= 0xffffu, any = true;
+    }
+  }
+  return v;
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 

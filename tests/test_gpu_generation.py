@@ -394,3 +394,124 @@ def test_other_streams_and_repeat():
                     got.append(nn_ops.attention_packed(*c, cu))
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- what a row cannot see -----------------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("kind,hq,hkv,d", [("f32", 2, 2, 64), ("bf16", 4, 2, 128), ("f16", 3, 1, 32), ("f32", 3, 1, 128)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_non_finite_keys_and_values_reach_only_the_rows_that_see_them(kind, hq, hkv, d, bad):
+    from aps_amd import nn_ops
+    lens, at = [90, 40], 37
+    q, k, v = (randn(sum(lens), h, d, dtype=TYPES[kind], seed=i) for i, h in enumerate((hq, hkv, hkv)))
+    cu = cu_of(lens)
+    table = torch.arange(2 * 6, dtype=torch.int32, device=DEV).view(2, 6)
+    kv_lens = torch.tensor(lens, device=DEV)
+    with torch.no_grad():
+        clean = nn_ops.attention_packed(q, k, v, cu)
+        for which in (k, v):
+            kept = which[at, 0, 5].clone()
+            which[at, 0, 5] = bad
+            out = nn_ops.attention_packed(q, k, v, cu)
+            cache = [torch.full((12, 16, hkv, d), float("nan"), dtype=q.dtype, device=DEV) for _ in range(2)]
+            nn_ops.paged_append(k, v, *cache, table, cu, kv_lens)
+            full = nn_ops.attention_paged(q, *cache, table, cu, kv_lens)
+            few = torch.tensor([0, 6, 6], device=DEV)  # the row's neighbours as new tokens: the few-row kernel
+            rows = torch.arange(at - 3, at + 3, device=DEV)
+            small = nn_ops.attention_paged(q[rows], *cache, table, few, torch.tensor([at + 3, 0], device=DEV))
+            which[at, 0, 5] = kept
+            assert torch.equal(out[:at], clean[:at]) and torch.equal(out[90:], clean[90:])
+            ref.check(full[:at], clean[:at].double().cpu(), torch.full(clean[:at].shape, 2e-2 if kind != "f32" else 1e-5))
+            ref.check(small[:3], clean[at - 3:at].double().cpu(),
+                      torch.full(small[:3].shape, 2e-2 if kind != "f32" else 1e-5))
+            if which is v:  # a weight is positive: the value arrives as it is, in its own element and heads
+                group = hq // hkv
+                for o in (out[at:90], full[at:90], small[3:]):
+                    hit = o[:, :group, 5].float()
+                    assert (torch.isnan(hit) if bad != bad else hit == bad).all()
+                    o[:, :group, 5] = 0
+                    assert torch.isfinite(o).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_rows_that_see_nothing_and_pages_that_are_not_there(kind):
+    from aps_amd import nn_ops
+    hq, hkv, d, page = 4, 2, 64, 16
+    dt = TYPES[kind]
+    kc, vc = (randn(8, page, hkv, d, dtype=dt, seed=i) for i in range(2))
+    # sequences: no positions, fewer positions than new tokens, a missing middle page, every page missing
+    table = torch.tensor([[0, 1, 2], [3, 4, 5], [0, 99, 2], [-1, -5, 8]], dtype=torch.int32, device=DEV)
+    for new in (1, 5, 40):
+        lens = torch.tensor([0, 3, 45, 45], device=DEV, dtype=torch.int32)
+        q = randn(4 * new, hq, d, dtype=dt, seed=9)
+        cu = cu_of([new] * 4)
+        with torch.no_grad():
+            out = nn_ops.attention_paged(q, kc, vc, table, cu, lens)
+        assert (out[:new] == 0).all() and (out[3 * new:] == 0).all()
+        for i in range(new):
+            for s, slots in ((1, [(3, p) for p in range(3)]), (2, [(0, p) for p in range(16)] + [(2, p) for p in range(13)])):
+                pos = (3 if s == 1 else 45) - new + i
+                # positions of the slots: sequence 1: 0 .. 2; sequence 2: 0 .. 15 and 32 .. 44
+                at = [p for p in (range(3) if s == 1 else list(range(16)) + list(range(32, 45))) if p <= pos]
+                use = slots[:len(at)]
+                got = out[s * new + i]
+                if not use:
+                    assert (got == 0).all()
+                    continue
+                ks = torch.stack([kc[a, b] for a, b in use]).cpu().double()
+                vs = torch.stack([vc[a, b] for a, b in use]).cpu().double()
+                for h in range(hq):
+                    want, bound = ref.attend(q[s * new + i, h][None].cpu().double(), ks[:, h // 2], vs[:, h // 2], 0, False,
+                                             d**-0.5, dt)
+                    ref.check(got[h][None], want, bound, f"new {new} row {i} sequence {s}")
+        before = (kc.clone(), vc.clone())
+        nn_ops.paged_append(q[:, :2], q[:, 2:], kc, vc, table[3:], cu_of([4 * new]), torch.tensor([4 * new], device=DEV))
+        assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+
+
+@gpu
+def test_empty_calls_and_layouts():
+    from aps_amd import nn_ops
+    e = torch.empty(0, 4, 64, device=DEV)
+    assert nn_ops.attention_packed(e, e, e, cu_of([0, 0])).shape == e.shape
+    x = randn(0, 4, 64).requires_grad_()
+    (gx,) = torch.autograd.grad(nn_ops.attention_packed(x, x, x, cu_of([0])).sum(), x)
+    assert gx.shape == x.shape
+    # any strides: heads before rows, a broadcast head, an expanded gradient, an unaligned slice
+    base = randn(3, 50, 72, seed=1)
+    q = base[:, :, 3:67].transpose(0, 1)          # unaligned, rows x heads by stride
+    k = randn(50, 1, 64, seed=2).expand(50, 3, 64)
+    v = randn(50, 3, 128, seed=3)[:, :, ::2]      # not contiguous in the last axis
+    lens = [20, 30]
+    (want,), (bound,) = ref.packed(q, k, v, lens, True)
+    ref.check(nn_ops.attention_packed(q, k, v, cu_of(lens)), want, bound)
+    leaf = randn(50, 1, 64, seed=2).requires_grad_()
+    out = nn_ops.attention_packed(q, leaf.expand(50, 3, 64), v, cu_of(lens))
+    (gl,) = torch.autograd.grad(out.sum(), leaf)
+    vals, bounds = ref.packed(q, k, v, lens, True, g=torch.ones(50, 3, 64))
+    ref.check(gl, vals[2].sum(1, keepdim=True), bounds[2].sum(1, keepdim=True) * 1.01 + 1e-6)
+
+
+@gpu
+def test_gradients_against_differences():
+    """central differences of a weighted sum in the directions of a few random tensors: f32, step h, error of the
+    difference <= h^2 |third derivative| / 6 + rounding of the sum / h, both far under 2e-3 of the slope here"""
+    from aps_amd import nn_ops
+    lens = [9, 1, 23]
+    x = [randn(33, h, 32, seed=i).requires_grad_() for i, h in enumerate((4, 2, 2))]
+    w = randn(33, 4, 32, seed=8).double()
+    grads = torch.autograd.grad((nn_ops.attention_packed(*x, cu_of(lens)) * w.float()).sum(), x)
+    for i in range(3):
+        for s in range(3):
+            step = randn(*x[i].shape, seed=20 + s)
+            h = 1e-2
+
+            def f(sign):
+                y = [t.detach() + (sign * h * step if j == i else 0) for j, t in enumerate(x)]
+                return (nn_ops.attention_packed(*y, cu_of(lens)).double() * w).sum().item()
+
+            slope = (f(1) - f(-1)) / (2 * h)
+            exact = (grads[i].double() * step.double()).sum().item()
+            assert abs(slope - exact) < 2e-3 * (grads[i].double().norm() * step.double().norm()).item()
