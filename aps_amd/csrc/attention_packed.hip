@@ -27,9 +27,8 @@ struct GradArgs {
 // dq: the forward kernel's walk, with V as the left operand of dP^T = V dO^T beside S^T = K Q^T and K
 // read transposed for dq^T = K^T dS^T
 template <typename T, int D>
-__global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void attention_rows_backward_kernel(GradArgs a) {
-  constexpr int BK = key_tile<T>(), E = chunk_elems<T>(), KS = 2 * E, NS = D / KS, NKB = BK / 32, NDB = D / 32;
-  constexpr int NPS = 32 / KS, TILE = BK * D * (int)sizeof(T);
+__global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attention_rows_backward_kernel(GradArgs a) {
+  constexpr int BK = key_tile<T, D>(), NS = D / 16, NKB = BK / 32, NDB = D / 32, PLANE = BK * D * 2, TILE = planes<T>() * PLANE;
   __shared__ __align__(16) char lds[4 * TILE];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
@@ -54,17 +53,18 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   const T* qp = static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + head * a.q_h;
   const T* gp = static_cast<const T*>(a.go) + (t.start + tok) * a.go_t + head * a.go_h;
   const T* op = static_cast<const T*>(a.o) + at * D;
-  u32x4 qf[NS], gf[NS];
+  Frag<T> qf[NS], gf[NS];
   float delta = 0.f;
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
-    qf[s] = gf[s] = u32x4{0, 0, 0, 0};
+    Raw<T> x = zero_raw<T>(), g = zero_raw<T>();
     if (live) {
-      const int c = (2 * s + half) * E;
-      qf[s] = *reinterpret_cast<const u32x4*>(qp + c);
-      gf[s] = *reinterpret_cast<const u32x4*>(gp + c);
-      delta += dot_chunk<T>(gf[s], *reinterpret_cast<const u32x4*>(op + c));
+      const int c = (2 * s + half) * kChunk;
+      x = load_raw<T>(reinterpret_cast<const char*>(qp + c));
+      g = load_raw<T>(reinterpret_cast<const char*>(gp + c));
+      delta += dot_raw<T>(g, load_raw<T>(reinterpret_cast<const char*>(op + c)));
     }
+    qf[s] = operand<T>(x), gf[s] = operand<T>(g);
   }
   delta += __shfl_xor(delta, 32, 64);
   const float lse = live ? a.lse[at] : INFINITY;
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
   st.template load<1>(vb, a.v_t, 0, end);
   st.template store<1>(lds + TILE);
   __syncthreads();
-  const LaneAt<T, D> at_lane(lane);
+  const LaneAt<T, D, PLANE> at_lane(lane);
   auto step = [&](int kt, int buf, auto masked) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(masked)::value;
     const char* tk = lds + buf * 2 * TILE;
@@ -125,8 +125,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
           if (k0 + b * 32 + result_row(i, half) > pos) p[i] = 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < NPS; ++i) {
-        const u32x4 pf = pack<T>(p + i * (KS / 2));
+      for (int i = 0; i < 2; ++i) {
+        const Frag<T> pf = pack<T>(p + i * 8);
 #pragma unroll
         for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(at_lane.frag_t(tk, b * 32, i, d), pf, acc[d]);
       }
@@ -161,14 +161,14 @@ __global__ __launch_bounds__(256, (sizeof(T) == 4 && D >= 128 ? 1 : 2)) void att
 // waits for (128-key tiles: %K128%; 64: %K64% on 12 sequences of 64 - 2 048 tokens, 16 / 4 heads of 128, bf16).  f32 with
 // D = 128 has no registers for the larger row tile: four times 32 keys there.
 template <typename T, int D>
-constexpr int grad_rows() { return D * sizeof(T) >= 512 ? 32 : 64; }
+constexpr int grad_rows() { return D * planes<T>() >= 384 ? 32 : 64; }
 template <typename T, int D>
 constexpr int grad_keys() { return 32 * 4 / (grad_rows<T, D>() / 32); }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention_keys_backward_kernel(GradArgs a) {
-  constexpr int BR = grad_rows<T, D>(), RG = BR / 32, KG = 4 / RG, E = chunk_elems<T>(), CH = D / E, KS = 2 * E, NS = D / KS;
-  constexpr int NDB = D / 32, NPS = 32 / KS, TILE = BR * D * (int)sizeof(T), PER = BR * CH / 256, STEP = 256 / CH;
+__global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attention_keys_backward_kernel(GradArgs a) {
+  constexpr int BR = grad_rows<T, D>(), RG = BR / 32, KG = 4 / RG, CH = D / kChunk, NS = D / 16, NDB = D / 32;
+  constexpr int PLANE = BR * D * 2, TILE = planes<T>() * PLANE, PER = BR * CH / 256, STEP = 256 / CH;
   __shared__ __align__(16) char lds[4 * TILE];
   __shared__ __align__(16) float s_lse[2][BR], s_delta[2][BR];
   __shared__ __align__(16) int s_pos[2][BR];
@@ -186,14 +186,15 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
   }
   const int tile0 = t.tile * grad_keys<T, D>(), key0 = tile0 + wv % KG * 32, key = key0 + (lane & 31);
   const bool live = key < t.len;
-  u32x4 kf[NS], vf[NS];
+  Frag<T> kf[NS], vf[NS];
   {
     const T* kp = static_cast<const T*>(a.k) + (t.start + (live ? key : 0)) * a.k_t + h * a.k_h;
     const T* vp = static_cast<const T*>(a.v) + (t.start + (live ? key : 0)) * a.v_t + h * a.v_h;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      kf[s] = live ? *reinterpret_cast<const u32x4*>(kp + (2 * s + half) * E) : u32x4{0, 0, 0, 0};
-      vf[s] = live ? *reinterpret_cast<const u32x4*>(vp + (2 * s + half) * E) : u32x4{0, 0, 0, 0};
+      const int c = (2 * s + half) * kChunk;
+      kf[s] = operand<T>(live ? load_raw<T>(reinterpret_cast<const char*>(kp + c)) : zero_raw<T>());
+      vf[s] = operand<T>(live ? load_raw<T>(reinterpret_cast<const char*>(vp + c)) : zero_raw<T>());
     }
   }
   f32x16 gk[NDB], gv[NDB];
@@ -216,13 +217,13 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
   for (int i = 0; i < PER; ++i) {
     place(threadIdx.x / CH + i * STEP, tok_i[i], head_i[i]);
     const int tk = min(tok_i[i], BR);
-    q_at[i] = (uint32_t)((tk * (int)a.q_t + head_i[i] * (int)a.q_h) * (int)sizeof(T) + threadIdx.x % CH * 16);
-    g_at[i] = (uint32_t)((tk * (int)a.go_t + head_i[i] * (int)a.go_h) * (int)sizeof(T) + threadIdx.x % CH * 16);
+    q_at[i] = (uint32_t)((tk * (int)a.q_t + head_i[i] * (int)a.q_h) * (int)sizeof(T) + threadIdx.x % CH * (kChunk * (int)sizeof(T)));
+    g_at[i] = (uint32_t)((tk * (int)a.go_t + head_i[i] * (int)a.go_h) * (int)sizeof(T) + threadIdx.x % CH * (kChunk * (int)sizeof(T)));
   }
   place(threadIdx.x & (BR - 1), tok_s, head_s);
   const char* qb = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + t.start * a.q_t + (int64_t)h * a.G * a.q_h);
   const char* gb = reinterpret_cast<const char*>(static_cast<const T*>(a.go) + t.start * a.go_t + (int64_t)h * a.G * a.go_h);
-  u32x4 qr[PER], gr[PER];
+  Raw<T> qr[PER], gr[PER];
   float r_lse = INFINITY, r_delta = 0.f;
   int r_pos = -1;
   auto load = [&](int rt) {
@@ -231,13 +232,13 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
     const char* g0 = gb + (tok0 * a.go_t + head0 * a.go_h) * (int)sizeof(T);
     if (toks * span == BR && tok0 + toks <= t.len && head0 + span <= a.G) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) qr[i] = load_chunk(q0, q_at[i]), gr[i] = load_chunk(g0, g_at[i]);
+      for (int i = 0; i < PER; ++i) qr[i] = load_chunk<T>(q0, q_at[i]), gr[i] = load_chunk<T>(g0, g_at[i]);
     } else {
       rare();
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        qr[i] = gr[i] = u32x4{0, 0, 0, 0};
-        if (tok_i[i] < t.len - tok0 && head0 + head_i[i] < a.G) qr[i] = load_chunk(q0, q_at[i]), gr[i] = load_chunk(g0, g_at[i]);
+        qr[i] = gr[i] = zero_raw<T>();
+        if (tok_i[i] < t.len - tok0 && head0 + head_i[i] < a.G) qr[i] = load_chunk<T>(q0, q_at[i]), gr[i] = load_chunk<T>(g0, g_at[i]);
       }
     }
     if (threadIdx.x < BR) {
@@ -252,9 +253,8 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
     char* tq = lds + buf * 2 * TILE;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int at = tile_at<T, D>(threadIdx.x / CH + i * STEP, threadIdx.x % CH);
-      *reinterpret_cast<u32x4*>(tq + at) = qr[i];
-      *reinterpret_cast<u32x4*>(tq + TILE + at) = gr[i];
+      store_chunk<T, D, PLANE>(tq, threadIdx.x / CH + i * STEP, threadIdx.x % CH, qr[i]);
+      store_chunk<T, D, PLANE>(tq + TILE, threadIdx.x / CH + i * STEP, threadIdx.x % CH, gr[i]);
     }
     if (threadIdx.x < BR)
       s_lse[buf][threadIdx.x] = r_lse, s_delta[buf][threadIdx.x] = r_delta, s_pos[buf][threadIdx.x] = r_pos;
@@ -262,8 +262,8 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
   load(lo);
   store(0);
   __syncthreads();
-  const int b = wv / KG, own = b * 32 * D * (int)sizeof(T);  // this wavefront's block of 32 rows of a tile
-  const LaneAt<T, D> at_lane(lane);
+  const int b = wv / KG, own = b * 32 * D * 2;  // this wavefront's block of 32 rows of a tile
+  const LaneAt<T, D, PLANE> at_lane(lane);
   auto step = [&](int rt, int buf, auto masked) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(masked)::value;
     const char* tq = lds + buf * 2 * TILE;
@@ -296,8 +296,8 @@ __global__ __launch_bounds__(256, (D * sizeof(T) >= 256 ? 1 : 2)) void attention
         if (key > s_pos[buf][b * 32 + result_row(i, half)]) p[i] = 0.f, ds[i] = 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < NPS; ++i) {
-      const u32x4 pf = pack<T>(p + i * (KS / 2)), df = pack<T>(ds + i * (KS / 2));
+    for (int i = 0; i < 2; ++i) {
+      const Frag<T> pf = pack<T>(p + i * 8), df = pack<T>(ds + i * 8);
 #pragma unroll
       for (int d = 0; d < NDB; ++d) {
         gv[d] = mma<T>(at_lane.frag_t(tg + own, 0, i, d), pf, gv[d]);

@@ -52,7 +52,7 @@ constexpr int kDecodeChunk = 32, kDecodeLeast = 8;  // keys a step; steps a spli
 
 template <typename T, int D, int R>
 __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void attention_decode_kernel(RowsArgs a) {
-  constexpr int E = chunk_elems<T>(), NS = D / (4 * E), VE = D / 16, VB = VE * (int)sizeof(T), VW = VB / 4;
+  constexpr int E = vec_elems<T>(), NS = D / (4 * E), VE = D / 16, VB = VE * (int)sizeof(T), VW = VB / 4;
   constexpr int ROWS = 16 * R;
   __shared__ __align__(16) float s_o[4][ROWS][D + 4];
   __shared__ float s_m[4][ROWS], s_l[4][ROWS];
@@ -227,9 +227,9 @@ __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void atte
         l[r] += p[i];
       }
       if constexpr (sizeof(T) == 2) {
-        const u32x4 pf = pack<T>(p);
+        const Frag<T> pf = pack<T>(p);
 #pragma unroll
-        for (int e = 0; e < VE; ++e) acc[r][e] = mma16<T>(va[e], pf, acc[r][e]);
+        for (int e = 0; e < VE; ++e) acc[r][e] = mma16<T>(va[e], pf.p[0], acc[r][e]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j)

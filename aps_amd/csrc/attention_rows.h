@@ -39,8 +39,9 @@ struct RowsArgs {
   int32_t splits;
 };
 
-template <typename T>
-constexpr int key_tile() { return sizeof(T) == 2 ? 64 : 32; }
+// keys of a tile (f32: three planes; D = 32: a chunk for every thread)
+template <typename T, int D>
+constexpr int key_tile() { return sizeof(T) == 2 || D == 32 ? 64 : 32; }
 constexpr int kRowTile = 128;
 
 // Rows of no sequence (behind the last one; before the first, if cu_seqlens does not begin at 0) are
@@ -53,22 +54,22 @@ __device__ __forceinline__ void clear_rows(T* out, const Index& cu, int64_t N, i
   const int64_t tail = max(tail_of(cu, N, total), (int64_t)lead);
   for (int64_t i = first; i < lead + total - tail; i += step) {
     T* row = out + (i < lead ? i : tail + i - lead) * (int64_t)H * D;
-    for (int i = threadIdx.x; i < H * D / chunk_elems<T>(); i += blockDim.x)
+    for (int i = threadIdx.x; i < H * D / vec_elems<T>(); i += blockDim.x)
       reinterpret_cast<u32x4*>(row)[i] = u32x4{0, 0, 0, 0};
   }
 }
 
 // The next tile of keys (then of values, in the same registers) on its way from global memory to LDS:
 // thread t carries chunk t % CH of rows t / CH + i * (256 / CH).  Rows outside [0, end) are zeros, so nothing
-// that lies there (an unwritten page, the next sequence) can reach a product.  Rows of 256 bytes and more (D = 128):
+// that lies there (an unwritten page, the next sequence) can reach a product.  16-bit rows of D = 128:
 // the keys are in flight during a tile's scores and the values, in the same registers, during its second
 // product, which is what keeps the kernel in 256 registers (a spilled register's reload waits for every load
-// issued before it).  Shorter rows: both are in flight during the whole tile.
+// issued before it).  Otherwise both are in flight during the whole tile.
 template <typename T, int D, bool PAGED>
 struct KvStage {
-  static constexpr int CH = D / chunk_elems<T>(), BK = key_tile<T>(), PER = BK * CH / 256, STEP = 256 / CH;
-  static constexpr bool TURNS = D * sizeof(T) >= 256;  // keys, then values
-  u32x4 r[TURNS ? PER : 2 * PER];
+  static constexpr int CH = D / kChunk, BK = key_tile<T, D>(), PER = BK * CH / 256, STEP = 256 / CH, PLANE = BK * D * 2;
+  static constexpr bool TURNS = sizeof(T) == 2 && D == 128;  // keys, then values
+  Raw<T> r[TURNS ? PER : 2 * PER];
   int slot[PER];  // paged: slots of the tile's rows, looked up a tile ahead of the loads: -1 behind the end, -2
                   // for a page outside the cache
 
@@ -87,44 +88,43 @@ struct KvStage {
   // base: the key head's row 0 (packed: of the sequence); row_stride in elements
   template <int WHICH>  // 0 keys, 1 values
   __device__ __forceinline__ void load(const T* base, int64_t row_stride, int key0, int end) {
-    u32x4* r = this->r + (TURNS ? 0 : WHICH * PER);
+    Raw<T>* r = this->r + (TURNS ? 0 : WHICH * PER);
     const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
     if constexpr (PAGED) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        r[i] = u32x4{0, 0, 0, 0};
-        if (slot[i] >= 0)
-          r[i] = *reinterpret_cast<const u32x4*>(base + slot[i] * row_stride + c * chunk_elems<T>());
+        r[i] = zero_raw<T>();
+        if (slot[i] >= 0) r[i] = load_raw<T>(reinterpret_cast<const char*>(base + slot[i] * row_stride + c * kChunk));
       }
     } else {
       const char* at = reinterpret_cast<const char*>(base + key0 * row_stride);
-      const uint32_t lane_at = (uint32_t)(r0 * (int)row_stride * (int)sizeof(T) + c * 16);
+      const uint32_t lane_at = (uint32_t)(r0 * (int)row_stride * (int)sizeof(T) + c * (kChunk * (int)sizeof(T)));
       const int64_t step = row_stride * (STEP * (int)sizeof(T));
       if (key0 + BK <= end) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) r[i] = load_chunk(at + i * step, lane_at);
+        for (int i = 0; i < PER; ++i) r[i] = load_chunk<T>(at + i * step, lane_at);
       } else {
         rare();
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          r[i] = u32x4{0, 0, 0, 0};
-          if (key0 + r0 + i * STEP < end) r[i] = load_chunk(at + i * step, lane_at);
+          r[i] = zero_raw<T>();
+          if (key0 + r0 + i * STEP < end) r[i] = load_chunk<T>(at + i * step, lane_at);
         }
       }
     }
   }
   template <int WHICH>
   __device__ __forceinline__ void store(char* tile) const {
-    const u32x4* r = this->r + (TURNS ? 0 : WHICH * PER);
+    const Raw<T>* r = this->r + (TURNS ? 0 : WHICH * PER);
     const int c = threadIdx.x % CH, r0 = threadIdx.x / CH;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) *reinterpret_cast<u32x4*>(tile + tile_at<T, D>(r0 + i * STEP, c)) = r[i];
+    for (int i = 0; i < PER; ++i) store_chunk<T, D, PLANE>(tile, r0 + i * STEP, c, r[i]);
   }
-  // Values on their way to a tile that some row sees only in part: 0 * infinity is not 0, so a non-finite
-  // value would reach the rows it is hidden from.  It goes to LDS as 0 and is added to the rows that see it
+  // Values on their way to a tile that some row sees only in part (f32: to any tile, a plane that is 0 times
+  // infinity being NaN): 0 * infinity is not 0, so a non-finite value would reach the rows it is hidden from.  It goes to LDS as 0 and is added to the rows that see it
   // in the end (`add_non_finite`).  True if there was one.
   __device__ __forceinline__ bool sanitize() {
-    u32x4* v = r + (TURNS ? 0 : PER);
+    Raw<T>* v = r + (TURNS ? 0 : PER);
     bool any = false;
 #pragma unroll
     for (int i = 0; i < PER; ++i) v[i] = only_finite<T>(v[i], any);
@@ -164,12 +164,14 @@ __device__ __forceinline__ void add_non_finite(const RowsArgs& a, const T* base,
 
 // wavefronts a SIMD has registers for
 template <typename T, int D>
-constexpr int rows_waves(bool paged) { return D * sizeof(T) >= 512 ? 1 : (D * sizeof(T) >= 256 || paged ? 2 : 3); }
+constexpr int rows_waves(bool paged) {
+  return D * planes<T>() >= 384 ? 1 : (D * planes<T>() >= 128 || paged ? 2 : 3);
+}
 
 template <typename T, int D, bool PAGED>
 __global__ __launch_bounds__(256, (rows_waves<T, D>(PAGED))) void attention_rows_kernel(RowsArgs a) {
-  constexpr int BK = key_tile<T>(), KS = 2 * chunk_elems<T>(), NS = D / KS, NKB = BK / 32, NDB = D / 32;
-  constexpr int NPS = 32 / KS, TILE = BK * D * (int)sizeof(T);
+  constexpr int BK = key_tile<T, D>(), NS = D / 16, NKB = BK / 32, NDB = D / 32, PLANE = BK * D * 2, TILE = planes<T>() * PLANE;
+  constexpr bool ALWAYS = sizeof(T) == 4;  // non-finite values are taken out of every tile
   __shared__ __align__(16) char lds[4 * TILE];
   __shared__ uint8_t s_hidden[2][64];  // paged: keys without a page
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
@@ -207,10 +209,10 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>(PAGED))) void attention_rows
     wave_end = 0;
   }
   const T* qp = static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + head * a.q_h;
-  u32x4 qf[NS];
+  Frag<T> qf[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s)
-    qf[s] = live ? *reinterpret_cast<const u32x4*>(qp + (2 * s + half) * chunk_elems<T>()) : u32x4{0, 0, 0, 0};
+    qf[s] = operand<T>(live ? load_raw<T>(reinterpret_cast<const char*>(qp + (2 * s + half) * kChunk)) : zero_raw<T>());
 
   int tile_lo = 0, tile_hi = (max(end, 0) + BK - 1) / BK;
   if constexpr (PAGED) {
@@ -239,11 +241,11 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>(PAGED))) void attention_rows
     st.mark(s_hidden[0]);
     st.template load<1>(vb, a.v_t, tile_lo * BK, end);
     st.locate(a, t.seq, (tile_lo + 1) * BK, end);
-    if (tile_lo >= clear) bad |= st.sanitize();
+    if (ALWAYS || tile_lo >= clear) bad |= st.sanitize();
     st.template store<1>(lds + TILE);
   }
   __syncthreads();
-  const LaneAt<T, D> at_lane(lane);
+  const LaneAt<T, D, PLANE> at_lane(lane);
   // one tile out of buffer `which`
   auto step = [&](int kt, int buf, auto edge) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(edge)::value;
@@ -253,7 +255,7 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>(PAGED))) void attention_rows
     const bool more = kt + 1 < tile_hi;
     const int k0 = kt * BK;
     const bool sees = !EDGE || k0 < wave_end;
-    u32x4 pf[NKB * NPS];
+    Frag<T> pf[NKB * 2];
     constexpr bool TURNS = KvStage<T, D, PAGED>::TURNS;
     if (more) {
       st.template load<0>(kb, a.k_t, k0 + BK, end);
@@ -316,7 +318,7 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>(PAGED))) void attention_rows
           l += p[i];
         }
 #pragma unroll
-        for (int i = 0; i < NPS; ++i) pf[b * NPS + i] = pack<T>(p + i * (KS / 2));
+        for (int i = 0; i < 2; ++i) pf[b * 2 + i] = pack<T>(p + i * 8);
       }
     }
     if (TURNS && more) {
@@ -329,14 +331,14 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>(PAGED))) void attention_rows
 #pragma unroll
       for (int b = 0; b < NKB; ++b)
 #pragma unroll
-        for (int i = 0; i < NPS; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(at_lane.frag_t(tv, b * 32, i, d), pf[b * NPS + i], acc[d]);
+          for (int d = 0; d < NDB; ++d) acc[d] = mma<T>(at_lane.frag_t(tv, b * 32, i, d), pf[b * 2 + i], acc[d]);
     }
     if (more) {
       if (!TURNS) st.template store<0>(nk);
-      if (EDGE || kt + 1 >= clear) {
-        rare();
+      if (ALWAYS || EDGE || kt + 1 >= clear) {
+        if (!ALWAYS) rare();
         bad |= st.sanitize();
       }
       st.template store<1>(nk + TILE);
@@ -347,9 +349,9 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>(PAGED))) void attention_rows
   for (; kt < clear; ++kt) step(kt, (kt - tile_lo) & 1, std::false_type());
   for (; kt < tile_hi; ++kt) step(kt, (kt - tile_lo) & 1, std::true_type());
   l += __shfl_xor(l, 32, 64);
-  if (clear < tile_hi && __syncthreads_or(bad)) {
+  if ((ALWAYS || clear < tile_hi) && __syncthreads_or(bad)) {
     rare();
-    add_non_finite<T, D, PAGED>(a, vb, t.seq, max(clear, tile_lo) * BK, min(end, tile_hi * BK), pos, half, acc);
+    add_non_finite<T, D, PAGED>(a, vb, t.seq, (ALWAYS ? tile_lo : max(clear, tile_lo)) * BK, min(end, tile_hi * BK), pos, half, acc);
   }
   if (!live) return;
   const int64_t at = (t.start + tok) * Hq + head;

@@ -2,14 +2,19 @@
 // attention_paged.hip): matrix fragments of 16-byte chunks, the swizzled LDS tile they are read from,
 // and the search of a workgroup's tile in a batch of sequences packed end to end.
 //
-// One formulation serves bf16, f16 and f32.  A tile in LDS is row-major with rows of D elements cut
-// into 16-byte chunks (8 or 4 elements); a matrix step contracts over KS = two chunks (16 or 8
-// elements): lanes 0-31 hold the even chunk, lanes 32-63 the odd one.  16-bit types: one 32x32x16
-// MFMA; f32: four 32x32x2 MFMAs, element e of both chunks in the e-th (exact fp32 products).
-// The 32x32 result holds column = lane % 32 and rows (i / 4) * 8 + (lane / 32) * 4 + i % 4 in register
-// i; registers s * KS / 2 .. (s + 1) * KS / 2 - 1 are therefore the B operand of the s-th step of a
-// product that contracts over those rows, provided the A operand takes its contraction index in the
-// same order (`frag_t`): no lane exchange lies between the two products of an attention tile.
+// One formulation serves bf16, f16 and f32.  A tile in LDS is row-major with rows of D 16-bit elements cut
+// into chunks of 8 (16 bytes); a matrix step contracts over two chunks: lanes 0-31 of the 32x32x16 MFMA hold
+// the even one, lanes 32-63 the odd one.  The 32x32 result holds column = lane % 32 and rows
+// (i / 4) * 8 + (lane / 32) * 4 + i % 4 in register i; registers 8 s .. 8 s + 7 are therefore the B operand of
+// the s-th step of a product that contracts over those rows, provided the A operand takes its contraction
+// index in the same order (`LaneAt::frag_t`): no lane exchange lies between the two products of a tile.
+//
+// f32 runs on the same pipe as three bf16 planes, x = h + m + l: h the upper 16 bits (finite for every finite
+// x), m and l what is left, each rounded to bf16, the sum exact to 2^-25 |x|.  Of the nine plane products six
+// are formed, h h + (h m + m h) + (h l + l h + m m), smallest first, in f32; the three left out are below
+// 2^-22 |x y| together, as is usual of an f32 product sum.  Any exponent is kept (no scaling); an infinity
+// makes what it is multiplied into NaN.  Six 16-bit MFMAs of 32 cycles stand for eight f32 ones of 64
+// (32x32x2, 16 deep): %F32%.
 #ifndef APS_AMD_ATTENTION_TILE_H_
 #define APS_AMD_ATTENTION_TILE_H_
 
@@ -35,7 +40,10 @@ constexpr float kLog2e = 1.4426950408889634f;
 enum { kTypeF32 = 0, kTypeBf16 = 1, kTypeF16 = 2 };
 
 template <typename T>
-constexpr int chunk_elems() { return 16 / (int)sizeof(T); }
+constexpr int vec_elems() { return 16 / (int)sizeof(T); }  // elements of 16 bytes in memory
+constexpr int kChunk = 8;                                   // elements of a chunk of a tile
+template <typename T>
+constexpr int planes() { return sizeof(T) == 4 ? 3 : 1; }
 
 template <typename T>
 struct Vec;
@@ -44,41 +52,89 @@ struct Vec<__bf16> { typedef bf16x4 v4; typedef bf16x8 v8; };
 template <>
 struct Vec<_Float16> { typedef f16x4 v4; typedef f16x8 v8; };
 
+// 8 elements as they lie in memory / as matrix operand
 template <typename T>
-__device__ __forceinline__ f32x16 mma(u32x4 a, u32x4 b, f32x16 c);
-template <>
-__device__ __forceinline__ f32x16 mma<__bf16>(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
-                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ f32x16 mma<_Float16>(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
-                                                __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ f32x16 mma<float>(u32x4 a, u32x4 b, f32x16 c) {
-  const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+struct Raw { u32x4 v[sizeof(T) / 2]; };
+template <typename T>
+struct Frag { u32x4 p[planes<T>()]; };
+
+template <typename T>
+__device__ __forceinline__ Raw<T> load_raw(const char* at) {
+  Raw<T> r;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[e], y[e], c, 0, 0, 0);
-  return c;
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = reinterpret_cast<const u32x4*>(at)[i];
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ Raw<T> zero_raw() {
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = u32x4{0, 0, 0, 0};
+  return r;
 }
 
-// registers p[0 .. KS/2) of a result as an operand chunk (one rounding to the 16-bit type: the weights
-// lie in [0, 1] up to a common factor, so the rounding is 2^-9 / 2^-12 of each weight; sums over
-// many keys average it out, and the softmax's own sum is kept from the unrounded values)
+// 8 floats as three planes
+__device__ __forceinline__ Frag<float> split8(const float* x) {
+  bf16x8 m, l;
+  u32x4 h;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = __float_as_uint(x[2 * i]), b = __float_as_uint(x[2 * i + 1]);
+    h[i] = __builtin_amdgcn_perm(b, a, 0x07060302);
+    const float ra = x[2 * i] - __uint_as_float(a & 0xffff0000u), rb = x[2 * i + 1] - __uint_as_float(b & 0xffff0000u);
+    m[2 * i] = (__bf16)ra, m[2 * i + 1] = (__bf16)rb;
+    l[2 * i] = (__bf16)(ra - (float)m[2 * i]), l[2 * i + 1] = (__bf16)(rb - (float)m[2 * i + 1]);
+  }
+  return Frag<float>{{h, __builtin_bit_cast(u32x4, m), __builtin_bit_cast(u32x4, l)}};
+}
+
 template <typename T>
-__device__ __forceinline__ u32x4 pack(const float* p) {
+__device__ __forceinline__ Frag<T> operand(const Raw<T>& r) {
+  if constexpr (sizeof(T) == 2) {
+    return Frag<T>{{r.v[0]}};
+  } else {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r.v[i >> 2][i & 3]);
+    return split8(x);
+  }
+}
+
+__device__ __forceinline__ f32x16 mma_bf16(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <typename T>
+__device__ __forceinline__ f32x16 mma(const Frag<T>& a, const Frag<T>& b, f32x16 c);
+template <>
+__device__ __forceinline__ f32x16 mma<__bf16>(const Frag<__bf16>& a, const Frag<__bf16>& b, f32x16 c) {
+  return mma_bf16(a.p[0], b.p[0], c);
+}
+template <>
+__device__ __forceinline__ f32x16 mma<_Float16>(const Frag<_Float16>& a, const Frag<_Float16>& b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a.p[0]), __builtin_bit_cast(f16x8, b.p[0]), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x16 mma<float>(const Frag<float>& a, const Frag<float>& b, f32x16 c) {
+  c = mma_bf16(a.p[0], b.p[2], c);
+  c = mma_bf16(a.p[2], b.p[0], c);
+  c = mma_bf16(a.p[1], b.p[1], c);
+  c = mma_bf16(a.p[0], b.p[1], c);
+  c = mma_bf16(a.p[1], b.p[0], c);
+  return mma_bf16(a.p[0], b.p[0], c);
+}
+
+// 8 registers of a result as an operand (16-bit types: one rounding -- the weights lie in [0, 1] up to a common
+// factor, so it is 2^-9 / 2^-12 of each weight; sums over many keys average it out, and the softmax's own sum is
+// kept from the unrounded values)
+template <typename T>
+__device__ __forceinline__ Frag<T> pack(const float* p) {
   if constexpr (sizeof(T) == 2) {
     typename Vec<T>::v8 v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = (T)p[e];
-    return __builtin_bit_cast(u32x4, v);
+    return Frag<T>{{__builtin_bit_cast(u32x4, v)}};
   } else {
-    f32x4 v;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = p[e];
-    return __builtin_bit_cast(u32x4, v);
+    return split8(p);
   }
 }
 
@@ -94,45 +150,43 @@ __device__ __forceinline__ void store4(T* p, f32x4 v) {
   }
 }
 
-// sum of the products of two chunks
+// sum of the products of 8 elements
 template <typename T>
-__device__ __forceinline__ float dot_chunk(u32x4 a, u32x4 b) {
+__device__ __forceinline__ float dot_raw(const Raw<T>& a, const Raw<T>& b) {
   float s = 0.f;
   if constexpr (sizeof(T) == 2) {
-    const typename Vec<T>::v8 x = __builtin_bit_cast(typename Vec<T>::v8, a);
-    const typename Vec<T>::v8 y = __builtin_bit_cast(typename Vec<T>::v8, b);
+    const typename Vec<T>::v8 x = __builtin_bit_cast(typename Vec<T>::v8, a.v[0]);
+    const typename Vec<T>::v8 y = __builtin_bit_cast(typename Vec<T>::v8, b.v[0]);
 #pragma unroll
     for (int e = 0; e < 8; ++e) s += (float)x[e] * (float)y[e];
   } else {
-    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s += x[e] * y[e];
+    for (int e = 0; e < 8; ++e) s += __uint_as_float(a.v[e >> 2][e & 3]) * __uint_as_float(b.v[e >> 2][e & 3]);
   }
   return s;
 }
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.4028234663852886e38f; }
 
-// element e of a chunk / the chunk with its non-finite elements zeroed (`any` set if there were some)
+// 8 elements with the non-finite ones zeroed (`any` set if there were some)
 template <typename T>
-__device__ __forceinline__ float chunk_at(u32x4 v, int e) {
-  if constexpr (sizeof(T) == 2) return (float)__builtin_bit_cast(typename Vec<T>::v8, v)[e];
-  else return __builtin_bit_cast(f32x4, v)[e];
-}
-template <typename T>
-__device__ __forceinline__ u32x4 only_finite(u32x4 v, bool& any) {
+__device__ __forceinline__ Raw<T> only_finite(Raw<T> r, bool& any) {
   // an exponent of ones: infinity or NaN
   constexpr uint32_t one = sizeof(T) == 4 ? 0x7f800000u : (__is_same(T, __bf16) ? 0x7f80u : 0x7c00u);
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if constexpr (sizeof(T) == 4) {
-      if ((v[w] & one) == one) v[w] = 0, any = true;
-    } else {
-      if ((v[w] & one) == one) v[w] &= 0xffff0000u, any = true;
-      if ((v[w] & (one << 16)) == one << 16) v[w] &= 0xffffu, any = true;
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      uint32_t v = r.v[i][w];
+      if constexpr (sizeof(T) == 4) {
+        if ((v & one) == one) v = 0, any = true;
+      } else {
+        if ((v & one) == one) v &= 0xffff0000u, any = true;
+        if ((v & (one << 16)) == one << 16) v &= 0xffffu, any = true;
+      }
+      r.v[i][w] = v;
     }
-  }
-  return v;
+  return r;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -140,74 +194,72 @@ __device__ __forceinline__ float log2_fast(float x) { return __builtin_amdgcn_lo
 
 // Chunk c of row r lies at chunk position c ^ swizzle(r).  The masks make both reads of a tile touch
 // every LDS bank once: 16 lanes reading one chunk of 16 rows (row fragments), and 16 lanes reading 32
-// bytes of 4 rows for the transposing read (16-bit) / rows r and r + 4 of one 128-byte run (f32).
-template <typename T, int D>
+// bytes of 4 rows (transposing read).
+template <int D>
 __device__ __forceinline__ int swizzle(int r) {
-  constexpr int CH = D / chunk_elems<T>();
-  if constexpr (sizeof(T) == 2) {
-    if constexpr (CH >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
-    if constexpr (CH == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
-    return (r >> 2) & 3;
-  } else {
-    if constexpr (CH >= 16) return (r & 3) | (((r >> 2) & 1) << 3) | (((r >> 3) & 1) << 2);
-    return (r >> 1) & 7;
-  }
+  if constexpr (D >= 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  if constexpr (D == 64) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  return (r >> 2) & 3;
 }
 
 // byte offset of chunk c of row r
-template <typename T, int D>
+template <int D>
 __device__ __forceinline__ int tile_at(int r, int c) {
-  return r * (D * (int)sizeof(T)) + ((c ^ swizzle<T, D>(r)) << 4);
+  return r * (D * 2) + ((c ^ swizzle<D>(r)) << 4);
 }
 
-// Where a lane's fragments lie, from a tile's first byte.  The swizzle depends on a row's last four bits, so
-// 32 rows (16 for the 16-bit transposing read) further on is a constant to the instruction's offset, and so
-// is the other buffer: the loops below run over both buffers in turn, unrolled, and add nothing per read.
-//   row fragment, step s:         row lane % 32, chunk 2 s + lane / 32
-//   transposed fragment (16-bit): ds_read_b64_tr_b16: within 16 lanes, lane j points at 4 elements of row
-//                                 j / 4 and receives column j of the 4 x 16 block
-template <typename T, int D>
+// Where a lane's fragments lie, from a tile's first byte (planes PLANE bytes apart).  The swizzle depends on a
+// row's last four bits, so 32 rows (16 for the transposing read) further on is a constant to the instruction's
+// offset, and so is another plane.
+//   row fragment, step s: row lane % 32, chunk 2 s + lane / 32
+//   transposed fragment:  ds_read_b64_tr_b16: within 16 lanes, lane j points at 4 elements of row j / 4 and
+//                         receives column j of the 4 x 16 block
+template <typename T, int D, int PLANE>
 struct LaneAt {
-  static constexpr int NS = D / (2 * chunk_elems<T>()), NDB = D / 32, PITCH = D * (int)sizeof(T);
-  int f[NS], t[sizeof(T) == 2 ? NDB : 1][2], lane;
+  static constexpr int NS = D / 16, NDB = D / 32, PITCH = D * 2;
+  int f[NS], t[NDB][2];
 
-  __device__ __forceinline__ explicit LaneAt(int l) : lane(l) {
+  __device__ __forceinline__ explicit LaneAt(int l) {
     const int half = l >> 5;
 #pragma unroll
-    for (int s = 0; s < NS; ++s) f[s] = tile_at<T, D>(l & 31, 2 * s + half);
-    if constexpr (sizeof(T) == 2) {
+    for (int s = 0; s < NS; ++s) f[s] = tile_at<D>(l & 31, 2 * s + half);
 #pragma unroll
-      for (int db = 0; db < NDB; ++db)
+    for (int db = 0; db < NDB; ++db)
 #pragma unroll
-        for (int hi = 0; hi < 2; ++hi)
-          t[db][hi] = tile_at<T, D>(half * 4 + ((l & 15) >> 2) + hi * 8, db * 4 + ((l >> 4) & 1) * 2 + ((l & 3) >> 1)) +
-                      (l & 1) * 8;
-    }
+      for (int hi = 0; hi < 2; ++hi)
+        t[db][hi] = tile_at<D>(half * 4 + ((l & 15) >> 2) + hi * 8, db * 4 + ((l >> 4) & 1) * 2 + ((l & 3) >> 1)) +
+                    (l & 1) * 8;
   }
   // rows row0 .. row0 + 31 (a multiple of 32)
-  __device__ __forceinline__ u32x4 frag(const char* tile, int row0, int s) const {
-    return *reinterpret_cast<const u32x4*>(tile + row0 * PITCH + f[s]);
-  }
-  // column db * 32 + lane % 32 of the KS rows that registers s * KS / 2 .. of a 32x32 result stand for
-  __device__ __forceinline__ u32x4 frag_t(const char* tile, int row0, int s, int db) const {
-    if constexpr (sizeof(T) == 2) {
-      typedef __attribute__((address_space(3))) s16x4* lds_ptr;
-      const char* p = tile + (row0 + s * 16) * PITCH;
-      const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + t[db][0])));
-      const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(p + t[db][1])));
-      return u32x4{a.x, a.y, b.x, b.y};
-    } else {
-      const int d = db * 32 + (lane & 31);
-      u32x4 v;
+  __device__ __forceinline__ Frag<T> frag(const char* tile, int row0, int s) const {
+    Frag<T> r;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int r = row0 + s * 8 + (lane >> 5) * 4 + e;
-        v[e] = *reinterpret_cast<const uint32_t*>(tile + tile_at<T, D>(r, d >> 2) + (d & 3) * 4);
-      }
-      return v;
+    for (int p = 0; p < planes<T>(); ++p)
+      r.p[p] = *reinterpret_cast<const u32x4*>(tile + p * PLANE + row0 * PITCH + f[s]);
+    return r;
+  }
+  // column db * 32 + lane % 32 of the 16 rows that registers 8 s .. 8 s + 7 of a 32x32 result stand for
+  __device__ __forceinline__ Frag<T> frag_t(const char* tile, int row0, int s, int db) const {
+    typedef __attribute__((address_space(3))) s16x4* lds_ptr;
+    Frag<T> r;
+#pragma unroll
+    for (int p = 0; p < planes<T>(); ++p) {
+      const char* at = tile + p * PLANE + (row0 + s * 16) * PITCH;
+      const u32x2 a = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + t[db][0])));
+      const u32x2 b = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(at + t[db][1])));
+      r.p[p] = u32x4{a.x, a.y, b.x, b.y};
     }
+    return r;
   }
 };
+
+// 8 elements to a tile
+template <typename T, int D, int PLANE>
+__device__ __forceinline__ void store_chunk(char* tile, int row, int c, const Raw<T>& r) {
+  const Frag<T> f = operand<T>(r);
+#pragma unroll
+  for (int p = 0; p < planes<T>(); ++p) *reinterpret_cast<u32x4*>(tile + p * PLANE + tile_at<D>(row, c)) = f.p[p];
+}
 
 // In a branch that is seldom taken: keeps the compiler from turning it into selects that every tile pays for
 __device__ __forceinline__ void rare() { asm volatile(""); }
@@ -216,9 +268,8 @@ __device__ __forceinline__ void rare() { asm volatile(""); }
 // from scalar registers, and a loop that steps the base adds nothing per lane.  (Strides are at most
 // kMaxStride bytes, so 128 rows stay within the 32-bit offset.)
 constexpr int64_t kMaxStride = 1 << 23;
-__device__ __forceinline__ u32x4 load_chunk(const char* base, uint32_t offset) {
-  return *reinterpret_cast<const u32x4*>(base + offset);
-}
+template <typename T>
+__device__ __forceinline__ Raw<T> load_chunk(const char* base, uint32_t offset) { return load_raw<T>(base + offset); }
 
 // row of a 32x32 result that register i of a lane holds
 __device__ __forceinline__ int result_row(int i, int half) { return (i >> 2) * 8 + half * 4 + (i & 3); }
