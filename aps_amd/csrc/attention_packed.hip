@@ -169,6 +169,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attention_keys_backward_kernel(GradArgs a) {
   constexpr int BR = grad_rows<T, D>(), RG = BR / 32, KG = 4 / RG, CH = D / kChunk, NS = D / 16, NDB = D / 32;
   constexpr int PLANE = BR * D * 2, TILE = planes<T>() * PLANE, PER = BR * CH / 256, STEP = 256 / CH;
+  constexpr bool AHEAD = D * planes<T>() >= 128 && D * planes<T>() < 384;
   __shared__ __align__(16) char lds[4 * TILE];
   __shared__ __align__(16) float s_lse[2][BR], s_delta[2][BR];
   __shared__ __align__(16) int s_pos[2][BR];
@@ -272,23 +273,29 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
     if (more) load(rt + 1);
     // (every wavefront multiplies every block, masked ones too: a branch around the products makes the
     // compiler move the 128 accumulators between the register files in every iteration)
-    f32x16 s = f32x16{0}, g = f32x16{0};
+    // One wavefront a SIMD (AHEAD): nothing hides an LDS read but distance, so the fragments of the first products
+    // are all requested before them, and those of the second ones' first half before the weights are formed.
+    Frag<T> qa[NS], ga[NS], qt[NDB], gt[NDB];
+    f32x4 lse[4], dl[4];
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-      s = mma<T>(at_lane.frag(tq + own, 0, i), kf[i], s);
-      g = mma<T>(at_lane.frag(tg + own, 0, i), vf[i], g);
-    }
-    float p[16], ds[16];
+    for (int i = 0; i < NS; ++i) qa[i] = at_lane.frag(tq + own, 0, i), ga[i] = at_lane.frag(tg + own, 0, i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const f32x4 lse = *reinterpret_cast<const f32x4*>(&s_lse[buf][b * 32 + j * 8 + half * 4]);
-      const f32x4 dl = *reinterpret_cast<const f32x4*>(&s_delta[buf][b * 32 + j * 8 + half * 4]);
+      lse[j] = *reinterpret_cast<const f32x4*>(&s_lse[buf][b * 32 + j * 8 + half * 4]);
+      dl[j] = *reinterpret_cast<const f32x4*>(&s_delta[buf][b * 32 + j * 8 + half * 4]);
+    }
+    if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+    f32x16 s = f32x16{0}, g = f32x16{0};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int i = j * 4 + e;
-        p[i] = exp2_fast(fmaf(s[i], a.c, -lse[e]));
-        ds[i] = p[i] * (g[i] - dl[e]);
-      }
+    for (int i = 0; i < NS; ++i) s = mma<T>(qa[i], kf[i], s), g = mma<T>(ga[i], vf[i], g);
+#pragma unroll
+    for (int d = 0; d < NDB; ++d) gt[d] = at_lane.frag_t(tg + own, 0, 0, d), qt[d] = at_lane.frag_t(tq + own, 0, 0, d);
+    if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+    float p[16], ds[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      p[i] = exp2_fast(fmaf(s[i], a.c, -lse[i >> 2][i & 3]));
+      ds[i] = p[i] * (g[i] - dl[i >> 2][i & 3]);
     }
     if (EDGE) {
 #pragma unroll
@@ -300,8 +307,8 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
       const Frag<T> pf = pack<T>(p + i * 8), df = pack<T>(ds + i * 8);
 #pragma unroll
       for (int d = 0; d < NDB; ++d) {
-        gv[d] = mma<T>(at_lane.frag_t(tg + own, 0, i, d), pf, gv[d]);
-        gk[d] = mma<T>(at_lane.frag_t(tq + own, 0, i, d), df, gk[d]);
+        gv[d] = mma<T>(i ? at_lane.frag_t(tg + own, 0, i, d) : gt[d], pf, gv[d]);
+        gk[d] = mma<T>(i ? at_lane.frag_t(tq + own, 0, i, d) : qt[d], df, gk[d]);
       }
     }
     if (more) store(buf ^ 1);
