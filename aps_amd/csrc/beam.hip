@@ -23,12 +23,11 @@ constexpr int kThreads = 256;
 constexpr int kMaxBeam = 64, kCandidates = 1024, kHeld = 4;
 constexpr float kLargest = 3.4028234663852886e38f;
 
-// e^x for x <= 0 in 64 bits, relative error < 1e-11: 2^f, |f| <= 1/2, by its series to f^9
-__device__ __forceinline__ double exp64(double x) {
-  const double y = x * 1.4426950408889634074;
+// 2^y for y <= 0 in 64 bits, relative error < 1e-9: 2^f, |f| <= 1/2, by its series to f^8; 0 for -infinity
+__device__ __forceinline__ double exp2_64(double y) {
+  y = fmax(y, -1100.);
   const double n = rint(y), f = y - n;
-  double p = 1.0178086009239697e-7;
-  p = fma(p, f, 1.3215486790144307e-6);
+  double p = 1.3215486790144307e-6;
   p = fma(p, f, 1.5252733804059839e-5);
   p = fma(p, f, 1.5403530393381608e-4);
   p = fma(p, f, 1.3333558146428443e-3);
@@ -37,8 +36,9 @@ __device__ __forceinline__ double exp64(double x) {
   p = fma(p, f, 2.4022650695910071e-1);
   p = fma(p, f, 6.9314718055994531e-1);
   p = fma(p, f, 1.0);
-  return ldexp(p, n < -2000. ? -2000 : (int)n);
+  return ldexp(p, (int)n);
 }
+constexpr double kLog2e64 = 1.4426950408889634074;
 
 // order-preserving integers: larger value, larger integer
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -112,8 +112,12 @@ __device__ __forceinline__ void widen(u32x4 raw, float* to) {
   }
 }
 
-// NaN counts as ruled out, +inf as the largest finite value, -0 as 0 (they tie)
-__device__ __forceinline__ float tame(float x) { return x != x ? -INFINITY : fminf(x, kLargest) + 0.f; }
+// NaN counts as ruled out, +inf as the largest finite value
+__device__ __forceinline__ float tame(float x) { return x != x ? -INFINITY : fminf(x, kLargest); }
+// (-0 and 0 tie)
+__device__ __forceinline__ uint64_t key_of(float x, int token) {
+  return ((uint64_t)ordered(x + 0.f) << 32) | (uint32_t)~token;
+}
 
 // A workgroup takes 256 PER elements of a row: 32 a thread where there are rows enough to fill the chip,
 // 8 (a shorter chain of dependent work) where there are not.
@@ -183,31 +187,20 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
   const uint32_t bound = max(max(s_kth[0], s_kth[1]), max(s_kth[2], s_kth[3]));
   // (ruled-out tokens are not collected: if they are needed at all, it is the lowest few)
   const float least = bound <= ordered(-kLargest) ? -kLargest : from_ordered(bound);
-  int mine = 0;
+  uint32_t hits = 0;
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < VE; ++i) mine += x[j * VE + i] >= least;
-  int at = place(mine, lane, &s_count);
-  if (mine) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const int e = first + j * kThreads * VE + i;
-        if (x[j * VE + i] >= least) {
-          if (at < kCandidates) s_cand[at] = ((uint64_t)ordered(x[j * VE + i]) << 32) | (uint32_t)~e;
-          ++at;
-        }
-      }
+  for (int i = 0; i < PER; ++i) hits |= x[i] >= least ? 1u << i : 0u;
+  int at = place(__popc(hits), lane, &s_count);
+  for (; hits; hits &= hits - 1) {  // few: read again rather than picked out of the registers
+    const int i = __ffs(hits) - 1, e = first + i / VE * (kThreads * VE) + i % VE;
+    if (at < kCandidates) s_cand[at] = key_of(tame((float)base[e]), e);
+    ++at;
   }
   double sum = 0.;
   if (top > -INFINITY) {
+    const double ref = -(double)top * kLog2e64;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const double e = exp64((double)x[i] - (double)top);
-      sum += x[i] > -INFINITY ? e : 0.;
-    }
+    for (int i = 0; i < PER; ++i) sum += exp2_64(fma((double)x[i], kLog2e64, ref));
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -251,7 +244,7 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
       for (int i = 0; i < VE; ++i) {
         const int e = first + j * kThreads * VE + i;
         if (!(x[j * VE + i] > -INFINITY)) continue;  // (there are more than K others)
-        const uint64_t key = ((uint64_t)ordered(x[j * VE + i]) << 32) | (uint32_t)~e;
+        const uint64_t key = key_of(x[j * VE + i], e);
         if (key < last && key > mx) mx = key;
       }
 #pragma unroll
@@ -303,7 +296,7 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
     if (top > -INFINITY)
       for (int s = 0; s < S; ++s)
         if (a.top[row * S + s] > -INFINITY)
-          sum += a.sum[row * S + s] * exp64((double)a.top[row * S + s] - (double)top);
+          sum += a.sum[row * S + s] * exp2_64(((double)a.top[row * S + s] - (double)top) * kLog2e64);
     s_add[tid] = top > -INFINITY ? (double)top + log(sum) : 0.;
     s_score[tid] = (double)tame(a.score[row]);
   }
