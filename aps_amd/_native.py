@@ -270,15 +270,16 @@ except AttributeError:
 
 
 def stream_of(t: th.Tensor):
-    return C.c_void_p(_raw_stream(t.device.index))
+    return C.c_void_p(_raw_stream(t.get_device()))
 
 
 _HERE = contextlib.nullcontext()
+_current_device = getattr(th._C, "_cuda_getDevice", th.cuda.current_device)
 
 
 def on_device_of(t: th.Tensor):
     """context in which the device of `t` is the current one (launches go to the current device)"""
-    return _HERE if t.get_device() == th.cuda.current_device() else th.cuda.device(t.device)
+    return _HERE if t.get_device() == _current_device() else th.cuda.device(t.device)
 
 
 def needs_grad(*tensors) -> bool:

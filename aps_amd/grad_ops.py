@@ -632,28 +632,35 @@ class AttentionPackedFn(th.autograd.Function):
         return out
 
     @staticmethod
-    @th.autograd.function.once_differentiable
     def backward(ctx, g):
-        from aps_amd import nn_ops
-        q, k, v, out, sums, cu_seqlens = ctx.saved_tensors
-        causal, scale = ctx.cfg
-        lib = nat.load()
-        T, Hq, D = q.shape
-        Hkv = k.shape[1]
-        g = nn_ops._strided16(g)
-        g_q = th.empty(q.shape, device=q.device, dtype=q.dtype)
-        g_k, g_v = (th.empty(k.shape, device=q.device, dtype=q.dtype) for _ in range(2))
-        if T:
-            ws = th.empty(lib.aps_attention_packed_backward_workspace(T, Hq), device=q.device, dtype=th.uint8)
-            with nat.on_device_of(q):
-                rc = lib.aps_attention_packed_backward(
-                    q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(), sums.data_ptr(),
-                    cu_seqlens.data_ptr(), int(cu_seqlens.dtype == th.int64), g_q.data_ptr(), g_k.data_ptr(),
-                    g_v.data_ptr(), T, cu_seqlens.shape[0] - 1, Hq, Hkv, D, q.stride(0), q.stride(1), k.stride(0),
-                    k.stride(1), v.stride(0), v.stride(1), g.stride(0), g.stride(1), nn_ops.ELEMENT_TYPES[q.dtype],
-                    int(causal), scale, ws.data_ptr(), nat.stream_of(q))
-            nat.check(rc, "aps_attention_packed_backward")
-        return g_q, g_k, g_v, None, None, None
+        if th.is_grad_enabled():  # create_graph: the gradients refuse to be differentiated again
+            return _attention_packed_backward_once(ctx, g)
+        return _attention_packed_backward(ctx, g)
+
+
+def _attention_packed_backward(ctx, g):
+    from aps_amd import nn_ops
+    q, k, v, out, sums, cu_seqlens = ctx.saved_tensors
+    causal, scale = ctx.cfg
+    T, Hq, D = q.shape
+    g = nn_ops._strided16(g)
+    g_q = th.empty_like(out)  # (contiguous, whatever q is)
+    g_k = th.empty_like(k, memory_format=th.contiguous_format)
+    g_v = th.empty_like(v, memory_format=th.contiguous_format)
+    if T:
+        ws = th.empty_like(sums)  # aps_attention_packed_backward_workspace bytes
+        with nat.on_device_of(q):
+            rc = nat.load().aps_attention_packed_backward(
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(), sums.data_ptr(),
+                cu_seqlens.data_ptr(), int(cu_seqlens.dtype == th.int64), g_q.data_ptr(), g_k.data_ptr(),
+                g_v.data_ptr(), T, cu_seqlens.shape[0] - 1, Hq, k.shape[1], D, q.stride(0), q.stride(1), k.stride(0),
+                k.stride(1), v.stride(0), v.stride(1), g.stride(0), g.stride(1), nn_ops.ELEMENT_TYPES[q.dtype],
+                int(causal), scale, ws.data_ptr(), nat.stream_of(q))
+        nat.check(rc, "aps_attention_packed_backward")
+    return g_q, g_k, g_v, None, None, None
+
+
+_attention_packed_backward_once = th.autograd.function.once_differentiable(_attention_packed_backward)
 
 
 class EmbeddingPosencFn(th.autograd.Function):

@@ -805,22 +805,23 @@ def beam_reorder(states: Sequence[th.Tensor], parent: th.Tensor, dims: Optional[
     N, K = parent.shape
     B, src, dst, outer, inner = 0, [], [], [], []
     for t, d in zip(states, dims):
-        if not -t.dim() <= d < t.dim():
-            raise RuntimeError(f"{what}: a state {tuple(t.shape)} has no axis {d}")
-        d %= t.dim()
-        rows = t.shape[d]
+        shape = t.shape
+        if not -len(shape) <= d < len(shape):
+            raise RuntimeError(f"{what}: a state {tuple(shape)} has no axis {d}")
+        rows = shape[d]
         if rows < N or rows % N or (B and rows != N * B):
-            raise RuntimeError(f"{what}: axis {d} of {tuple(t.shape)} is not {N} x {B or 'hypotheses'}")
+            raise RuntimeError(f"{what}: axis {d} of {tuple(shape)} is not {N} x {B or 'hypotheses'}")
         B = rows // N
         t = t.contiguous()
-        shape = t.shape
         src.append(t)
         if B == K:
             dst.append(th.empty_like(t))
         else:
-            dst.append(th.empty(*shape[:d], N * K, *shape[d + 1:], device=t.device, dtype=t.dtype))
-        outer.append(math.prod(shape[:d]))
-        inner.append(math.prod(shape[d + 1:]) * t.element_size())
+            d %= len(shape)
+            dst.append(t.new_empty(*shape[:d], N * K, *shape[d + 1:]))
+        ahead = math.prod(shape[:d]) if d else 1
+        outer.append(ahead)
+        inner.append(t.numel() // (ahead * rows) * t.element_size() if ahead else 0)
     parent = parent.contiguous()
     n = len(src)
     # the call's four host arrays, one behind the other

@@ -515,3 +515,27 @@ def test_gradients_against_differences():
             slope = (f(1) - f(-1)) / (2 * h)
             exact = (grads[i].double() * step.double()).sum().item()
             assert abs(slope - exact) < 2e-3 * (grads[i].double().norm() * step.double().norm()).item()
+
+
+@gpu
+def test_gradients_of_gradients_are_refused():
+    from aps_amd import nn_ops
+    x = [randn(7, 2, 32, seed=i).requires_grad_() for i in range(3)]
+    out = nn_ops.attention_packed(*x, cu_of([4, 3]))
+    (gq,) = torch.autograd.grad(out.square().sum(), x[:1], create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(gq.sum(), x[1])
+
+
+@gpu
+def test_gradients_of_permuted_inputs():
+    """heads-major leaves seen as rows x heads: dense, but not in the order the kernels write"""
+    from aps_amd import nn_ops
+    lens = [11, 30]
+    x = [randn(h, 41, 64, seed=i).requires_grad_() for i, h in enumerate((4, 2, 2))]
+    q, k, v = (t.transpose(0, 1) for t in x)
+    g = randn(4, 41, 64, seed=5).transpose(0, 1)
+    grads = torch.autograd.grad(nn_ops.attention_packed(q, k, v, cu_of(lens)), x, g)
+    vals, bounds = ref.packed(q, k, v, lens, True, g=g)
+    for got, want, bound in zip(grads, vals[1:], bounds[1:]):
+        ref.check(got.transpose(0, 1), want, bound)
