@@ -164,12 +164,10 @@ __device__ __forceinline__ void add_non_finite(const RowsArgs& a, const T* base,
 
 // wavefronts a SIMD has registers for
 template <typename T, int D>
-constexpr int rows_waves(bool paged) {
-  return D * planes<T>() >= 384 ? 1 : (D * planes<T>() >= 128 || paged ? 2 : 3);
-}
+constexpr int rows_waves() { return D * planes<T>() >= 384 ? 1 : (D * planes<T>() >= 96 ? 2 : 3); }
 
 template <typename T, int D, bool PAGED>
-__global__ __launch_bounds__(256, (rows_waves<T, D>(PAGED))) void attention_rows_kernel(RowsArgs a) {
+__global__ __launch_bounds__(256, (rows_waves<T, D>())) void attention_rows_kernel(RowsArgs a) {
   constexpr int BK = key_tile<T, D>(), NS = D / 16, NKB = BK / 32, NDB = D / 32, PLANE = BK * D * 2, TILE = planes<T>() * PLANE;
   constexpr bool ALWAYS = sizeof(T) == 4;  // non-finite values are taken out of every tile
   __shared__ __align__(16) char lds[4 * TILE];
@@ -283,11 +281,14 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>(PAGED))) void attention_rows
       if constexpr (PAGED) {
         const uint64_t hidden = __ballot(lane < BK && s_hidden[buf][lane]);
         if (hidden) {
-  #pragma unroll
-          for (int b = 0; b < NKB; ++b)
+          rare();
+#pragma unroll
+          for (int b = 0; b < NKB; ++b) {
+            const uint32_t mine = (uint32_t)(hidden >> (b * 32)) >> (half * 4);
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              if ((hidden >> (b * 32 + result_row(i, half))) & 1) s[b][i] = -INFINITY;
+              if ((mine >> ((i >> 2) * 8 + (i & 3))) & 1) s[b][i] = -INFINITY;
+          }
         }
       }
       float top = -INFINITY;
