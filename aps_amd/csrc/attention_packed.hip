@@ -25,7 +25,8 @@ struct GradArgs {
 };
 
 // dq: the forward kernel's walk, with V as the left operand of dP^T = V dO^T beside S^T = K Q^T and K
-// read transposed for dq^T = K^T dS^T
+// read transposed for dq^T = K^T dS^T.  (The 12 sequences named at the next kernel: 122 us, 540 TFLOP/s; the 3:
+// 195 us, 760.)
 template <typename T, int D>
 __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attention_rows_backward_kernel(GradArgs a) {
   constexpr int BK = key_tile<T, D>(), NS = D / 16, NKB = BK / 32, NDB = D / 32, PLANE = BK * D * 2, TILE = planes<T>() * PLANE;
@@ -158,8 +159,11 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attenti
 // dv^T = dO^T P and dk^T = Q^T dS as they stand.  Two of the four wavefronts share 32 keys and take
 // alternate blocks of 32 rows, their sums meeting in LDS at the end: a tile of 64 keys, because the first
 // keys of a causal sequence are seen by every row of the group and the longest tile is what the launch
-// waits for (128-key tiles: %K128%; 64: %K64% on 12 sequences of 64 - 2 048 tokens, 16 / 4 heads of 128, bf16).  f32 with
-// D = 128 has no registers for the larger row tile: four times 32 keys there.
+// waits for (12 sequences of 195 - 2 048 tokens, 16 heads over 4 of 128, bf16: 439 us with tiles of 128, 373 with
+// 64 when it was changed).  f32 with D = 128 has no registers for the larger row tile: four times 32 keys there.
+// That case takes 247 us now, 360 TFLOP/s: 604 tiles on 256 CUs whose longest walks 128 row tiles of 1.9 us, one
+// wavefront a SIMD (376 registers), LDS and the waits for it half of each; 3 sequences of 3 582 - 4 500, 16 heads of
+// 64, f16, two wavefronts a SIMD: 290 us, 680 TFLOP/s.
 template <typename T, int D>
 constexpr int grad_rows() { return D * planes<T>() >= 384 ? 32 : 64; }
 template <typename T, int D>

@@ -13,8 +13,9 @@
 // x), m and l what is left, each rounded to bf16, the sum exact to 2^-25 |x|.  Of the nine plane products six
 // are formed, h h + (h m + m h) + (h l + l h + m m), smallest first, in f32; the three left out are below
 // 2^-22 |x y| together, as is usual of an f32 product sum.  Any exponent is kept (no scaling); an infinity
-// makes what it is multiplied into NaN.  Six 16-bit MFMAs of 32 cycles stand for eight f32 ones of 64
-// (32x32x2, 16 deep): %F32%.
+// makes what it is multiplied into NaN.  Six 16-bit MFMAs of 32 cycles stand for eight f32 ones of 64 (32x32x2,
+// 16 deep): 8 sequences of 1 400 - 1 500 tokens, 8 heads of 64, causal, forward and gradients 775 us; with
+// the f32 instructions 1 160 (head size 128: 1 640 against 2 566).
 #ifndef APS_AMD_ATTENTION_TILE_H_
 #define APS_AMD_ATTENTION_TILE_H_
 
@@ -288,7 +289,7 @@ struct SeqTile {
   int tile;       // tile within the sequence
   int64_t start;  // first token of the sequence
   int len;        // its tokens
-  int used;       // seq == -1: tiles there are in all
+  int64_t used;   // seq == -1: tiles there are in all
 };
 
 // tokens [start, end) of sequence n, whatever the array holds: inside [0, total), never negative (token
@@ -304,7 +305,7 @@ __device__ __forceinline__ void seq_range(const Index& cu, int64_t n, int64_t to
 // same answer.
 __device__ __forceinline__ SeqTile find_tile(const Index& cu, int64_t N, int64_t total, int per, int rows,
                                              int want, int lane) {
-  int base = 0;
+  int64_t base = 0;  // (64 bits: sequences that overlap, which they must not, count more tiles than there are)
   for (int64_t n0 = 0; n0 < N; n0 += 64) {
     int s = 0, e = 0;
     if (n0 + lane < N) seq_range(cu, n0 + lane, total, s, e);
@@ -320,7 +321,7 @@ __device__ __forceinline__ SeqTile find_tile(const Index& cu, int64_t N, int64_t
       const int at = __builtin_ctzll(beyond);
       SeqTile t;
       t.seq = (int)n0 + at;
-      t.tile = want - base - __builtin_amdgcn_readlane(upto - tiles, at);
+      t.tile = (int)(want - base) - __builtin_amdgcn_readlane(upto - tiles, at);
       t.len = __builtin_amdgcn_readlane(len, at);
       t.start = __builtin_amdgcn_readlane(s, at);
       t.used = 0;

@@ -539,3 +539,80 @@ def test_gradients_of_permuted_inputs():
     vals, bounds = ref.packed(q, k, v, lens, True, g=g)
     for got, want, bound in zip(grads, vals[1:], bounds[1:]):
         ref.check(got.transpose(0, 1), want, bound)
+
+
+@gpu
+def test_captured_training_step_replays():
+    """forward and gradients captured together; replays on other inputs equal the eager pass bit for bit"""
+    from aps_amd import nn_ops
+    lens = [100, 37, 1, 64]
+    x = [randn(sum(lens), h, 64, dtype=torch.bfloat16, seed=i).requires_grad_() for i, h in enumerate((6, 2, 2))]
+    g = randn(sum(lens), 6, 64, dtype=torch.bfloat16, seed=9)
+    cu = cu_of(lens)
+
+    def step():
+        out = nn_ops.attention_packed(*x, cu)
+        return [out.detach(), *torch.autograd.grad(out, x, g)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        with torch.no_grad():
+            for j, t in enumerate((*x, g)):
+                t.copy_(randn(*t.shape, dtype=t.dtype, seed=100 * i + j))
+        graph.replay()
+        torch.cuda.synchronize()
+        first = [t.clone() for t in held]
+        again = step()
+        assert all(torch.equal(a, b) for a, b in zip(first, again)), i
+
+
+@gpu
+@pytest.mark.parametrize("group", [3, 5, 7, 65, 130])
+def test_gradients_of_odd_groups(group):
+    """groups that leave rows of a tile empty, and groups of more heads than a tile has rows"""
+    from aps_amd import nn_ops
+    lens = [33, 0, 70]
+    x = [randn(103, h, 32, dtype=torch.bfloat16, seed=i).requires_grad_() for i, h in enumerate((group, 1, 1))]
+    g = randn(103, group, 32, dtype=torch.bfloat16, seed=4)
+    for causal in (True, False):
+        out = nn_ops.attention_packed(*x, cu_of(lens), causal=causal)
+        grads = torch.autograd.grad(out, x, g)
+        vals, bounds = ref.packed(*x, lens, causal, g=g)
+        for name, got, want, bound in zip(("out", "gq", "gk", "gv"), (out,) + grads, vals, bounds):
+            ref.check(got, want, bound, f"{name} causal={causal}")
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_many_sequences(kind):
+    """more sequences than a wavefront scans at once, most of them short or empty"""
+    from aps_amd import nn_ops
+    lens = [(i * 7) % 5 for i in range(200)] + [90]
+    q, k, v = (randn(sum(lens), 2, 64, dtype=TYPES[kind], seed=i) for i in range(3))
+    (want,), (bound,) = ref.packed(q, k, v, lens, True)
+    with torch.no_grad():
+        ref.check(nn_ops.attention_packed(q, k, v, cu_of(lens, torch.int64)), want, bound)
+        table = torch.arange(201 * 12, dtype=torch.int32, device=DEV).view(201, 12)
+        cache = [torch.zeros(201 * 12, 8, 2, 64, dtype=TYPES[kind], device=DEV) for _ in range(2)]
+        args = (*cache, table, cu_of(lens), torch.tensor(lens, device=DEV))
+        nn_ops.paged_append(k, v, *args)
+        ref.check(nn_ops.attention_paged(q, *args), want, bound)
+
+
+@gpu
+def test_large_scores_and_scale():
+    """scores in the thousands and a scale of one's own: no overflow, the weights of the largest keys"""
+    from aps_amd import nn_ops
+    lens = [150]
+    q, k, v = (randn(150, 2, 64, seed=i, std=s) for i, s in enumerate((30.0, 30.0, 1.0)))
+    for scale in (1.0, 1e-4, 0.3):
+        (want,), (bound,) = ref.packed(q, k, v, lens, True, scale=scale)
+        with torch.no_grad():
+            ref.check(nn_ops.attention_packed(q, k, v, cu_of(lens), scale=scale), want, bound, f"scale {scale}")
