@@ -161,9 +161,9 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attenti
 // keys of a causal sequence are seen by every row of the group and the longest tile is what the launch
 // waits for (12 sequences of 195 - 2 048 tokens, 16 heads over 4 of 128, bf16: 439 us with tiles of 128, 373 with
 // 64 when it was changed).  f32 with D = 128 has no registers for the larger row tile: four times 32 keys there.
-// That case takes 247 us now, 360 TFLOP/s: 604 tiles on 256 CUs whose longest walks 128 row tiles of 1.9 us, one
-// wavefront a SIMD (376 registers), LDS and the waits for it half of each; 3 sequences of 3 582 - 4 500, 16 heads of
-// 64, f16, two wavefronts a SIMD: 290 us, 680 TFLOP/s.
+// That case takes 217 us now, 410 TFLOP/s: 604 tiles on 256 CUs whose longest walks 128 row tiles of 1.7 us, one
+// wavefront a SIMD, LDS and the waits for it half of each; 3 sequences of 3 582 - 4 500, 16 heads of
+// 64, f16, two wavefronts a SIMD: 266 us, 740 TFLOP/s.
 template <typename T, int D>
 constexpr int grad_rows() { return D * planes<T>() >= 384 ? 32 : 64; }
 template <typename T, int D>
@@ -173,7 +173,7 @@ template <typename T, int D>
 __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attention_keys_backward_kernel(GradArgs a) {
   constexpr int BR = grad_rows<T, D>(), RG = BR / 32, KG = 4 / RG, CH = D / kChunk, NS = D / 16, NDB = D / 32;
   constexpr int PLANE = BR * D * 2, TILE = planes<T>() * PLANE, PER = BR * CH / 256, STEP = 256 / CH;
-  constexpr bool AHEAD = D * planes<T>() >= 128 && D * planes<T>() < 384;
+  constexpr bool TIGHT = D * planes<T>() >= 384, AHEAD = D * planes<T>() >= 128 && !TIGHT;
   __shared__ __align__(16) char lds[4 * TILE];
   __shared__ __align__(16) float s_lse[2][BR], s_delta[2][BR];
   __shared__ __align__(16) int s_pos[2][BR];
@@ -216,35 +216,57 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
     tok = j / span, head = j - tok * span;
     if (tok >= toks) tok = 1 << 30;  // an empty row
   };
+  auto at_of = [&](int tok, int head, int64_t s_t, int64_t s_h) {
+    return (uint32_t)((tok * (int)s_t + head * (int)s_h) * (int)sizeof(T) + threadIdx.x % CH * (kChunk * (int)sizeof(T)));
+  };
   uint32_t q_at[PER], g_at[PER];
   int tok_i[PER], head_i[PER], tok_s, head_s;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     place(threadIdx.x / CH + i * STEP, tok_i[i], head_i[i]);
-    const int tk = min(tok_i[i], BR);
-    q_at[i] = (uint32_t)((tk * (int)a.q_t + head_i[i] * (int)a.q_h) * (int)sizeof(T) + threadIdx.x % CH * (kChunk * (int)sizeof(T)));
-    g_at[i] = (uint32_t)((tk * (int)a.go_t + head_i[i] * (int)a.go_h) * (int)sizeof(T) + threadIdx.x % CH * (kChunk * (int)sizeof(T)));
+    q_at[i] = at_of(min(tok_i[i], BR), head_i[i], a.q_t, a.q_h);
+    g_at[i] = at_of(min(tok_i[i], BR), head_i[i], a.go_t, a.go_h);
   }
   place(threadIdx.x & (BR - 1), tok_s, head_s);
   const char* qb = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + t.start * a.q_t + (int64_t)h * a.G * a.q_h);
   const char* gb = reinterpret_cast<const char*>(static_cast<const T*>(a.go) + t.start * a.go_t + (int64_t)h * a.G * a.go_h);
   Raw<T> qr[PER], gr[PER];
-  float r_lse = INFINITY, r_delta = 0.f;
-  int r_pos = -1;
+  float r_lse, r_delta;
+  int r_pos;
   auto load = [&](int rt) {
     const int tok0 = segs == 1 ? rt * toks : rt / segs, head0 = segs == 1 ? 0 : (rt - tok0 * segs) * BR;
     const char* q0 = qb + (tok0 * a.q_t + head0 * a.q_h) * (int)sizeof(T);
     const char* g0 = gb + (tok0 * a.go_t + head0 * a.go_h) * (int)sizeof(T);
-    if (toks * span == BR && tok0 + toks <= t.len && head0 + span <= a.G) {
+    const bool whole = toks * span == BR && tok0 + toks <= t.len && head0 + span <= a.G;
+    if constexpr (TIGHT) {  // (320 registers hold operands and sums: none for a second set of offsets)
+      if (whole) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i) qr[i] = load_chunk<T>(q0, q_at[i]), gr[i] = load_chunk<T>(g0, g_at[i]);
-    } else {
-      rare();
+        for (int i = 0; i < PER; ++i) qr[i] = load_chunk<T>(q0, q_at[i]), gr[i] = load_chunk<T>(g0, g_at[i]);
+      } else {
+        rare();
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        qr[i] = gr[i] = zero_raw<T>();
-        if (tok_i[i] < t.len - tok0 && head0 + head_i[i] < a.G) qr[i] = load_chunk<T>(q0, q_at[i]), gr[i] = load_chunk<T>(g0, g_at[i]);
+        for (int i = 0; i < PER; ++i) {
+          qr[i] = gr[i] = zero_raw<T>();
+          if (tok_i[i] < t.len - tok0 && head0 + head_i[i] < a.G) qr[i] = load_chunk<T>(q0, q_at[i]), gr[i] = load_chunk<T>(g0, g_at[i]);
+        }
       }
+    } else {
+      // An empty row reads the last token's, which every key's sum holds already, and gets the weight 0 by lse = inf:
+      // only offsets lie behind the branch.  (With loads on both of its ways, those met in a wait for all but the
+      // last pair: 253 us against 217 on the 12 sequences.)
+      uint32_t qo[PER], go[PER];
+#pragma unroll
+      for (int i = 0; i < PER; ++i) qo[i] = q_at[i], go[i] = g_at[i];
+      if (!whole) {
+        rare();
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const int tok = min(tok_i[i], t.len - 1 - tok0), head = min(head_i[i], a.G - 1 - head0);
+          qo[i] = at_of(tok, head, a.q_t, a.q_h), go[i] = at_of(tok, head, a.go_t, a.go_h);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < PER; ++i) qr[i] = load_chunk<T>(q0, qo[i]), gr[i] = load_chunk<T>(g0, go[i]);
     }
     if (threadIdx.x < BR) {
       r_lse = INFINITY, r_delta = 0.f, r_pos = -1;
