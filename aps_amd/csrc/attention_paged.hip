@@ -103,18 +103,15 @@ __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void atte
     for (int e = 0; e < VE; ++e) acc[r][e] = f32x4{0};
   }
   const int32_t* table = a.table + (int64_t)t.seq * a.table_stride;
-  // slot of key (lane % 32) of a chunk; -1 past the end or for a page outside the cache
-  auto slot_of = [&](int chunk) {
-    const int key = chunk * kDecodeChunk + (lane & 31);
-    if (key >= end) return -1;
-    const int32_t p = table[key >> a.page_shift];
-    if (p < 0 || p >= a.num_pages) return -1;
-    return (p << a.page_shift) + (key & ((1 << a.page_shift) - 1));  // (the cache has < 2^31 slots)
-  };
-  int next = lo + wv < hi ? slot_of(lo + wv) : -1;
+  // The table's entry for key (lane % 32) of a chunk is asked for a chunk ahead and not looked at before its turn (memory
+  // answers in order: before this chunk's loads are asked for, or it would wait for them too)
+  auto page_of = [&](int chunk) { return table[min(chunk * kDecodeChunk + (lane & 31), end - 1) >> a.page_shift]; };
+  int32_t next = lo + wv < hi ? page_of(lo + wv) : -1;
   for (int ch = lo + wv; ch < hi; ch += 4) {
-    const int slot = next;
-    if (ch + 4 < hi) next = slot_of(ch + 4);
+    // slot of key (lane % 32); -1 past the end or for a page outside the cache (which has < 2^31 slots)
+    const int key = ch * kDecodeChunk + (lane & 31);
+    const int slot = key >= end || next < 0 || next >= a.num_pages ? -1 : (next << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+    next = page_of(ch + 4);
     u32x4 kf[2][NS];
 #pragma unroll
     for (int b = 0; b < 2; ++b) {

@@ -66,8 +66,8 @@ __device__ __forceinline__ void clear_rows(T* out, const Index& cu, int64_t N, i
 }
 
 // The next tile of keys (then of values, in the same registers) on its way from global memory to LDS:
-// thread t carries chunk t % CH of rows t / CH + i * (256 / CH).  Rows outside [0, end) are zeros, so nothing
-// that lies there (an unwritten page, the next sequence) can reach a product.  16-bit rows of D = 128:
+// thread t carries chunk t % CH of rows t / CH + i * (256 / CH).  Paged rows outside [0, end) are zeros, packed ones
+// the last key's, so nothing that lies there (an unwritten page, the next sequence) can reach a product.  16-bit rows of D = 128:
 // the keys are in flight during a tile's scores and the values, in the same registers, during its second
 // product, which is what keeps the kernel in 256 registers (a spilled register's reload waits for every load
 // issued before it).  Otherwise both are in flight during the whole tile.
@@ -76,18 +76,25 @@ struct KvStage {
   static constexpr int CH = D / kChunk, BK = key_tile<T, D>(), PER = BK * CH / 256, STEP = 256 / CH, PLANE = BK * D * 2;
   static constexpr bool TURNS = sizeof(T) == 2 && D == 128;  // keys, then values
   Raw<T> r[TURNS ? PER : 2 * PER];
-  int slot[PER];  // paged: slots of the tile's rows, looked up a tile ahead of the loads: -1 behind the end, -2
-                  // for a page outside the cache
+  int32_t page[PER];  // paged: the table's entries for the rows of the tile behind the next one
+  int slot[PER];      // paged: slots of the next tile's rows: -1 behind the end, -2 for a page outside the cache
 
+  // The table is read a tile ahead of `resolve`, before the loads of the tile in between: memory answers in order, so
+  // a look at an entry that was asked for behind them would wait for them all.
   __device__ __forceinline__ void locate(const RowsArgs& a, int seq, int key0, int end) {
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        page[i] = a.table[(int64_t)seq * a.table_stride + (min(key0 + (int)threadIdx.x / CH + i * STEP, end - 1) >> a.page_shift)];
+    }
+  }
+  __device__ __forceinline__ void resolve(const RowsArgs& a, int key0, int end) {
     if constexpr (PAGED) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int key = key0 + (int)threadIdx.x / CH + i * STEP;
-        slot[i] = -1;
-        if (key >= end) continue;
-        const int32_t p = a.table[(int64_t)seq * a.table_stride + (key >> a.page_shift)];
-        slot[i] = p < 0 || p >= a.num_pages ? -2 : (p << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+        slot[i] = page[i] < 0 || page[i] >= a.num_pages ? -2 : (page[i] << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+        if (key >= end) slot[i] = -1;
       }
     }
   }
@@ -103,20 +110,23 @@ struct KvStage {
         if (slot[i] >= 0) r[i] = load_raw<T>(reinterpret_cast<const char*>(base + slot[i] * row_stride + c * kChunk));
       }
     } else {
+      // (rows behind the end read the last one: only offsets lie behind the branch, since two ways with loads on both
+      // meet in a wait for them)
       const char* at = reinterpret_cast<const char*>(base + key0 * row_stride);
-      const uint32_t lane_at = (uint32_t)(r0 * (int)row_stride * (int)sizeof(T) + c * (kChunk * (int)sizeof(T)));
-      const int64_t step = row_stride * (STEP * (int)sizeof(T));
-      if (key0 + BK <= end) {
+      const uint32_t chunk_at = c * (kChunk * (int)sizeof(T));
+      const int last = end - 1 - key0;
+      uint32_t lane_at[PER];
 #pragma unroll
-        for (int i = 0; i < PER; ++i) r[i] = load_chunk<T>(at + i * step, lane_at);
-      } else {
+      for (int i = 0; i < PER; ++i) lane_at[i] = (uint32_t)(r0 * (int)row_stride * (int)sizeof(T)) + chunk_at;
+      if (last < BK - 1) {
         rare();
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          r[i] = zero_raw<T>();
-          if (key0 + r0 + i * STEP < end) r[i] = load_chunk<T>(at + i * step, lane_at);
-        }
+        for (int i = 0; i < PER; ++i)
+          lane_at[i] = (uint32_t)(min(r0, max(last - i * STEP, 0)) * (int)row_stride * (int)sizeof(T)) + chunk_at;
       }
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        r[i] = load_chunk<T>(at + min(i * STEP, last) * (row_stride * (int)sizeof(T)), lane_at[i]);
     }
   }
   template <int WHICH>
@@ -240,14 +250,16 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>())) void attention_rows_kern
   const int clear = min(tile_hi, (block_min + 1) / BK);
   if (tile_lo < tile_hi) {
     st.locate(a, t.seq, tile_lo * BK, end);
+    st.resolve(a, tile_lo * BK, end);
+    st.locate(a, t.seq, (tile_lo + 1) * BK, end);
     st.template load<0>(kb, a.k_t, tile_lo * BK, end);
     st.template store<0>(lds);
     st.mark(s_hidden[0]);
     st.template load<1>(vb, a.v_t, tile_lo * BK, end);
-    st.locate(a, t.seq, (tile_lo + 1) * BK, end);
     if (ALWAYS || tile_lo >= clear) bad |= st.sanitize();
     st.template store<1>(lds + TILE);
   }
+  loads_done();
   __syncthreads();
   const LaneAt<T, D, PLANE> at_lane(lane);
   // one tile out of buffer `which`
@@ -262,11 +274,12 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>())) void attention_rows_kern
     Frag<T> pf[NKB * 2];
     constexpr bool TURNS = KvStage<T, D, PAGED>::TURNS;
     if (more) {
+      st.resolve(a, k0 + BK, end);
+      st.locate(a, t.seq, k0 + 2 * BK, end);
       st.template load<0>(kb, a.k_t, k0 + BK, end);
       if (!TURNS) {
         st.template load<1>(vb, a.v_t, k0 + BK, end);
         st.mark(s_hidden[buf ^ 1]);
-        st.locate(a, t.seq, k0 + 2 * BK, end);
       }
     }
     if (sees) {
@@ -332,7 +345,6 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>())) void attention_rows_kern
       st.template store<0>(nk);
       st.mark(s_hidden[buf ^ 1]);
       st.template load<1>(vb, a.v_t, k0 + BK, end);
-      st.locate(a, t.seq, k0 + 2 * BK, end);
     }
     if (sees) {
 #pragma unroll

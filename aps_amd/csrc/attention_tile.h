@@ -262,6 +262,10 @@ __device__ __forceinline__ void store_chunk(char* tile, int row, int c, const Ra
   for (int p = 0; p < planes<T>(); ++p) *reinterpret_cast<u32x4*>(tile + p * PLANE + tile_at<D>(row, c)) = f.p[p];
 }
 
+// Wait for every global load.  Said before a loop where its operands have arrived anyway on the way that is
+// taken: the compiler, which sees another way, else waits in the loop, for the loop's own loads too.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 // In a branch that is seldom taken: keeps the compiler from turning it into selects that every tile pays for
 __device__ __forceinline__ void rare() { asm volatile(""); }
 
