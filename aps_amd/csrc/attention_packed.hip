@@ -79,8 +79,9 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attenti
   const T* vb = static_cast<const T*>(a.v) + h * a.v_h + t.start * a.v_t;
   KvStage<T, D, false> st;
   st.template load<0>(kb, a.k_t, 0, end);
+  if (!st.TURNS) st.template load<1>(vb, a.v_t, 0, end);
   st.template store<0>(lds);
-  st.template load<1>(vb, a.v_t, 0, end);
+  if (st.TURNS) st.template load<1>(vb, a.v_t, 0, end);
   st.template store<1>(lds + TILE);
   __syncthreads();
   const LaneAt<T, D, PLANE> at_lane(lane);

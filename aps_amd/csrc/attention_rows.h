@@ -253,9 +253,10 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>())) void attention_rows_kern
     st.resolve(a, tile_lo * BK, end);
     st.locate(a, t.seq, (tile_lo + 1) * BK, end);
     st.template load<0>(kb, a.k_t, tile_lo * BK, end);
+    if (!st.TURNS) st.template load<1>(vb, a.v_t, tile_lo * BK, end);
     st.template store<0>(lds);
     st.mark(s_hidden[0]);
-    st.template load<1>(vb, a.v_t, tile_lo * BK, end);
+    if (st.TURNS) st.template load<1>(vb, a.v_t, tile_lo * BK, end);
     if (ALWAYS || tile_lo >= clear) bad |= st.sanitize();
     st.template store<1>(lds + TILE);
   }
