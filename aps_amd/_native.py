@@ -203,9 +203,9 @@ SIGNATURES = {
                                               _I64, _F, _P]),
     "aps_mvdr_covariance_backward": (C.c_int, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64,
                                                _I64, _I64, _I32, _P, _P]),
-    "aps_attention_packed": (C.c_int, [_P, _P, _P, _P, _I32, _P, _P] + [_I64] * 11 + [_I32, _I32, _F, _P]),
+    "aps_attention_packed": (C.c_int, [_P, _P, _P, _P, _I32, _P, _P, _P] + [_I64] * 11 + [_I32, _I32, _F, _P]),
     "aps_attention_packed_backward_workspace": (_I64, [_I64, _I64]),
-    "aps_attention_packed_backward": (C.c_int, [_P] * 7 + [_I32, _P, _P, _P] + [_I64] * 13 +
+    "aps_attention_packed_backward": (C.c_int, [_P] * 8 + [_I32, _P, _P, _P] + [_I64] * 13 +
                                       [_I32, _I32, _F, _P, _P]),
     "aps_paged_append": (C.c_int, [_P] * 6 + [_I32, _P, _I32] + [_I64] * 12 + [_I32, _P]),
     "aps_attention_paged_workspace": (_I64, [_I64] * 7 + [_I32]),

@@ -1,6 +1,9 @@
 // Attention over sequences packed end to end, and its gradients:
 //   P_rj = exp(scale q_r . k_j - lse_r),  o_r = sum_j P_rj v_j                    (attention_rows.h)
-//   D_r  = do_r . o_r
+//   D_r  = do_r . o_r        (16-bit: of o and of what its rounding took away, which the forward pass keeps for it.
+//          D_r enters every dS_rj, and sequences of 64 tokens would lose more by o's rounding than by that of
+//          dS: dq off by 3.0e-3 instead of 2.3e-3 in bf16, where rounding the result alone is 1.7e-3.  Writing
+//          and reading it takes 7 + 5 us of 418 on the 12 sequences named below.)
 //   dS_rj = P_rj (do_r . v_j - D_r) scale
 //   dq_r = sum_j dS_rj k_j,   dk_j = sum_r dS_rj q_r,   dv_j = sum_r P_rj do_r
 // with r over the rows (token, head of the group) that see key j: the sums over a group's heads are part
@@ -13,7 +16,7 @@ namespace aps {
 namespace att {
 
 struct GradArgs {
-  const void *q, *k, *v, *o, *go;
+  const void *q, *k, *v, *o, *rest, *go;  // rest (16-bit): what the rounding of o took away
   const float* lse;    // [total, Hq]
   float* delta;        // [total, Hq]
   void *gq, *gk, *gv;  // [total, Hq | Hkv, D]
@@ -25,8 +28,8 @@ struct GradArgs {
 };
 
 // dq: the forward kernel's walk, with V as the left operand of dP^T = V dO^T beside S^T = K Q^T and K
-// read transposed for dq^T = K^T dS^T.  (The 12 sequences named at the next kernel: 122 us, 540 TFLOP/s; the 3:
-// 195 us, 760.)
+// read transposed for dq^T = K^T dS^T.  (The 12 sequences named at the next kernel: 112 us, 590 TFLOP/s; the 3:
+// 200 us, 740.)
 template <typename T, int D>
 __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attention_rows_backward_kernel(GradArgs a) {
   constexpr int BK = key_tile<T, D>(), NS = D / 16, NKB = BK / 32, NDB = D / 32, PLANE = BK * D * 2, TILE = planes<T>() * PLANE;
@@ -54,21 +57,30 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attenti
   const T* qp = static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + head * a.q_h;
   const T* gp = static_cast<const T*>(a.go) + (t.start + tok) * a.go_t + head * a.go_h;
   const T* op = static_cast<const T*>(a.o) + at * D;
+  // (a row behind the last one computes with the sequence's first token, into a column that is not stored: loads
+  // without a branch, so that all of them are under way together)
   Frag<T> qf[NS], gf[NS];
   float delta = 0.f;
+  Raw<T> g[NS], o[NS];
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
-    Raw<T> x = zero_raw<T>(), g = zero_raw<T>();
-    if (live) {
-      const int c = (2 * s + half) * kChunk;
-      x = load_raw<T>(reinterpret_cast<const char*>(qp + c));
-      g = load_raw<T>(reinterpret_cast<const char*>(gp + c));
-      delta += dot_raw<T>(g, load_raw<T>(reinterpret_cast<const char*>(op + c)));
-    }
-    qf[s] = operand<T>(x), gf[s] = operand<T>(g);
+    const int c = (2 * s + half) * kChunk;
+    qf[s] = operand<T>(load_raw<T>(reinterpret_cast<const char*>(qp + c)));
+    g[s] = load_raw<T>(reinterpret_cast<const char*>(gp + c));
+    o[s] = load_raw<T>(reinterpret_cast<const char*>(op + c));
   }
+  if constexpr (sizeof(T) == 2) {
+    const T* rp = static_cast<const T*>(a.rest) + at * D;
+    Raw<T> r[NS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s) r[s] = load_raw<T>(reinterpret_cast<const char*>(rp + (2 * s + half) * kChunk));
+#pragma unroll
+    for (int s = 0; s < NS; ++s) delta += dot_raw<T>(g[s], r[s]);
+  }
+#pragma unroll
+  for (int s = 0; s < NS; ++s) delta += dot_raw<T>(g[s], o[s]), gf[s] = operand<T>(g[s]);
   delta += __shfl_xor(delta, 32, 64);
-  const float lse = live ? a.lse[at] : INFINITY;
+  const float lse = a.lse[at];
   if (live && half == 0) a.delta[at] = delta;
 
   f32x16 acc[NDB];
@@ -403,17 +415,17 @@ using namespace aps;
 using namespace aps::att;
 
 extern "C" int aps_attention_packed(const void* q, const void* k, const void* v, const void* cu_seqlens,
-                                    int32_t cu_wide, void* out, float* lse, int64_t total, int64_t N,
+                                    int32_t cu_wide, void* out, void* out_rest, float* lse, int64_t total, int64_t N,
                                     int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t q_t, int64_t q_h,
                                     int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h, int32_t dtype,
                                     int32_t causal, float scale, void* stream) {
   if (total == 0) return APS_OK;
   APS_CHECK_ARG(q && k && v && cu_seqlens && out && sizes_fit(total, N, Hq, Hkv) && scale > 0.f);
   const int64_t e = dtype == kTypeF32 ? 4 : 8;
-  APS_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out));
+  APS_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_rest));
   APS_CHECK_ARG(strides_fit(q_t, q_h, e) && strides_fit(k_t, k_h, e) && strides_fit(v_t, v_h, e));
   RowsArgs a{};
-  a.q = q, a.k = k, a.v = v, a.out = out, a.lse = lse;
+  a.q = q, a.k = k, a.v = v, a.out = out, a.rest = dtype == kTypeF32 ? nullptr : out_rest, a.lse = lse;
   a.cu = Index{cu_seqlens, cu_wide};
   a.total = total, a.N = N;
   a.G = (int32_t)(Hq / Hkv), a.Hkv = (int32_t)Hkv;
@@ -432,7 +444,7 @@ extern "C" int64_t aps_attention_packed_backward_workspace(int64_t total, int64_
 }
 
 extern "C" int aps_attention_packed_backward(const void* q, const void* k, const void* v, const void* out,
-                                             const void* g_out, const float* lse, const void* cu_seqlens,
+                                             const void* out_rest, const void* g_out, const float* lse, const void* cu_seqlens,
                                              int32_t cu_wide, void* g_q, void* g_k, void* g_v, int64_t total,
                                              int64_t N, int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t q_t,
                                              int64_t q_h, int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h,
@@ -440,14 +452,15 @@ extern "C" int aps_attention_packed_backward(const void* q, const void* k, const
                                              float scale, void* workspace, void* stream) {
   if (total == 0) return APS_OK;
   APS_CHECK_ARG(q && k && v && out && g_out && lse && cu_seqlens && g_q && g_k && g_v && workspace);
+  APS_CHECK_ARG(dtype == kTypeF32 || out_rest);
   APS_CHECK_ARG(sizes_fit(total, N, Hq, Hkv) && scale > 0.f);
   const int64_t e = dtype == kTypeF32 ? 4 : 8;
-  APS_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(g_out));
+  APS_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_rest) && aligned16(g_out));
   APS_CHECK_ARG(aligned16(g_q) && aligned16(g_k) && aligned16(g_v));
   APS_CHECK_ARG(strides_fit(q_t, q_h, e) && strides_fit(k_t, k_h, e) && strides_fit(v_t, v_h, e));
   APS_CHECK_ARG(strides_fit(go_t, go_h, e));
   GradArgs a{};
-  a.q = q, a.k = k, a.v = v, a.o = out, a.go = g_out, a.lse = lse, a.delta = static_cast<float*>(workspace);
+  a.q = q, a.k = k, a.v = v, a.o = out, a.rest = out_rest, a.go = g_out, a.lse = lse, a.delta = static_cast<float*>(workspace);
   a.gq = g_q, a.gk = g_k, a.gv = g_v;
   a.cu = Index{cu_seqlens, cu_wide};
   a.total = total, a.N = N;

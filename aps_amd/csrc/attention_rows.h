@@ -27,6 +27,7 @@ namespace att {
 struct RowsArgs {
   const void *q, *k, *v;  // packed: k, v [total, Hkv, D] by strides; paged: pages [P, page, Hkv, D]
   void* out;              // [total, Hq, D]
+  void* rest;             // packed, 16-bit: what the rounding of `out` took away, [total, Hq, D]; or null
   float* lse;             // [total, Hq] log2 of the softmax sum, +inf for a row that sees nothing; or null
   Index cu;               // [N + 1]
   Index kv_lens;          // paged: [N] keys of each sequence, its new tokens included
@@ -223,10 +224,10 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>())) void attention_rows_kern
     wave_end = 0;
   }
   const T* qp = static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + head * a.q_h;
-  Frag<T> qf[NS];
+  Frag<T> qf[NS];  // (a row behind the last one: the sequence's first token, into a column that is not stored)
 #pragma unroll
   for (int s = 0; s < NS; ++s)
-    qf[s] = operand<T>(live ? load_raw<T>(reinterpret_cast<const char*>(qp + (2 * s + half) * kChunk)) : zero_raw<T>());
+    qf[s] = operand<T>(load_raw<T>(reinterpret_cast<const char*>(qp + (2 * s + half) * kChunk)));
 
   int tile_lo = 0, tile_hi = (max(end, 0) + BK - 1) / BK;
   if constexpr (PAGED) {
@@ -390,12 +391,20 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>())) void attention_rows_kern
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
   T* po = static_cast<T*>(a.out) + at * D;
+  T* pr = a.rest ? static_cast<T*>(a.rest) + at * D : nullptr;
 #pragma unroll
   for (int d = 0; d < NDB; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; i += 4)
-      store4<T>(po + d * 32 + result_row(i, half),
-                f32x4{acc[d][i] * inv, acc[d][i + 1] * inv, acc[d][i + 2] * inv, acc[d][i + 3] * inv});
+    for (int i = 0; i < 16; i += 4) {
+      const f32x4 x = f32x4{acc[d][i] * inv, acc[d][i + 1] * inv, acc[d][i + 2] * inv, acc[d][i + 3] * inv};
+      store4<T>(po + d * 32 + result_row(i, half), x);
+      if (sizeof(T) == 2 && !PAGED && pr) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = x[e] - (float)(T)x[e];
+        store4<T>(pr + d * 32 + result_row(i, half), y);
+      }
+    }
   if (a.lse && half == 0) a.lse[at] = l > 0.f ? m + log2_fast(l) : (l != l ? l : INFINITY);
 }
 

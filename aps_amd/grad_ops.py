@@ -626,8 +626,8 @@ class AttentionPackedFn(th.autograd.Function):
     def forward(ctx, q, k, v, cu_seqlens, causal, scale):
         from aps_amd import nn_ops
         q, k, v = (nn_ops._strided16(t.detach()) for t in (q, k, v))
-        out, sums = nn_ops.attention_packed_forward(q, k, v, cu_seqlens, causal, scale, lse=True)
-        ctx.save_for_backward(q, k, v, out, sums, cu_seqlens)
+        out, sums, rest = nn_ops.attention_packed_forward(q, k, v, cu_seqlens, causal, scale, train=True)
+        ctx.save_for_backward(q, k, v, out, rest, sums, cu_seqlens)
         ctx.cfg = (causal, scale)
         return out
 
@@ -640,7 +640,7 @@ class AttentionPackedFn(th.autograd.Function):
 
 def _attention_packed_backward(ctx, g):
     from aps_amd import nn_ops
-    q, k, v, out, sums, cu_seqlens = ctx.saved_tensors
+    q, k, v, out, rest, sums, cu_seqlens = ctx.saved_tensors
     causal, scale = ctx.cfg
     T, Hq, D = q.shape
     g = nn_ops._strided16(g)
@@ -651,7 +651,7 @@ def _attention_packed_backward(ctx, g):
         ws = th.empty_like(sums)  # aps_attention_packed_backward_workspace bytes
         with nat.on_device_of(q):
             rc = nat.load().aps_attention_packed_backward(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(), sums.data_ptr(),
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if rest is None else rest.data_ptr(), g.data_ptr(), sums.data_ptr(),
                 cu_seqlens.data_ptr(), int(cu_seqlens.dtype == th.int64), g_q.data_ptr(), g_k.data_ptr(),
                 g_v.data_ptr(), T, cu_seqlens.shape[0] - 1, Hq, k.shape[1], D, q.stride(0), q.stride(1), k.stride(0),
                 k.stride(1), v.stride(0), v.stride(1), g.stride(0), g.stride(1), nn_ops.ELEMENT_TYPES[q.dtype],

@@ -608,24 +608,27 @@ def attention_packed(q: th.Tensor, k: th.Tensor, v: th.Tensor, cu_seqlens: th.Te
     return attention_packed_forward(q, k, v, cu_seqlens, bool(causal), scale)[0]
 
 
-def attention_packed_forward(q, k, v, cu_seqlens, causal: bool, scale: float, lse: bool = False):
-    """the launch behind `attention_packed` -> (context, log2 of the softmax sums T x Hq | None)"""
+def attention_packed_forward(q, k, v, cu_seqlens, causal: bool, scale: float, train: bool = False):
+    """the launch behind `attention_packed` -> (context, and with train what the backward pass needs: log2 of the
+    softmax sums T x Hq, and in 16 bits what the context's rounding took away | None)"""
     nat.require_device(q, k, v, cu_seqlens)
     lib = nat.load()
     T, Hq, D = q.shape
     q, k, v = _strided16(q), _strided16(k), _strided16(v)
     out = th.empty(T, Hq, D, device=q.device, dtype=q.dtype)
-    sums = th.empty(T, Hq, device=q.device, dtype=th.float32) if lse else None
+    sums = th.empty(T, Hq, device=q.device, dtype=th.float32) if train else None
+    rest = th.empty_like(out) if train and q.dtype != th.float32 else None
     if T:
         with nat.on_device_of(q):
             rc = lib.aps_attention_packed(q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(),
                                           int(cu_seqlens.dtype == th.int64), out.data_ptr(),
+                                          None if rest is None else rest.data_ptr(),
                                           None if sums is None else sums.data_ptr(), T, cu_seqlens.shape[0] - 1,
                                           Hq, k.shape[1], D, q.stride(0), q.stride(1), k.stride(0), k.stride(1),
                                           v.stride(0), v.stride(1), ELEMENT_TYPES[q.dtype], int(causal), scale,
                                           nat.stream_of(q))
         nat.check(rc, "aps_attention_packed")
-    return out, sums
+    return out, sums, rest
 
 
 def _check_cache(what: str, rows: int, k_pages: th.Tensor, v_pages: th.Tensor, page_table: th.Tensor,

@@ -1060,18 +1060,20 @@ int aps_conformer_stack(float* x, const int64_t* lens, const ApsMegaLayer* layer
 
 /* out[r, h] = sum_j softmax_j(scale q[r, h] . k[j, h']) v[j, h'] over the keys of r's own sequence, those
  * up to r if `causal`; q [total, Hq, dh], k / v [total, Hkv, dh] -> out [total, Hq, dh] contiguous.
- * lse (or NULL) [total, Hq]: log2 of the softmax's sum, what the backward pass needs. */
+ * What the backward pass needs: lse (or NULL) [total, Hq], log2 of the softmax's sum; out_rest (or NULL; f32: not
+ * touched) like out, what the rounding of out took away. */
 int aps_attention_packed(const void* q, const void* k, const void* v, const void* cu_seqlens, int32_t cu_wide,
-                         void* out, float* lse, int64_t total, int64_t N, int64_t Hq, int64_t Hkv,
+                         void* out, void* out_rest, float* lse, int64_t total, int64_t N, int64_t Hq, int64_t Hkv,
                          int64_t head_dim, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t v_t,
                          int64_t v_h, int32_t dtype, int32_t causal, float scale, void* stream);
 /* its adjoint: g_out [total, Hq, dh] by strides -> g_q [total, Hq, dh], g_k / g_v [total, Hkv, dh]
- * contiguous, the same bits on every run (no atomics).  out, lse: of the forward call.
+ * contiguous, the same bits on every run (no atomics).  out, lse, out_rest (f32: NULL): of the forward call.  A
+ * non-finite value of a sequence may reach all gradients of that sequence (0 * infinity is NaN), none of another.
  * workspace: aps_attention_packed_backward_workspace bytes. */
 int64_t aps_attention_packed_backward_workspace(int64_t total, int64_t Hq);
 int aps_attention_packed_backward(const void* q, const void* k, const void* v, const void* out,
-                                  const void* g_out, const float* lse, const void* cu_seqlens,
-                                  int32_t cu_wide, void* g_q, void* g_k, void* g_v, int64_t total, int64_t N,
+                                  const void* out_rest, const void* g_out, const float* lse,
+                                  const void* cu_seqlens, int32_t cu_wide, void* g_q, void* g_k, void* g_v, int64_t total, int64_t N,
                                   int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t q_t, int64_t q_h,
                                   int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h, int64_t go_t,
                                   int64_t go_h, int32_t dtype, int32_t causal, float scale, void* workspace,

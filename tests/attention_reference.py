@@ -67,7 +67,9 @@ def gradients(q, k, v, g, causal, scale, dtype):
     gp = g @ v.T
     e_gp = (d + 2) * U * (g.abs() @ v.abs().T)
     delta = (g * out).sum(-1, keepdim=True)
-    e_delta = (g.abs() * e_out).sum(-1, keepdim=True) + (d + 2) * U * (g * out).abs().sum(-1, keepdim=True)
+    # (delta is formed from out and what its rounding took away, itself rounded to the type)
+    e_whole = 1.01 * ((rel + t) * (w @ v.abs()) + z * (see @ v.abs()) + (t * t + 2 * U) * out.abs() + z)
+    e_delta = (g.abs() * e_whole).sum(-1, keepdim=True) + (d + 2) * U * (g * out).abs().sum(-1, keepdim=True)
     gs = w * (gp - delta)
     e_gs = w * (e_gp + e_delta + 2 * U * (gp.abs() + delta.abs())) + (rel + t) * gs.abs() + z * see
     gv = w.T @ g

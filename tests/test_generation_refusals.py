@@ -102,7 +102,7 @@ def test_c_entries_refuse_before_the_device():
 
     def packed(q=p, **kw):
         a = {**ok, **kw}
-        return lib.aps_attention_packed(q, p, p, p, 0, p, None, a["total"], a["N"], a["Hq"], a["Hkv"], a["D"], a["q_t"],
+        return lib.aps_attention_packed(q, p, p, p, 0, p, None, None, a["total"], a["N"], a["Hq"], a["Hkv"], a["D"], a["q_t"],
                                         a["q_h"], a["k_t"], a["k_h"], a["v_t"], a["v_h"], a["dtype"], 1, a["scale"], None)
 
     assert packed(total=0) == 0
@@ -171,3 +171,23 @@ def test_beam_search_refusals():
     small = TorchTransformerDecoder(9, num_layers=1, arch_kwargs={**arch, "nhead": 8}).eval()
     with pytest.raises(NotImplementedError):
         small.beam_search(enc, None, prompt, 1)
+
+
+def test_backward_arguments_at_the_c_entry():
+    """16-bit gradients need what the rounding of the output took away; shapes, alignment and workspace as forward"""
+    import ctypes
+    from aps_amd import _native as nat
+    lib = nat.load()
+    buf = ctypes.create_string_buffer(64)
+    p = ctypes.addressof(buf)
+    p += -p % 16
+
+    def backward(total=5, N=1, Hq=4, D=64, dtype=1, rest=p, ws=p, go=p, scale=1.0):
+        return lib.aps_attention_packed_backward(p, p, p, p, rest, go, p, p, 0, p, p, p, total, N, Hq, 2, D, 256, 64, 128,
+                                                 64, 128, 64, 256, 64, dtype, 1, scale, ws, None)
+
+    assert backward(total=0) == 0
+    for bad in ({"rest": None}, {"rest": p + 2}, {"dtype": 2, "rest": None}, {"ws": None}, {"go": p + 4}, {"N": 0},
+                {"Hq": 5}, {"scale": 0.0}, {"total": -1}):
+        assert backward(**bad) == -1, bad
+    assert backward(D=96) == -2 and backward(dtype=5) == -2
