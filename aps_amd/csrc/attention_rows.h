@@ -11,11 +11,11 @@
 // per tile.  Running maximum, sum and output stay in fp32; the output is rescaled only when the running
 // maximum grows by more than 2^8 (the weights are then at most 2^8, exact to the same relative error).
 //
-// Measured (MI355X): 6 prompts of 660 - 8 192 tokens, 32 heads over 8 of 128, bf16, causal: 1.31 ms, 830
-// TFLOP/s; a large bf16 matrix product of the library reaches 1 157.  The matrix pipe is busy 42 % of the cycles,
-// the vector pipe (half of it the exponentials) 35 %; the two wavefronts of a SIMD overlap the two only in
-// part.  Wave priorities around the products or around the softmax cost 6 %.  Short sequences are bound by the
-// chain bounds -> rows -> first tiles, about 5 us.
+// Measured (MI355X): 6 prompts of 660 - 8 192 tokens, 32 heads over 8 of 128, bf16, causal: 1.16 - 1.36 ms by card, 800 -
+// 940 TFLOP/s; a large bf16 matrix product of the library reaches 1 157.  The matrix pipe is busy 45 % of the cycles
+// (at 1.8 GHz: the card is at its power limit), the vector pipe, half of it the exponentials, about as much; the
+// two wavefronts of a SIMD overlap the two only in part.  Wave priorities around the products or around the softmax
+// cost 6 %.  Short sequences are bound by the chain bounds -> rows -> first tiles, about 5 us.
 #ifndef APS_AMD_ATTENTION_ROWS_H_
 #define APS_AMD_ATTENTION_ROWS_H_
 
