@@ -260,7 +260,8 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           qr[i] = gr[i] = zero_raw<T>();
-          if (tok_i[i] < t.len - tok0 && head0 + head_i[i] < a.G) qr[i] = load_chunk<T>(q0, q_at[i]), gr[i] = load_chunk<T>(g0, g_at[i]);
+          if (tok_i[i] < t.len - tok0 && head0 + head_i[i] < a.G)
+            qr[i] = load_chunk<T>(q0, q_at[i]), gr[i] = load_chunk<T>(g0, g_at[i]);
         }
       }
     } else {

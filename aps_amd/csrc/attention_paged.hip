@@ -110,7 +110,8 @@ __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void atte
   for (int ch = lo + wv; ch < hi; ch += 4) {
     // slot of key (lane % 32); -1 past the end or for a page outside the cache (which has < 2^31 slots)
     const int key = ch * kDecodeChunk + (lane & 31);
-    const int slot = key >= end || next < 0 || next >= a.num_pages ? -1 : (next << a.page_shift) + (key & ((1 << a.page_shift) - 1));
+    const int slot = key >= end || next < 0 || next >= a.num_pages
+                         ? -1 : (next << a.page_shift) + (key & ((1 << a.page_shift) - 1));
     next = page_of(ch + 4);
     u32x4 kf[2][NS];
 #pragma unroll

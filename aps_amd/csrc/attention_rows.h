@@ -85,8 +85,10 @@ struct KvStage {
   __device__ __forceinline__ void locate(const RowsArgs& a, int seq, int key0, int end) {
     if constexpr (PAGED) {
 #pragma unroll
-      for (int i = 0; i < PER; ++i)
-        page[i] = a.table[(int64_t)seq * a.table_stride + (min(key0 + (int)threadIdx.x / CH + i * STEP, end - 1) >> a.page_shift)];
+      for (int i = 0; i < PER; ++i) {
+        const int key = min(key0 + (int)threadIdx.x / CH + i * STEP, end - 1);
+        page[i] = a.table[(int64_t)seq * a.table_stride + (key >> a.page_shift)];
+      }
     }
   }
   __device__ __forceinline__ void resolve(const RowsArgs& a, int key0, int end) {
@@ -138,8 +140,8 @@ struct KvStage {
     for (int i = 0; i < PER; ++i) store_chunk<T, D, PLANE>(tile, r0 + i * STEP, c, r[i]);
   }
   // Values on their way to a tile that some row sees only in part (f32: to any tile, a plane that is 0 times
-  // infinity being NaN): 0 * infinity is not 0, so a non-finite value would reach the rows it is hidden from.  It goes to LDS as 0 and is added to the rows that see it
-  // in the end (`add_non_finite`).  True if there was one.
+  // infinity being NaN): 0 * infinity is not 0, so a non-finite value would reach the rows it is hidden from.  It
+  // goes to LDS as 0 and is added to the rows that see it in the end (`add_non_finite`).  True if there was one.
   __device__ __forceinline__ bool sanitize() {
     Raw<T>* v = r + (TURNS ? 0 : PER);
     bool any = false;

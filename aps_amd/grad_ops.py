@@ -620,7 +620,8 @@ class AttentionCrossFn(th.autograd.Function):
 
 class AttentionPackedFn(th.autograd.Function):
     """nn_ops.attention_packed with its adjoint (aps_attention_packed_backward): the forward keeps the
-    softmax sums, the backward forms the weights again from them, a tile at a time"""
+    softmax sums (16-bit types: and what the output's rounding took away), the backward forms the weights
+    again from them, a tile at a time"""
 
     @staticmethod
     def forward(ctx, q, k, v, cu_seqlens, causal, scale):
@@ -651,9 +652,9 @@ def _attention_packed_backward(ctx, g):
         ws = th.empty_like(sums)  # aps_attention_packed_backward_workspace bytes
         with nat.on_device_of(q):
             rc = nat.load().aps_attention_packed_backward(
-                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if rest is None else rest.data_ptr(), g.data_ptr(), sums.data_ptr(),
-                cu_seqlens.data_ptr(), int(cu_seqlens.dtype == th.int64), g_q.data_ptr(), g_k.data_ptr(),
-                g_v.data_ptr(), T, cu_seqlens.shape[0] - 1, Hq, k.shape[1], D, q.stride(0), q.stride(1), k.stride(0),
+                q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if rest is None else rest.data_ptr(),
+                g.data_ptr(), sums.data_ptr(), cu_seqlens.data_ptr(), int(cu_seqlens.dtype == th.int64),
+                g_q.data_ptr(), g_k.data_ptr(), g_v.data_ptr(), T, cu_seqlens.shape[0] - 1, Hq, k.shape[1], D, q.stride(0), q.stride(1), k.stride(0),
                 k.stride(1), v.stride(0), v.stride(1), g.stride(0), g.stride(1), nn_ops.ELEMENT_TYPES[q.dtype],
                 int(causal), scale, ws.data_ptr(), nat.stream_of(q))
         nat.check(rc, "aps_attention_packed_backward")
