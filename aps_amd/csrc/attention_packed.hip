@@ -3,7 +3,7 @@
 //   D_r  = do_r . o_r        (16-bit: of o and of what its rounding took away, which the forward pass keeps for it.
 //          D_r enters every dS_rj, and sequences of 64 tokens would lose more by o's rounding than by that of
 //          dS: dq off by 3.0e-3 instead of 2.3e-3 in bf16, where rounding the result alone is 1.7e-3.  Writing
-//          and reading it takes 7 + 5 us of 418 on the 12 sequences named below.)
+//          and reading it takes 7 + 5 us of 400 on the 12 sequences named below.)
 //   dS_rj = P_rj (do_r . v_j - D_r) scale
 //   dq_r = sum_j dS_rj k_j,   dk_j = sum_r dS_rj q_r,   dv_j = sum_r P_rj do_r
 // with r over the rows (token, head of the group) that see key j: the sums over a group's heads are part
@@ -23,21 +23,22 @@ struct GradArgs {
   Index cu;
   int64_t total, N, tiles;
   int64_t q_t, q_h, k_t, k_h, v_t, v_h, go_t, go_h;
-  int32_t G, Hkv, causal;
+  int32_t G, Hkv, causal, by_cost;
   float c, scale;
 };
 
 // dq: the forward kernel's walk, with V as the left operand of dP^T = V dO^T beside S^T = K Q^T and K
-// read transposed for dq^T = K^T dS^T.  (The 12 sequences named at the next kernel: 112 us, 590 TFLOP/s; the 3:
-// 200 us, 740.)
+// read transposed for dq^T = K^T dS^T.  (The 12 sequences named at the next kernel: 101 us, 660 TFLOP/s; the 3:
+// 183 us, 810.)
 template <typename T, int D>
 __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attention_rows_backward_kernel(GradArgs a) {
   constexpr int BK = key_tile<T, D>(), NS = D / 16, NKB = BK / 32, NDB = D / 32, PLANE = BK * D * 2, TILE = planes<T>() * PLANE;
   __shared__ __align__(16) char lds[4 * TILE];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
-  const int want = (int)a.tiles - 1 - blockIdx.x / a.Hkv;
-  const SeqTile t = find_tile(a.cu, a.N, a.total, a.G, kRowTile, want, lane);
+  const int number = blockIdx.x / a.Hkv, want = a.by_cost ? number : (int)a.tiles - 1 - number;
+  const SeqTile t = a.by_cost ? find_tile_by_cost(a.cu, (int)a.N, a.total, a.G, kRowTile, want, lane)
+                              : find_tile(a.cu, a.N, a.total, a.G, kRowTile, want, lane);
   const int Hq = a.Hkv * a.G;
   if (t.seq < 0) {
     if (h == 0)
@@ -415,6 +416,14 @@ static void launch_keys_backward(GradArgs a, hipStream_t st) {
 using namespace aps;
 using namespace aps::att;
 
+// Tiles by cost where the card takes two to eight rounds of them (512 workgroups at two a CU).  The 12 sequences (1 248
+// workgroups): forward 93.6 -> 86.0 us, dq 108 -> 101; the 3 (1 568): 149.7 -> 145.4 and 191 -> 183.  One round needs no
+// order; over many rounds the ends even out, and neighbours of one sequence share its keys in the L2: 6 prompts
+// (5 968) take 1 354 us in the sequences' order and 1 381 by cost.
+static inline int tiles_by_cost(int32_t causal, int64_t N, unsigned grid) {
+  return causal != 0 && N > 1 && N <= 64 && grid > 512 && grid <= 4096;
+}
+
 extern "C" int aps_attention_packed(const void* q, const void* k, const void* v, const void* cu_seqlens,
                                     int32_t cu_wide, void* out, void* out_rest, float* lse, int64_t total, int64_t N,
                                     int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t q_t, int64_t q_h,
@@ -435,6 +444,7 @@ extern "C" int aps_attention_packed(const void* q, const void* k, const void* v,
   a.causal = causal != 0, a.zero_tail = 1, a.splits = 1;
   a.c = scale * kLog2e;
   const unsigned grid = (unsigned)(a.tiles * Hkv);
+  a.by_cost = tiles_by_cost(causal, N, grid);
   hipStream_t st = static_cast<hipStream_t>(stream);
   APS_ATT_DISPATCH(launch_rows, a, grid, st);
   return aps_launch_status();
@@ -471,6 +481,7 @@ extern "C" int aps_attention_packed_backward(const void* q, const void* k, const
   hipStream_t st = static_cast<hipStream_t>(stream);
   a.tiles = (total * a.G + kRowTile - 1) / kRowTile + N + 1;
   const unsigned grid = (unsigned)(a.tiles * Hkv);
+  a.by_cost = tiles_by_cost(causal, N, grid);
   APS_ATT_DISPATCH(launch_rows_backward, a, grid, st);
   if (aps_launch_status() != APS_OK) return APS_ERR_LAUNCH;
   APS_ATT_DISPATCH(launch_keys_backward, a, st);

@@ -39,6 +39,7 @@ struct RowsArgs {
   int32_t page_shift;                    // paged: log2 of the page size
   int32_t G, Hkv;
   int32_t causal, zero_tail;
+  int32_t by_cost;        // packed: tiles in the order of find_tile_by_cost
   float c;                // scale * log2(e) > 0
   // split over the keys (paged): partial results [split][total * Hq]{D floats} and {max, sum}
   float* part_o;
@@ -194,8 +195,9 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>())) void attention_rows_kern
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
   // the last tiles of a sequence see the most keys: they go first
-  const int want = (int)a.tiles - 1 - blockIdx.x / a.Hkv;
-  const SeqTile t = find_tile(a.cu, a.N, a.total, a.G, kRowTile, want, lane);
+  const int number = blockIdx.x / a.Hkv, want = !PAGED && a.by_cost ? number : (int)a.tiles - 1 - number;
+  const SeqTile t = !PAGED && a.by_cost ? find_tile_by_cost(a.cu, (int)a.N, a.total, a.G, kRowTile, want, lane)
+                                        : find_tile(a.cu, a.N, a.total, a.G, kRowTile, want, lane);
   const int Hq = a.Hkv * a.G;
   if (t.seq < 0) {
     if (a.zero_tail && h == 0 && blockIdx.y == 0)

@@ -336,6 +336,42 @@ __device__ __forceinline__ SeqTile find_tile(const Index& cu, int64_t N, int64_t
   return SeqTile{-1, 0, 0, 0, base};
 }
 
+// The sum over the wavefront of numbers 0 <= v < 2^bits, by one ballot a bit
+__device__ __forceinline__ int sum_by_bits(int v, int bits) {
+  int sum = 0;
+  for (int b = 0; b < bits; ++b) sum += __builtin_popcountll(__ballot((v >> b) & 1)) << b;
+  return sum;
+}
+
+// The same tiles, those with the highest number within their sequence first: tile i of a causal sequence sees the keys
+// up to its own, so that is the order of their cost, and the launch does not end on a long one.  N <= 64.
+__device__ __forceinline__ SeqTile find_tile_by_cost(const Index& cu, int N, int64_t total, int per, int rows, int want,
+                                                     int lane) {
+  int s = 0, e = 0;
+  if (lane < N) seq_range(cu, lane, total, s, e);
+  const int len = e - s, tiles = (int)(((uint32_t)len * (uint32_t)per + rows - 1) / (uint32_t)rows);
+  int most = 1;  // 2^bits > tiles of any sequence
+  int bits = 0;
+  while (__ballot(tiles >= most)) most <<= 1, ++bits;
+  const int all = sum_by_bits(tiles, bits);
+  if (want >= all) return SeqTile{-1, 0, 0, 0, all};
+  // the largest number `lo` such that more than `want` tiles have it or a higher one
+  int lo = 0, hi = most, above = 0;  // above: tiles numbered `hi` or higher
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1, n = sum_by_bits(max(tiles - mid, 0), bits);
+    if (n > want) lo = mid;
+    else hi = mid, above = n;
+  }
+  const uint64_t have = __ballot(tiles > lo);
+  const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(have >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)have, 0));
+  const int at = __builtin_ctzll(__ballot(tiles > lo && before == want - above));
+  SeqTile t;
+  t.seq = at, t.tile = lo, t.used = 0;
+  t.len = __builtin_amdgcn_readlane(len, at);
+  t.start = __builtin_amdgcn_readlane(s, at);
+  return t;
+}
+
 // first token behind the last sequence
 __device__ __forceinline__ int64_t tail_of(const Index& cu, int64_t N, int64_t total) {
   const int64_t e = cu.at(N);

@@ -616,3 +616,19 @@ def test_large_scores_and_scale():
         (want,), (bound,) = ref.packed(q, k, v, lens, True, scale=scale)
         with torch.no_grad():
             ref.check(nn_ops.attention_packed(q, k, v, cu_of(lens), scale=scale), want, bound, f"scale {scale}")
+
+
+@gpu
+@pytest.mark.parametrize("lens", [[260, 0, 700, 1, 130, 690], [1023, 1024]])
+def test_tiles_in_the_order_of_their_cost(lens):
+    """enough tiles for several rounds of the card: taken by cost, every one once, the rows behind the last sequence zeros"""
+    from aps_amd import nn_ops
+    H, T = 34, sum(lens) + 9
+    x = [randn(T, H, 32, dtype=torch.bfloat16, seed=i).requires_grad_() for i in range(3)]
+    g = randn(T, H, 32, dtype=torch.bfloat16, seed=7)
+    out = nn_ops.attention_packed(*x, cu_of(lens))
+    grads = torch.autograd.grad(out, x, g)
+    vals, bounds = ref.packed(*x, lens, True, g=g)
+    for name, got, want, bound in zip(("out", "gq", "gk", "gv"), (out,) + grads, vals, bounds):
+        ref.check(got, want, bound, name)
+        assert not got[sum(lens):].any()
