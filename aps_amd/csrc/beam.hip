@@ -23,22 +23,26 @@ constexpr int kThreads = 256;
 constexpr int kMaxBeam = 64, kCandidates = 1024, kHeld = 4;
 constexpr float kLargest = 3.4028234663852886e38f;
 
-// 2^y for y <= 0 in 64 bits, relative error < 1e-9: 2^f, |f| <= 1/2, by its series to f^8; 0 for -infinity
-__device__ __forceinline__ double exp2_64(double y) {
-  y = fmax(y, -1100.);
-  const double n = rint(y), f = y - n;
-  double p = 1.3215486790144307e-6;
-  p = fma(p, f, 1.5252733804059839e-5);
-  p = fma(p, f, 1.5403530393381608e-4);
-  p = fma(p, f, 1.3333558146428443e-3);
-  p = fma(p, f, 9.6181291076284772e-3);
-  p = fma(p, f, 5.5504108664821580e-2);
-  p = fma(p, f, 2.4022650695910071e-1);
-  p = fma(p, f, 6.9314718055994531e-1);
+// e^d for d <= 0 in 64 bits: 2^(i / 32) from a table, i the whole part of 32 d log2(e) and |f| <= 1/2 the rest, times
+// e^(f ln(2) / 32) by its series to f^5 (cut off below 3e-15).  d is a difference from the largest logit, formed before
+// anything is multiplied: it is 0 for that logit whatever its size, where d log2(e) taken as a difference of two
+// products is the rounding error of the second (1e22 for the largest finite f32).  Relative error below
+// 4e-15 + |d| 2^-52.  Table and series: as many operations as a series to f^8 alone, which is good to 1e-9.
+constexpr int kOctave = 32;
+constexpr double kStep = 46.16624130844683;  // kOctave log2(e)
+__device__ __forceinline__ double exp_neg(double d, const double* table) {
+  const double y = fmax(d * kStep, -34500.);           // (2^-1078: 0)
+  const double t = y + 6755399441055744.;              // 1.5 * 2^52: the low bits are the nearest integer
+  const int i = (int)(uint32_t)__double_as_longlong(t);
+  const double f = y - (t - 6755399441055744.);
+  double p = 3.9737099845494154e-11;  // (ln(2) / 32)^k / k!
+  p = fma(p, f, 9.172562701824643e-09);
+  p = fma(p, f, 1.6938509724371819e-06);
+  p = fma(p, f, 2.3459619820224677e-04);
+  p = fma(p, f, 2.166084939249829e-02);
   p = fma(p, f, 1.0);
-  return ldexp(p, (int)n);
+  return ldexp(p * table[i & (kOctave - 1)], i >> 5);
 }
-constexpr double kLog2e64 = 1.4426950408889634074;
 
 // order-preserving integers: larger value, larger integer
 __device__ __forceinline__ uint32_t ordered(float x) {
@@ -125,7 +129,7 @@ template <typename T, int PER>
 __global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
   constexpr int VE = 16 / (int)sizeof(T), NV = PER / VE, TILE = kThreads * PER;
   __shared__ __align__(16) uint64_t s_cand[kCandidates];
-  __shared__ double s_sum[4];
+  __shared__ double s_sum[4], s_table[kOctave];
   __shared__ float s_top[4];
   __shared__ uint32_t s_kth[4];
   __shared__ uint64_t s_best[4];
@@ -135,6 +139,7 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
   const int split = blockIdx.y, V = a.V, K = a.K;
   uint64_t* out = a.keys + (row * a.splits + split) * K;
   if (tid == 0) s_count = 0;
+  if (tid < kOctave) s_table[tid] = exp2(tid * (1. / kOctave));
   const uint64_t none = (uint64_t)ordered(-INFINITY) << 32;  // key of a ruled-out token, its index apart
   const bool done = a.done && a.done[row];
   const bool dead = !(a.score[row] > -INFINITY);  // (NaN too)
@@ -198,9 +203,8 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
   }
   double sum = 0.;
   if (top > -INFINITY) {
-    const double ref = -(double)top * kLog2e64;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) sum += exp2_64(fma((double)x[i], kLog2e64, ref));
+    for (int i = 0; i < PER; ++i) sum += exp_neg((double)x[i] - (double)top, s_table);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
@@ -278,8 +282,9 @@ struct MergeArgs {
 __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
   __shared__ uint64_t s_key[kCandidates];
   __shared__ uint32_t s_flat[kCandidates];
-  __shared__ double s_add[kMaxBeam];  // score - log sum exp of a hypothesis
-  __shared__ double s_score[kMaxBeam];
+  // of a hypothesis: its score, its largest logit, log sum exp(logit - largest).  The last two stay apart: beside a
+  // logit of 1e30 their sum would lose the logarithm.
+  __shared__ double s_score[kMaxBeam], s_top[kMaxBeam], s_log[kMaxBeam];
   __shared__ uint32_t s_kth[4];
   __shared__ uint64_t s_best[4];
   __shared__ uint32_t s_best_flat[4];
@@ -296,8 +301,9 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
     if (top > -INFINITY)
       for (int s = 0; s < S; ++s)
         if (a.top[row * S + s] > -INFINITY)
-          sum += a.sum[row * S + s] * exp2_64(((double)a.top[row * S + s] - (double)top) * kLog2e64);
-    s_add[tid] = top > -INFINITY ? (double)top + log(sum) : 0.;
+          sum += a.sum[row * S + s] * exp((double)a.top[row * S + s] - (double)top);
+    s_top[tid] = top > -INFINITY ? (double)top : 0.;
+    s_log[tid] = top > -INFINITY ? log(sum) : 0.;
     s_score[tid] = (double)tame(a.score[row]);
   }
   const uint64_t* keys = a.keys + n * B * S * K;
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
     const uint32_t token = ~(uint32_t)key;
     flat = (uint32_t)b * (uint32_t)a.V + token;
     const float x = from_ordered((uint32_t)(key >> 32));
-    return ordered(x > -INFINITY ? s_score[b] + ((double)x - s_add[b]) + 0. : (double)-INFINITY);
+    return ordered(x > -INFINITY ? s_score[b] + ((double)x - s_top[b] - s_log[b]) + 0. : (double)-INFINITY);
   };
   uint64_t best = 0;
   uint32_t held_flat[kHeld];
