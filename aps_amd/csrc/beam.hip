@@ -8,7 +8,8 @@
 // row into registers, forms their maximum, their sum of exponentials and their K largest
 // (`beam_rows_kernel`); a workgroup per utterance merges the B * splits * K candidates
 // (`beam_merge_kernel`).  Sum and totals are in 64 bits: two candidates may lie closer than the
-// rounding of a 32-bit log-softmax, and the order must not depend on how the sum was cut.
+// rounding of a 32-bit log-softmax.  A row is cut by its tokens' numbers, wherever it lies in memory, so rows of
+// equal logits have equal sums to the last bit and the tie between their hypotheses goes to the first.
 #include "common.h"
 
 namespace aps {
@@ -16,6 +17,9 @@ namespace beam {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// 16 bytes at any element: a global load takes them in one instruction wherever they begin
+template <typename T>
+struct __attribute__((packed, aligned(sizeof(T)))) Unaligned { u32x4 v; };
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
@@ -161,20 +165,18 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
     }
     return;
   }
-  // aligned vectors: element e0 + i of the row; the first vector may begin before the row
   const T* base = static_cast<const T*>(a.x) + row * a.stride;
-  const int shift = (int)((reinterpret_cast<uintptr_t>(base) & 15) / sizeof(T));
-  const int first = split * TILE + tid * VE - shift;  // vector j of the thread: first + j * 256 VE
+  const int first = split * TILE + tid * VE;  // vector j of the thread: tokens first + j * 256 VE ..
   float x[PER];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int e0 = first + j * kThreads * VE;
     float* to = x + j * VE;
-    if (e0 >= 0 && e0 + VE <= V) {
-      widen<T>(*reinterpret_cast<const u32x4*>(base + e0), to);
+    if (e0 + VE <= V) {
+      widen<T>(reinterpret_cast<const Unaligned<T>*>(base + e0)->v, to);
     } else {
 #pragma unroll
-      for (int i = 0; i < VE; ++i) to[i] = (e0 + i >= 0 && e0 + i < V) ? (float)base[e0 + i] : -INFINITY;
+      for (int i = 0; i < VE; ++i) to[i] = e0 + i < V ? (float)base[e0 + i] : -INFINITY;
     }
   }
   float best = -INFINITY;
@@ -226,7 +228,7 @@ __global__ __launch_bounds__(kThreads) void beam_rows_kernel(RowsArgs a) {
     if (count < K) {
       // Of the split's first K + count tokens at most `count` are not ruled out: the lowest ones of the rest
       // follow, then nothing.  (K + count < 128: two wavefronts)
-      const int lo = max(0, split * TILE - shift), hi = min(V, split * TILE - shift + TILE);
+      const int lo = split * TILE, hi = min(V, lo + TILE);
       bool out_of = false;
       if (tid < 128 && lo + tid < hi) out_of = tame((float)base[lo + tid]) == -INFINITY;
       const uint64_t mask = __ballot(out_of);
@@ -474,7 +476,7 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
 static int per_thread(int64_t rows, int64_t V) { return rows * ((V + 8191) / 8192) < 512 ? 8 : 32; }
 static int64_t splits_of(int64_t rows, int64_t V) {
   const int64_t tile = kThreads * per_thread(rows, V);
-  return (V + 7 + tile - 1) / tile;  // (a row may begin up to 7 elements into its first vector)
+  return (V + tile - 1) / tile;
 }
 static bool sizes_fit(int64_t N, int64_t B, int64_t V, int64_t K) {
   return N >= 1 && B >= 1 && B <= kMaxBeam && K >= 1 && K <= kMaxBeam && V >= 1 && V <= (1 << 24) &&

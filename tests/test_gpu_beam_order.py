@@ -47,8 +47,8 @@ def definition(logits, scores, K):
 
 def check(logits, scores, K):
     from aps_amd import nn_ops
-    got = [x.cpu() for x in nn_ops.beam_select(logits.to(DEV), scores.to(DEV), 1, beam=K)]
-    best, parent, token = definition(logits, scores, K)
+    got = [t.cpu() for t in nn_ops.beam_select(logits.to(DEV), scores.to(DEV), 1, beam=K)]
+    best, parent, token = definition(logits.cpu(), scores, K)
     assert torch.equal(got[1], parent), (got[1], parent)
     assert torch.equal(got[2], token), (got[2], token)
     assert torch.equal(got[3], token == 1)
@@ -99,3 +99,19 @@ def test_rows_of_one_large_value():
     for value in (1e38, -1e38, 3e15, -7e20, torch.finfo(torch.float32).max, torch.finfo(torch.float32).min):
         for v in (33, 9000):
             check(torch.full((6, v), value), SCORES, 7)
+
+
+@gpu
+@pytest.mark.parametrize("kind,v", [("f32", 501), ("f32", 4233), ("bf16", 10007), ("f16", 333), ("f32", 20011)])
+def test_equal_hypotheses_tie_to_the_first(kind, v):
+    """hypotheses with the same logits and the same score: every token of the first comes ahead of the second's,
+    whatever address their rows begin at"""
+    n, b = 12, 5
+    x = randn(n, 1, v, dtype=TYPES[kind], seed=v, std=2.0).expand(n, b, v).reshape(n * b, v)
+    scores = -randn(n, 1, seed=3).abs().expand(n, b).contiguous()
+    for K in (b, 2 * b + 1):
+        check(x, scores, K)
+    wide = torch.zeros(n * b, v + 5, dtype=TYPES[kind], device=DEV)
+    for first in (0, 1, 3):
+        wide[:, first:first + v] = x.to(DEV)
+        check(wide[:, first:first + v], scores, b)
