@@ -24,7 +24,7 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kThreads = 256;
-constexpr int kMaxBeam = 64, kCandidates = 1024, kHeld = 4;
+constexpr int kMaxBeam = 64, kTokenBits = 24, kCandidates = 1024, kHeld = 4;
 constexpr float kLargest = 3.4028234663852886e38f;
 
 // e^d for d <= 0 in 64 bits: 2^(i / 32) from a table, i the whole part of 32 d log2(e) and |f| <= 1/2 the rest, times
@@ -278,18 +278,16 @@ struct MergeArgs {
   int64_t *parent, *token;
   uint8_t* new_done;
   int64_t eos;
-  int32_t B, V, K, splits;
+  int32_t B, K, splits;
 };
 
 __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
-  __shared__ uint64_t s_key[kCandidates];
-  __shared__ uint32_t s_flat[kCandidates];
+  __shared__ uint64_t s_key[kCandidates], s_tie[kCandidates];
   // of a hypothesis: its score, its largest logit, log sum exp(logit - largest).  The last two stay apart: beside a
   // logit of 1e30 their sum would lose the logarithm.
   __shared__ double s_score[kMaxBeam], s_top[kMaxBeam], s_log[kMaxBeam];
   __shared__ uint32_t s_kth[4];
-  __shared__ uint64_t s_best[4];
-  __shared__ uint32_t s_best_flat[4];
+  __shared__ uint64_t s_best[4], s_best_tie[4];
   __shared__ int s_count;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int64_t n = blockIdx.x;
@@ -315,26 +313,27 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) held[i] = tid + i * kThreads < total ? keys[tid + i * kThreads] : 0;
   __syncthreads();
-  // candidate c of the utterance: its total as an ordered integer (0: none) and its flat index
-  auto candidate = [&](int c, uint64_t key, uint32_t& flat) -> uint64_t {
+  // Candidate c of the utterance: its total as an ordered integer (0: none), and what decides between equal totals,
+  // the larger the better: the lower hypothesis, then the larger logit (64 bits may round two to one total, where the
+  // row has kept the larger ones), then the lower token
+  auto candidate = [&](int c, uint64_t key, uint64_t& tie) -> uint64_t {
     if (!key) return 0;
     const int b = c / (S * K);
-    const uint32_t token = ~(uint32_t)key;
-    flat = (uint32_t)b * (uint32_t)a.V + token;
+    tie = (uint64_t)(kMaxBeam - 1 - b) << 56 | (key >> 32) << kTokenBits | ((uint32_t)key & ((1 << kTokenBits) - 1));
     const float x = from_ordered((uint32_t)(key >> 32));
     return ordered(x > -INFINITY ? s_score[b] + ((double)x - s_top[b] - s_log[b]) + 0. : (double)-INFINITY);
   };
   uint64_t best = 0;
-  uint32_t held_flat[kHeld];
+  uint64_t held_tie[kHeld];
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) {
-    held_flat[i] = 0;
-    held[i] = candidate(tid + i * kThreads, held[i], held_flat[i]);
+    held_tie[i] = 0;
+    held[i] = candidate(tid + i * kThreads, held[i], held_tie[i]);
     best = held[i] > best ? held[i] : best;
   }
   for (int c = tid + kHeld * kThreads; c < total; c += kThreads) {
-    uint32_t flat;
-    const uint64_t v = candidate(c, keys[c], flat);
+    uint64_t tie;
+    const uint64_t v = candidate(c, keys[c], tie);
     best = v > best ? v : best;
   }
   const uint32_t kth = wave_kth<0>((uint32_t)(best >> 32), K);  // (bounds the totals by their upper halves)
@@ -346,26 +345,26 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
 #pragma unroll
   for (int i = 0; i < kHeld; ++i) mine += held[i] >= least;
   for (int c = tid + kHeld * kThreads; c < total; c += kThreads) {
-    uint32_t flat;
-    mine += candidate(c, keys[c], flat) >= least;
+    uint64_t tie;
+    mine += candidate(c, keys[c], tie) >= least;
   }
   int at = place(mine, lane, &s_count);
-  auto collect = [&](uint64_t v, uint32_t flat) {
+  auto collect = [&](uint64_t v, uint64_t tie) {
     if (v < least) return;
-    if (at < kCandidates) s_key[at] = v, s_flat[at] = flat;
+    if (at < kCandidates) s_key[at] = v, s_tie[at] = tie;
     ++at;
   };
 #pragma unroll
-  for (int i = 0; i < kHeld; ++i) collect(held[i], held_flat[i]);
+  for (int i = 0; i < kHeld; ++i) collect(held[i], held_tie[i]);
   for (int c = tid + kHeld * kThreads; c < total; c += kThreads) {
-    uint32_t flat = 0;
-    const uint64_t v = candidate(c, keys[c], flat);
-    collect(v, flat);
+    uint64_t tie = 0;
+    const uint64_t v = candidate(c, keys[c], tie);
+    collect(v, tie);
   }
   __syncthreads();
   const int count = s_count;
-  auto put = [&](int rank, uint64_t v, uint32_t flat) {
-    const int64_t b = flat / (uint32_t)a.V, token = flat % (uint32_t)a.V;
+  auto put = [&](int rank, uint64_t v, uint64_t tie) {
+    const int64_t b = kMaxBeam - 1 - (int64_t)(tie >> 56), token = ~(uint32_t)tie & ((1 << kTokenBits) - 1);
     const int64_t at = n * K + rank;
     a.new_score[at] = (float)from_ordered(v);
     a.parent[at] = b;
@@ -375,38 +374,35 @@ __global__ __launch_bounds__(kThreads) void beam_merge_kernel(MergeArgs a) {
   if (count <= kCandidates) {
     for (int c = tid; c < count; c += kThreads) {
       const uint64_t v = s_key[c];
-      const uint32_t flat = s_flat[c];
+      const uint64_t tie = s_tie[c];
       int rank = 0;
 #pragma unroll 8
-      for (int o = 0; o < count; ++o) rank += s_key[o] > v || (s_key[o] == v && s_flat[o] < flat);
-      if (rank < K) put(rank, v, flat);
+      for (int o = 0; o < count; ++o) rank += s_key[o] > v || (s_key[o] == v && s_tie[o] > tie);
+      if (rank < K) put(rank, v, tie);
     }
     return;
   }
-  uint64_t last = ~0ull;
-  uint32_t last_flat = 0;
+  uint64_t last = ~0ull, last_tie = ~0ull;
   for (int k = 0; k < K; ++k) {
-    uint64_t mx = 0;
-    uint32_t mx_flat = 0;
+    uint64_t mx = 0, mx_tie = 0;
     for (int c = tid; c < total; c += kThreads) {
-      uint32_t flat = 0;
-      const uint64_t v = candidate(c, keys[c], flat);
-      if (!v || !(v < last || (v == last && flat > last_flat))) continue;
-      if (v > mx || (v == mx && flat < mx_flat)) mx = v, mx_flat = flat;
+      uint64_t tie = 0;
+      const uint64_t v = candidate(c, keys[c], tie);
+      if (!v || !(v < last || (v == last && tie < last_tie))) continue;
+      if (v > mx || (v == mx && tie > mx_tie)) mx = v, mx_tie = tie;
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
-      const uint64_t v = __shfl_xor(mx, o, 64);
-      const uint32_t flat = __shfl_xor(mx_flat, o, 64);
-      if (v > mx || (v == mx && flat < mx_flat)) mx = v, mx_flat = flat;
+      const uint64_t v = __shfl_xor(mx, o, 64), tie = __shfl_xor(mx_tie, o, 64);
+      if (v > mx || (v == mx && tie > mx_tie)) mx = v, mx_tie = tie;
     }
-    if (lane == 0) s_best[wv] = mx, s_best_flat[wv] = mx_flat;
+    if (lane == 0) s_best[wv] = mx, s_best_tie[wv] = mx_tie;
     __syncthreads();
-    last = s_best[0], last_flat = s_best_flat[0];
+    last = s_best[0], last_tie = s_best_tie[0];
 #pragma unroll
     for (int w = 1; w < 4; ++w)
-      if (s_best[w] > last || (s_best[w] == last && s_best_flat[w] < last_flat)) last = s_best[w], last_flat = s_best_flat[w];
-    if (tid == 0) put(k, last, last_flat);
+      if (s_best[w] > last || (s_best[w] == last && s_best_tie[w] > last_tie)) last = s_best[w], last_tie = s_best_tie[w];
+    if (tid == 0) put(k, last, last_tie);
     __syncthreads();
   }
 }
@@ -479,7 +475,7 @@ static int64_t splits_of(int64_t rows, int64_t V) {
   return (V + tile - 1) / tile;
 }
 static bool sizes_fit(int64_t N, int64_t B, int64_t V, int64_t K) {
-  return N >= 1 && B >= 1 && B <= kMaxBeam && K >= 1 && K <= kMaxBeam && V >= 1 && V <= (1 << 24) &&
+  return N >= 1 && B >= 1 && B <= kMaxBeam && K >= 1 && K <= kMaxBeam && V >= 1 && V <= (1 << kTokenBits) &&
          K <= B * V && N <= 0x7fffffff / B;
 }
 
@@ -525,7 +521,7 @@ extern "C" int aps_beam_select(const void* logits, int64_t row_stride, const flo
   MergeArgs m{};
   m.keys = r.keys, m.top = r.top, m.sum = r.sum, m.score = scores, m.done = finished, m.eos = eos;
   m.new_score = new_scores, m.parent = parent, m.token = token, m.new_done = new_finished;
-  m.B = (int32_t)B, m.V = (int32_t)V, m.K = (int32_t)K, m.splits = (int32_t)S;
+  m.B = (int32_t)B, m.K = (int32_t)K, m.splits = (int32_t)S;
   hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)N), dim3(kThreads), 0, st, m);
   return aps_launch_status();
 }

@@ -746,8 +746,8 @@ def beam_select(logits: th.Tensor, scores: th.Tensor, eos: int, finished: Option
     """One step of a beam search: logits N B x V (| N x B x V; f32 | bf16 | f16, not normalised) of B
     hypotheses of N utterances with scores N x B (f32) -> (scores, parent, token, finished), each N x K: the K =
     `beam` (default B) best of score + log_softmax(logits) over an utterance's B V continuations, best first,
-    ties to the lowest b V + v; parent (which of the B) and token int64, finished = the parent was, or the
-    token is `eos`.  finished N x B bool: such a hypothesis has one continuation, `eos` at its own score.
+    ties to the lowest b V + v (where 64 bits round different logits of one hypothesis to one total: the larger logit
+    first); parent (which of the B) and token int64, finished = the parent was, or the token is `eos`.  finished N x B bool: such a hypothesis has one continuation, `eos` at its own score.
     Ruled-out tokens are -inf logits, unused hypotheses -inf scores (the first step: B = 1, or scores 0, -inf,
     ...); they are selected only when nothing else is left.  NaN counts as -inf.  Totals in 64 bits."""
     what = "beam_select"

@@ -115,3 +115,21 @@ def test_equal_hypotheses_tie_to_the_first(kind, v):
     for first in (0, 1, 3):
         wide[:, first:first + v] = x.to(DEV)
         check(wide[:, first:first + v], scores, b)
+
+
+@gpu
+def test_logits_too_near_for_their_totals():
+    """totals of one hypothesis that 64 bits round to the same number are taken by logit: a vocabulary of tiny logits, and
+    one whose largest is the largest f32, which hides all differences of the others"""
+    for v in (90, 5000):
+        x = randn(4, v, seed=v) * 1e-25
+        check(x, torch.zeros(4, 1), 11)
+        check(x, torch.zeros(2, 2), 11)
+        x = randn(4, v, seed=v)
+        x[:, v // 3] = torch.finfo(torch.float32).max
+        check(x, torch.zeros(4, 1), 9)
+        x[:, 5] = INF
+        check(x, torch.zeros(4, 1), 9)
+    # more equal totals than the candidate list holds
+    x = randn(24, 60, seed=9) * 1e-25
+    check(x, torch.zeros(1, 24), 50)
