@@ -10,6 +10,14 @@
 // of the same accumulation.  Two launches, neither with atomics, so the gradients are bit-reproducible:
 // the first walks the keys for a tile of rows (D_r, dq), the second walks the rows for a tile of keys
 // (dk, dv); P is formed again in each from the saved lse.
+//
+// P and dS are rounded to the tensors' type between the products (attention_tile.h: `pack`).  f16 has 30 binary
+// orders: dS, of the size of do / (row length), would fall below its normal numbers with upstream gradients of 1e-3 and
+// pass its largest with 1e4, and P of long rows is small too.  So f16 takes both times powers of two, which come out
+// again in f32 at the end: P times 2^14 where it is rounded (dv), dS times 2^(14 - e), 2^e > |do_r| |v_j|, so that
+// |dS| <= 2 |do_r| |v_j| becomes at most 2^15.  For dq, e goes by the row's own norm and the largest norm of its
+// sequence's values (a launch ahead leaves one for every 128 keys: 6 us of 620 on the 3 sequences named below); for
+// dk by the key tile's values and the rows that see it (the dq launch leaves a norm for every 32 rows).
 #include "attention_rows.h"
 
 namespace aps {
@@ -19,6 +27,8 @@ struct GradArgs {
   const void *q, *k, *v, *o, *rest, *go;  // rest (16-bit): what the rounding of o took away
   const float* lse;    // [total, Hq]
   float* delta;        // [total, Hq]
+  float* row_norm;     // f16: largest |do_r|^2 of 32 rows, at [h][start G + first row]; of the [Hkv][total G] few are used
+  float* value_norm;   // f16: largest |v_j|^2 of 128 keys, at [h][start + first key]
   void *gq, *gk, *gv;  // [total, Hq | Hkv, D]
   Index cu;
   int64_t total, N, tiles;
@@ -26,6 +36,41 @@ struct GradArgs {
   int32_t G, Hkv, causal, by_cost;
   float c, scale;
 };
+
+template <typename T>
+constexpr bool narrow() { return __is_same(T, _Float16); }  // P and dS are scaled
+constexpr int kNormKeys = 128, kOrders = 14;
+
+// (an infinity or a NaN is left out: it makes NaN of what it reaches, whatever the factor)
+__device__ __forceinline__ float finite_or_zero(float x) { return finite(x) ? x : 0.f; }
+// the least e with |do| |v| < 2^e, from the norms' squares
+__device__ __forceinline__ int order_of(float do2, float v2) { return (__builtin_amdgcn_frexp_expf(do2 * v2) + 1) >> 1; }
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attention_value_norms_kernel(GradArgs a) {
+  constexpr int CH = D / kChunk, STEP = 256 / CH;
+  __shared__ float s_max[4];
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, h = blockIdx.x % a.Hkv;
+  const SeqTile t = find_tile(a.cu, a.N, a.total, 1, kNormKeys, blockIdx.x / a.Hkv, lane);
+  if (t.seq < 0) return;
+  const int key0 = t.tile * kNormKeys;
+  const T* v = static_cast<const T*>(a.v) + (t.start + key0) * a.v_t + h * a.v_h + threadIdx.x % CH * kChunk;
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < kNormKeys / STEP; ++i) {
+    const int key = min((int)threadIdx.x / CH + i * STEP, t.len - 1 - key0);  // (behind the end: the last one again)
+    const Raw<T> r = load_raw<T>(reinterpret_cast<const char*>(v + key * a.v_t));
+    float s = dot_raw<T>(r, r);
+#pragma unroll
+    for (int o = 1; o < CH; o <<= 1) s += __shfl_xor(s, o, 64);
+    most = fmaxf(most, finite_or_zero(s));
+  }
+  most = wave_max(most);
+  if (lane == 0) s_max[wv] = most;
+  __syncthreads();
+  if (threadIdx.x == 0)
+    a.value_norm[h * a.total + t.start + key0] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+}
 
 // dq: the forward kernel's walk, with V as the left operand of dP^T = V dO^T beside S^T = K Q^T and K
 // read transposed for dq^T = K^T dS^T.  (The 12 sequences named at the next kernel: 101 us, 660 TFLOP/s; the 3:
@@ -83,6 +128,20 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attenti
   delta += __shfl_xor(delta, 32, 64);
   const float lse = a.lse[at];
   if (live && half == 0) a.delta[at] = delta;
+  float times = 1.f, back = a.scale;  // f16: the factor of dS, and what takes it out again
+  if constexpr (narrow<T>()) {
+    float own = 0.f, most = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) own += dot_raw<T>(g[s], g[s]);
+    own = finite_or_zero(own + __shfl_xor(own, 32, 64));
+    for (int key = lane * kNormKeys; key < end; key += 64 * kNormKeys)
+      most = fmaxf(most, a.value_norm[h * a.total + t.start + key]);
+    const int order = order_of(own, wave_max(most));
+    times = ldexpf(1.f, kOrders - order), back = ldexpf(a.scale, order - kOrders);
+    delta *= times;
+    const float rows_most = wave_max(live ? own : 0.f);
+    if (lane == 0 && row0 < rows) a.row_norm[h * a.total * a.G + t.start * a.G + row0] = rows_most;
+  }
 
   f32x16 acc[NDB];
 #pragma unroll
@@ -133,7 +192,8 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attenti
       if (!sees) continue;
       float p[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) p[i] = exp2_fast(fmaf(s[i], a.c, -lse)) * (g[i] - delta);
+      for (int i = 0; i < 16; ++i)
+        p[i] = exp2_fast(fmaf(s[i], a.c, -lse)) * (narrow<T>() ? fmaf(g[i], times, -delta) : g[i] - delta);
       if (EDGE && k0 + BK - 1 > wave_min) {
 #pragma unroll
         for (int i = 0; i < 16; ++i)
@@ -164,7 +224,7 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attenti
 #pragma unroll
     for (int i = 0; i < 16; i += 4)
       store4<T>(po + d * 32 + result_row(i, half),
-                f32x4{acc[d][i] * a.scale, acc[d][i + 1] * a.scale, acc[d][i + 2] * a.scale, acc[d][i + 3] * a.scale});
+                f32x4{acc[d][i] * back, acc[d][i + 1] * back, acc[d][i + 2] * back, acc[d][i + 3] * back});
 }
 
 // dk, dv: a workgroup per (tile of keys, key head), a wavefront per 32 keys whose K and V rows stay in
@@ -191,6 +251,7 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
   __shared__ __align__(16) char lds[4 * TILE];
   __shared__ __align__(16) float s_lse[2][BR], s_delta[2][BR];
   __shared__ __align__(16) int s_pos[2][BR];
+  __shared__ float s_most[4];
   const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = lane >> 5;
   const int h = blockIdx.x % a.Hkv;
   const int want = blockIdx.x / a.Hkv;  // the first keys are seen by the most rows: they go first
@@ -244,6 +305,7 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
   place(threadIdx.x & (BR - 1), tok_s, head_s);
   const char* qb = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + t.start * a.q_t + (int64_t)h * a.G * a.q_h);
   const char* gb = reinterpret_cast<const char*>(static_cast<const T*>(a.go) + t.start * a.go_t + (int64_t)h * a.G * a.go_h);
+  float times = 1.f, back_k = a.scale, back_v = 1.f;  // f16: the factors of dS (beyond P's) and what takes them out again
   Raw<T> qr[PER], gr[PER];
   float r_lse, r_delta;
   int r_pos;
@@ -298,10 +360,26 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
       store_chunk<T, D, PLANE>(tq, threadIdx.x / CH + i * STEP, threadIdx.x % CH, qr[i]);
       store_chunk<T, D, PLANE>(tq + TILE, threadIdx.x / CH + i * STEP, threadIdx.x % CH, gr[i]);
     }
-    if (threadIdx.x < BR)
-      s_lse[buf][threadIdx.x] = r_lse, s_delta[buf][threadIdx.x] = r_delta, s_pos[buf][threadIdx.x] = r_pos;
+    if (threadIdx.x < BR) {
+      s_lse[buf][threadIdx.x] = narrow<T>() ? r_lse - kOrders : r_lse;
+      s_delta[buf][threadIdx.x] = narrow<T>() ? r_delta * times : r_delta;
+      s_pos[buf][threadIdx.x] = r_pos;
+    }
   };
   load(lo);
+  if constexpr (narrow<T>()) {
+    static_assert(kNormKeys % grad_keys<T, D>() == 0, "a tile's keys share a norm");
+    float most = 0.f;
+    const float* norms = a.row_norm + (h * a.total + t.start) * a.G;
+    for (int r = (a.causal ? tile0 * a.G / 32 + (int)threadIdx.x : (int)threadIdx.x) * 32; r < t.len * a.G; r += 256 * 32)
+      most = fmaxf(most, norms[r]);
+    most = wave_max(most);
+    if (lane == 0) s_most[wv] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
+    const int order = order_of(most, a.value_norm[h * a.total + t.start + tile0 / kNormKeys * kNormKeys]);
+    times = ldexpf(1.f, -order), back_k = ldexpf(a.scale, order - kOrders), back_v = ldexpf(1.f, -kOrders);
+  }
   store(0);
   __syncthreads();
   const int b = wv / KG, own = b * 32 * D * 2;  // this wavefront's block of 32 rows of a tile
@@ -336,7 +414,7 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       p[i] = exp2_fast(fmaf(s[i], a.c, -lse[i >> 2][i & 3]));
-      ds[i] = p[i] * (g[i] - dl[i >> 2][i & 3]);
+      ds[i] = p[i] * (narrow<T>() ? fmaf(g[i], times, -dl[i >> 2][i & 3]) : g[i] - dl[i >> 2][i & 3]);
     }
     if (EDGE) {
 #pragma unroll
@@ -391,8 +469,8 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
 #pragma unroll
     for (int i = 0; i < 16; i += 4) {
       const int c = d * 32 + result_row(i, half);
-      store4<T>(pk + c, f32x4{gk[d][i] * a.scale, gk[d][i + 1] * a.scale, gk[d][i + 2] * a.scale, gk[d][i + 3] * a.scale});
-      store4<T>(pv + c, f32x4{gv[d][i], gv[d][i + 1], gv[d][i + 2], gv[d][i + 3]});
+      store4<T>(pk + c, f32x4{gk[d][i] * back_k, gk[d][i + 1] * back_k, gk[d][i + 2] * back_k, gk[d][i + 3] * back_k});
+      store4<T>(pv + c, f32x4{gv[d][i] * back_v, gv[d][i + 1] * back_v, gv[d][i + 2] * back_v, gv[d][i + 3] * back_v});
     }
 }
 
@@ -402,6 +480,10 @@ static void launch_rows(const RowsArgs& a, unsigned grid, hipStream_t st) {
 }
 template <typename T, int D>
 static void launch_rows_backward(const GradArgs& a, unsigned grid, hipStream_t st) {
+  if constexpr (narrow<T>()) {
+    const int64_t tiles = (a.total + kNormKeys - 1) / kNormKeys + a.N;
+    hipLaunchKernelGGL((attention_value_norms_kernel<T, D>), dim3((unsigned)(tiles * a.Hkv)), dim3(256), 0, st, a);
+  }
   hipLaunchKernelGGL((attention_rows_backward_kernel<T, D>), dim3(grid), dim3(256), 0, st, a);
 }
 template <typename T, int D>
@@ -451,7 +533,7 @@ extern "C" int aps_attention_packed(const void* q, const void* k, const void* v,
 }
 
 extern "C" int64_t aps_attention_packed_backward_workspace(int64_t total, int64_t Hq) {
-  return total < 0 || Hq < 1 ? -1 : total * Hq * (int64_t)sizeof(float);
+  return total < 0 || Hq < 1 ? -1 : 3 * total * Hq * (int64_t)sizeof(float);
 }
 
 extern "C" int aps_attention_packed_backward(const void* q, const void* k, const void* v, const void* out,
@@ -471,7 +553,8 @@ extern "C" int aps_attention_packed_backward(const void* q, const void* k, const
   APS_CHECK_ARG(strides_fit(q_t, q_h, e) && strides_fit(k_t, k_h, e) && strides_fit(v_t, v_h, e));
   APS_CHECK_ARG(strides_fit(go_t, go_h, e));
   GradArgs a{};
-  a.q = q, a.k = k, a.v = v, a.o = out, a.rest = out_rest, a.go = g_out, a.lse = lse, a.delta = static_cast<float*>(workspace);
+  a.q = q, a.k = k, a.v = v, a.o = out, a.rest = out_rest, a.go = g_out, a.lse = lse;
+  a.delta = static_cast<float*>(workspace), a.row_norm = a.delta + total * Hq, a.value_norm = a.row_norm + total * Hq;
   a.gq = g_q, a.gk = g_k, a.gv = g_v;
   a.cu = Index{cu_seqlens, cu_wide};
   a.total = total, a.N = N;

@@ -649,7 +649,7 @@ def _attention_packed_backward(ctx, g):
     g_k = th.empty_like(k, memory_format=th.contiguous_format)
     g_v = th.empty_like(v, memory_format=th.contiguous_format)
     if T:
-        ws = th.empty_like(sums)  # aps_attention_packed_backward_workspace bytes
+        ws = th.empty(3, T, Hq, device=q.device, dtype=th.float32)  # aps_attention_packed_backward_workspace bytes
         with nat.on_device_of(q):
             rc = nat.load().aps_attention_packed_backward(
                 q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), None if rest is None else rest.data_ptr(),

@@ -593,7 +593,10 @@ def attention_packed(q: th.Tensor, k: th.Tensor, v: th.Tensor, cu_seqlens: th.Te
     cu[n + 1] - 1; from 0, non-decreasing; rows behind cu[N] belong to no sequence and give zeros.
     causal: a token sees its own sequence up to itself, else all of it; scale defaults to D ** -0.5.
     q, k, v may be slices of one fused projection (read in place).  Differentiable in q, k and v
-    (aps_attention_packed_backward: the same bits on every run)."""
+    (aps_attention_packed_backward: the same bits on every run).  In 16 bits the weights, and the gradients of the
+    scores, are rounded to the type between the products (f16: after powers of two that keep them in its range), sums
+    and softmax are in f32; a training call keeps a second tensor of the output's size, what the output's rounding took
+    away."""
     what = "attention_packed"
     if k.dim() != 3 or v.dim() != 3 or k.shape[0] != q.shape[0]:
         raise RuntimeError(f"{what}: k {tuple(k.shape)} / v {tuple(v.shape)} must be {q.shape[0]} x heads x head_dim")

@@ -1069,6 +1069,8 @@ int aps_attention_packed(const void* q, const void* k, const void* v, const void
 /* its adjoint: g_out [total, Hq, dh] by strides -> g_q [total, Hq, dh], g_k / g_v [total, Hkv, dh]
  * contiguous, the same bits on every run (no atomics).  out, lse, out_rest (f32: NULL): of the forward call.  A
  * non-finite value of a sequence may reach all gradients of that sequence (0 * infinity is NaN), none of another.
+ * f16: P and dS are rounded after powers of two taken from the norms of g_out and v, so gradients of any size keep
+ * their 11 bits.
  * workspace: aps_attention_packed_backward_workspace bytes. */
 int64_t aps_attention_packed_backward_workspace(int64_t total, int64_t Hq);
 int aps_attention_packed_backward(const void* q, const void* k, const void* v, const void* out,
