@@ -68,11 +68,10 @@ __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void atte
       clear_rows<T, D>(static_cast<T*>(a.out), a.cu, a.N, a.total, Hq, want - t.used, a.tiles - t.used);
     return;
   }
-  const int64_t n = a.kv_lens.at(t.seq);
-  const int kv = (int)(n < 0 ? 0 : (n > a.max_keys ? a.max_keys : n));
-  const int off = kv - t.len, rows = t.len * a.G, row0 = t.tile * ROWS;
-  const int end = min(kv, off + (min(row0 + ROWS, rows) - 1) / a.G + 1);
-  const int least = off + row0 / a.G;  // the tile's first position: keys up to it need no mask
+  const int off = first_position(a.kv_lens, t.seq, t.len, a.max_keys), kv = max(clipped(off, t.len, (int)a.max_keys), 0);
+  const int rows = t.len * a.G, row0 = t.tile * ROWS;
+  const int end = clipped(off, (min(row0 + ROWS, rows) - 1) / a.G + 1, kv);
+  const int least = clipped(off, row0 / a.G, kv - 1);  // the tile's first position: keys up to it need no mask
   int pos[R];
   u32x4 qf[R][NS];
 #pragma unroll
@@ -80,7 +79,7 @@ __global__ __launch_bounds__(256, (sizeof(T) * D * R >= 1024 ? 1 : 2)) void atte
     const int row = row0 + r * 16 + c;
     const bool live = row < rows;
     const int tok = live ? row / a.G : 0, head = h * a.G + (live ? row - tok * a.G : 0);
-    pos[r] = live ? off + tok : -1;
+    pos[r] = live ? clipped(off, tok, kv - 1) : -1;
     const T* qp = static_cast<const T*>(a.q) + (t.start + tok) * a.q_t + head * a.q_h;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
@@ -352,10 +351,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   int start, end;
   seq_range(a.cu, lo, a.total, start, end);
   if (tok < start || tok >= end) return;
-  int64_t kv = a.kv_lens.at(lo);
-  kv = kv < 0 ? 0 : (kv > a.max_keys ? a.max_keys : kv);
-  const int64_t pos = kv - (end - tok);
-  if (pos < 0) return;
+  const int64_t pos = (int64_t)first_position(a.kv_lens, lo, end - start, a.max_keys) + (tok - start);
+  if (pos < 0 || pos >= a.max_keys) return;
   const int32_t p = a.table[lo * a.table_stride + (pos >> a.page_shift)];
   if (p < 0 || p >= a.num_pages) return;
   const int64_t slot = ((int64_t)p << a.page_shift) + (pos & ((1 << a.page_shift) - 1));

@@ -47,6 +47,17 @@ struct RowsArgs {
   int32_t splits;
 };
 
+// Position of the first of a sequence's `len` new tokens, the last of its kv_lens[n] positions.  Whatever the array
+// holds it lies in [-len, max_keys]: a token behind the table's `max_keys` positions keeps its place there, without a
+// page of its own, and one before 0 sees nothing.
+__device__ __forceinline__ int first_position(const Index& kv_lens, int64_t n, int len, int64_t max_keys) {
+  const int64_t kv = kv_lens.at(n);
+  return (int)(kv < 0 ? 0 : (kv > max_keys + len ? max_keys + len : kv)) - len;
+}
+
+// off + i, at most `most`
+__device__ __forceinline__ int clipped(int off, int i, int most) { return (int)min((int64_t)off + i, (int64_t)most); }
+
 // keys of a tile (f32: three planes; D = 32: a chunk for every thread)
 template <typename T, int D>
 constexpr int key_tile() { return sizeof(T) == 2 || D == 32 ? 64 : 32; }
@@ -204,26 +215,27 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>())) void attention_rows_kern
       clear_rows<T, D>(static_cast<T*>(a.out), a.cu, a.N, a.total, Hq, want - t.used, a.tiles - t.used);
     return;
   }
-  int kv = t.len;
+  int kv = t.len, off = 0;  // keys; position of the sequence's first query
   if constexpr (PAGED) {
-    const int64_t n = a.kv_lens.at(t.seq);
-    kv = (int)(n < 0 ? 0 : (n > a.max_keys ? a.max_keys : n));
+    off = first_position(a.kv_lens, t.seq, t.len, a.max_keys);
+    kv = max(clipped(off, t.len, (int)a.max_keys), 0);
   }
-  const int off = kv - t.len;  // position of the sequence's first query
+  // the last key that token i of the sequence sees
+  auto place = [&](int i) { return PAGED ? clipped(off, i, kv - 1) : i; };
   const int rows = t.len * a.G;
   const int row0 = t.tile * kRowTile + wv * 32;
   const int row = row0 + (lane & 31);
   const bool live = row < rows;
   const int tok = live ? row / a.G : 0, head = h * a.G + (live ? row - tok * a.G : 0);
-  const int pos = live ? (a.causal ? off + tok : kv - 1) : -1;
+  const int pos = live ? (a.causal ? place(tok) : kv - 1) : -1;
   // keys the tile / the wavefront can see; the least position in the wavefront (no mask below it)
   const int tile_last = min(t.tile * kRowTile + kRowTile, rows) - 1;
   const int last = min(row0 + 32, rows) - 1;
   int end = kv, wave_end = kv, wave_min = kv - 1;
   if (a.causal) {
-    end = min(kv, off + tile_last / a.G + 1);
-    wave_end = row0 < rows ? min(kv, off + last / a.G + 1) : 0;
-    wave_min = off + row0 / a.G;
+    end = place(tile_last / a.G) + 1;
+    wave_end = row0 < rows ? place(last / a.G) + 1 : 0;
+    wave_min = place(row0 / a.G);
   } else if (row0 >= rows) {
     wave_end = 0;
   }
@@ -251,7 +263,7 @@ __global__ __launch_bounds__(256, (rows_waves<T, D>())) void attention_rows_kern
   KvStage<T, D, PAGED> st;
   bool bad = false;  // a non-finite value in a tile that some row sees only in part
   // tiles that every row of the workgroup sees whole: no mask, no branch; then the others
-  const int block_min = a.causal ? off + t.tile * kRowTile / a.G : kv - 1;
+  const int block_min = a.causal ? place(t.tile * kRowTile / a.G) : kv - 1;
   const int clear = min(tile_hi, (block_min + 1) / BK);
   if (tile_lo < tile_hi) {
     st.locate(a, t.seq, tile_lo * BK, end);

@@ -661,7 +661,8 @@ def paged_append(k: th.Tensor, v: th.Tensor, k_pages: th.Tensor, v_pages: th.Ten
     """Write the keys / values of new tokens (k / v T x Hkv x D, sequence n's at rows cu_seqlens[n] ..) into
     a paged cache: k_pages / v_pages P x page x Hkv x D (page a power of two), page_table N x W int32 (position
     p of sequence n lies in page page_table[n, p // page]), kv_lens N: the positions of each sequence WITH its new
-    tokens, which are the last of them.  Positions without a page (an entry outside 0 .. P - 1) are not written.
+    tokens, which are the last of them.  Positions without a page (behind the table's W pages, or an entry outside
+    0 .. P - 1) are not written.
     Only the written slots change; two sequences must not write the same slot."""
     what = "paged_append"
     if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or k.shape[2] not in PACKED_HEAD_DIMS or \

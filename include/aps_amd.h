@@ -1085,9 +1085,9 @@ int aps_attention_packed_backward(const void* q, const void* k, const void* v, c
  * (page 1: a slot per token, so the row of a table is a history that can be copied and regrouped);
  * page_table int32 [N, width] (row stride table_stride): position p of sequence n lies in page
  * page_table[n, p / page]; kv_lens [N] (int32, or int64 with kv_wide = 1): positions of sequence n, the
- * new tokens (its cu_seqlens range) being the last of them.  A position whose page is outside
- * [0, num_pages) is hidden from the attention and not written; one before 0 (more new tokens than
- * positions) sees nothing and is not written.
+ * new tokens (its cu_seqlens range) being the last of them.  A position behind the table's width, or whose page is
+ * outside [0, num_pages), is hidden from the attention and not written; one before 0 (more new tokens than positions)
+ * sees nothing and is not written.
  * aps_paged_append: k / v [total, Hkv, dh] (by strides) of the new tokens into the cache. */
 int aps_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
                      const void* cu_seqlens, int32_t cu_wide, const void* kv_lens, int32_t kv_wide,

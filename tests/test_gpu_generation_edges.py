@@ -38,3 +38,37 @@ def test_gradients_of_rows_far_apart(group):
         vals, bounds = ref.packed(leaf, k, v, [n], causal, g=g)
         for name, got, want, bound in zip(("out", "gq", "gk", "gv"), (out,) + grads, vals, bounds):
             ref.check(got, want, bound, f"{name} causal={causal}")
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("new", [1, 5, 40, 90])
+def test_positions_behind_the_table(kind, new):
+    """more positions than the table has pages for: such tokens are not written and see what is cached; the others
+    keep their places"""
+    from aps_amd import nn_ops
+    hq, hkv, d, page, width = 4, 2, 64, 8, 9
+    most = page * width
+    kv_lens = [most + 3, most + new, most + 2000, most - 1, (1 << 31) - 1]
+    n = len(kv_lens)
+    cache = [randn(n * width + 1, page, hkv, d, dtype=TYPES[kind], seed=i) for i in (1, 2)]
+    table = (torch.randperm(n * width, generator=torch.Generator().manual_seed(3)).view(n, width) + 1).int()
+    q, k, v = (randn(n * new, h, d, dtype=TYPES[kind], seed=i) for i, h in ((4, hq), (5, hkv), (6, hkv)))
+    want = [c.clone() for c in cache]
+    for i, kv in enumerate(kv_lens):
+        for j in range(new):
+            p = kv - new + j
+            if 0 <= p < most:
+                want[0][table[i, p // page], p % page] = k[i * new + j]
+                want[1][table[i, p // page], p % page] = v[i * new + j]
+    args = (*cache, table.to(DEV), cu_of([new] * n), torch.tensor(kv_lens, device=DEV))
+    nn_ops.paged_append(k, v, *args)
+    assert torch.equal(cache[0], want[0]) and torch.equal(cache[1], want[1])
+    out = nn_ops.attention_paged(q, *args)
+    for i, kv in enumerate(kv_lens):
+        ks, vs = (c[table[i].long()].reshape(most, hkv, d).double().cpu() for c in cache)
+        for h in range(hq):
+            rows = q[i * new:(i + 1) * new, h].double().cpu()
+            off = min(kv - new, most)  # (a position behind the table sees all of it)
+            val, bound = ref.attend(rows, ks[:, h // 2], vs[:, h // 2], off, True, d**-0.5, TYPES[kind])
+            ref.check(out[i * new:(i + 1) * new, h], val, bound, f"sequence {i} head {h}")
