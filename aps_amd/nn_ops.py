@@ -643,17 +643,22 @@ def _check_cache(what: str, rows: int, k_pages: th.Tensor, v_pages: th.Tensor, p
     page = k_pages.shape[1]
     if page < 1 or page & (page - 1) or page > 65536 or k_pages.shape[0] < 1:
         raise RuntimeError(f"{what}: {k_pages.shape[0]} pages of {page}: the page size must be a power of two up to 65536")
-    if page_table.dim() != 2 or page_table.dtype != th.int32 or page_table.shape[1] < 1 or page_table.stride(1) != 1:
+    if page_table.dim() != 2 or page_table.dtype != th.int32 or page_table.shape[1] < 1 or \
+            (page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise RuntimeError(f"{what}: page_table must be int32 sequences x pages, got {tuple(page_table.shape)} "
                            f"{page_table.dtype}")
-    N = page_table.shape[0]
-    if page_table.stride(0) < page_table.shape[1]:
+    N, W = page_table.shape
+    if N > 1 and page_table.stride(0) < W:  # (a single row may have any stride: `_table_stride`)
         page_table = page_table.contiguous()
     cu_seqlens = _index_array(cu_seqlens, f"{what}: cu_seqlens", N + 1)
     kv_lens = _index_array(kv_lens, f"{what}: kv_lens", N)
     if N < 1 and rows:
         raise RuntimeError(f"{what}: {rows} tokens and no sequence")
     return page_table, cu_seqlens, kv_lens
+
+
+def _table_stride(page_table: th.Tensor) -> int:
+    return max(page_table.stride(0), page_table.shape[1])
 
 
 def paged_append(k: th.Tensor, v: th.Tensor, k_pages: th.Tensor, v_pages: th.Tensor, page_table: th.Tensor,
@@ -684,7 +689,7 @@ def paged_append(k: th.Tensor, v: th.Tensor, k_pages: th.Tensor, v_pages: th.Ten
             k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
             cu_seqlens.data_ptr(), int(cu_seqlens.dtype == th.int64), kv_lens.data_ptr(),
             int(kv_lens.dtype == th.int64), T, page_table.shape[0], H, D, k_pages.shape[0], k_pages.shape[1],
-            page_table.shape[1], page_table.stride(0), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            page_table.shape[1], _table_stride(page_table), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
             ELEMENT_TYPES[k.dtype], nat.stream_of(k))
     nat.check(rc, "aps_paged_append")
 
@@ -725,7 +730,7 @@ def attention_paged(q: th.Tensor, k_pages: th.Tensor, v_pages: th.Tensor, page_t
         rc = lib.aps_attention_paged(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), cu_seqlens.data_ptr(),
             int(cu_seqlens.dtype == th.int64), kv_lens.data_ptr(), int(kv_lens.dtype == th.int64), out.data_ptr(), T,
-            N, Hq, Hkv, D, P, page, W, page_table.stride(0), q.stride(0), q.stride(1), dtype, scale, int(keep),
+            N, Hq, Hkv, D, P, page, W, _table_stride(page_table), q.stride(0), q.stride(1), dtype, scale, int(keep),
             None if ws is None else ws.data_ptr(), nat.stream_of(q))
     nat.check(rc, "aps_attention_paged")
     return out

@@ -72,3 +72,27 @@ def test_positions_behind_the_table(kind, new):
             off = min(kv - new, most)  # (a position behind the table sees all of it)
             val, bound = ref.attend(rows, ks[:, h // 2], vs[:, h // 2], off, True, d**-0.5, TYPES[kind])
             ref.check(out[i * new:(i + 1) * new, h], val, bound, f"sequence {i} head {h}")
+
+
+@gpu
+def test_tables_of_one_row_or_one_column():
+    """a table whose only row or column has the stride of what it was cut from"""
+    from aps_amd import nn_ops
+    hkv, d, page = 2, 64, 16
+    pages = torch.tensor([5, 0, 3, 2], dtype=torch.int32, device=DEV)
+    for table, kv in ((pages.view(4, 1).t(), [60]),               # 1 x 4, strides (1, 1)
+                      (pages.view(1, 4)[:, :3], [40]),
+                      (pages.view(1, 4).t(), [16, 3, 9, 1]),      # 4 x 1, strides (1, 4)
+                      (pages.repeat(3, 1).t()[:, 1:2], [4, 16, 2, 7]),
+                      (pages[:1].expand(1, 1), [12]),
+                      (torch.stack([pages, pages.flip(0)]).t()[::2].t(), [30, 2])):
+        n = len(kv)
+        plain = table.contiguous().clone()
+        q, k, v = (randn(n, h, d, seed=i) for i, h in enumerate((4, hkv, hkv)))
+        got = []
+        for t in (plain, table if table.stride(1) == 1 or table.shape[1] == 1 else plain):
+            cache = [randn(6, page, hkv, d, seed=i) for i in (7, 8)]
+            args = (*cache, t, cu_of([1] * n), torch.tensor(kv, device=DEV))
+            nn_ops.paged_append(k, v, *args)
+            got.append([nn_ops.attention_paged(q, *args), *cache])
+        assert all(torch.equal(a, b) for a, b in zip(*got))
