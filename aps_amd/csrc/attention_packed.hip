@@ -512,7 +512,7 @@ extern "C" int aps_attention_packed(const void* q, const void* k, const void* v,
                                     int64_t k_t, int64_t k_h, int64_t v_t, int64_t v_h, int32_t dtype,
                                     int32_t causal, float scale, void* stream) {
   if (total == 0) return APS_OK;
-  APS_CHECK_ARG(q && k && v && cu_seqlens && out && sizes_fit(total, N, Hq, Hkv) && scale > 0.f);
+  APS_CHECK_ARG(q && k && v && cu_seqlens && out && sizes_fit(total, N, Hq, Hkv) && scale_fits(scale));
   const int64_t e = dtype == kTypeF32 ? 4 : 8;
   APS_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_rest));
   APS_CHECK_ARG(strides_fit(q_t, q_h, e) && strides_fit(k_t, k_h, e) && strides_fit(v_t, v_h, e));
@@ -546,7 +546,7 @@ extern "C" int aps_attention_packed_backward(const void* q, const void* k, const
   if (total == 0) return APS_OK;
   APS_CHECK_ARG(q && k && v && out && g_out && lse && cu_seqlens && g_q && g_k && g_v && workspace);
   APS_CHECK_ARG(dtype == kTypeF32 || out_rest);
-  APS_CHECK_ARG(sizes_fit(total, N, Hq, Hkv) && scale > 0.f);
+  APS_CHECK_ARG(sizes_fit(total, N, Hq, Hkv) && scale_fits(scale));
   const int64_t e = dtype == kTypeF32 ? 4 : 8;
   APS_CHECK_ARG(aligned16(q) && aligned16(k) && aligned16(v) && aligned16(out) && aligned16(out_rest) && aligned16(g_out));
   APS_CHECK_ARG(aligned16(g_q) && aligned16(g_k) && aligned16(g_v));

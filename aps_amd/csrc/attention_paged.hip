@@ -429,7 +429,7 @@ extern "C" int aps_attention_paged(const void* q, const void* k_pages, const voi
                                    int64_t q_h, int32_t dtype, float scale, int32_t keep_tail, void* workspace,
                                    void* stream) {
   if (total == 0) return APS_OK;
-  APS_CHECK_ARG(q && k_pages && v_pages && page_table && cu_seqlens && kv_lens && out && scale > 0.f);
+  APS_CHECK_ARG(q && k_pages && v_pages && page_table && cu_seqlens && kv_lens && out && scale_fits(scale));
   APS_CHECK_ARG(paged_sizes_fit(total, N, Hq, Hkv, num_pages, page, width) && table_stride >= width);
   const int64_t e = dtype == kTypeF32 ? 4 : 8;
   APS_CHECK_ARG(aligned16(q) && aligned16(k_pages) && aligned16(v_pages) && aligned16(out));

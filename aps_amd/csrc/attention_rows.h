@@ -438,6 +438,12 @@ static inline bool strides_fit(int64_t t, int64_t h, int64_t e) {
   return t % e == 0 && h % e == 0 && t >= 0 && t <= most && h >= 0 && h <= most;
 }
 
+// a scale whose product with log2(e) is a normal f32
+static inline bool scale_fits(float scale) {
+  const float c = scale * kLog2e;
+  return c >= 1.17549435e-38f && c <= 3.4028234663852886e38f;
+}
+
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace att

@@ -580,8 +580,8 @@ def _check_heads(what: str, q: th.Tensor, k: th.Tensor, v: th.Tensor) -> None:
 
 def _softmax_scale(what: str, scale: Optional[float], D: int) -> float:
     scale = D**-0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        raise RuntimeError(f"{what}: scale must be positive and finite, got {scale}")
+    if not 1e-37 < scale < 1e38:
+        raise RuntimeError(f"{what}: scale must be positive and finite in f32 (1e-37 .. 1e38), got {scale}")
     return scale
 
 

@@ -1054,6 +1054,7 @@ int aps_conformer_stack(float* x, const int64_t* lens, const ApsMegaLayer* layer
  *   cu_seqlens [N + 1] (int32, or int64 with cu_wide = 1): tokens cu[n] .. cu[n + 1] - 1 of the packed
  *     axis are sequence n; from 0, non-decreasing, at most `total`.  Values outside that are clamped on
  *     the device.  Rows behind the last sequence belong to none: their outputs / gradients are zeros.
+ *   scale: positive; with log2(e) a normal finite f32.
  *   strides q_t, q_h, ... in elements (token, head; the last axis is contiguous); pointers 16-byte
  *     aligned, strides multiples of 16 bytes.
  * ------------------------------------------------------------------------------------------- */

@@ -1,0 +1,36 @@
+"""CPU: more calls that the packed / paged attention, the beam step and the searches refuse before anything reaches a
+device (the C entries' sizes and pointers: beside test_generation_refusals.py)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from aps_amd import _native as nat
+from aps_amd import nn_ops
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+def buffer():
+    p = C.addressof(C.create_string_buffer(64))
+    return p + -p % 16
+
+
+@pytest.mark.parametrize("scale", [1e39, 3e38, 1e-46, 1e-40, float("inf"), -1e39])
+def test_scales_that_f32_does_not_hold(scale):
+    """1e39 is finite in Python and infinite in f32; 1e-46 is 0 there"""
+    q, cu = t(5, 4, 64), torch.tensor([0, 5], dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="scale"):
+        nn_ops.attention_packed(q, q, q, cu, scale=scale)
+    pages = t(3, 4, 4, 64)
+    with pytest.raises(RuntimeError, match="scale"):
+        nn_ops.attention_paged(q, pages, pages, t(1, 3, dtype=torch.int32), cu, cu[1:], scale=scale)
+    lib, p = nat.load(), buffer()
+    assert lib.aps_attention_packed(p, p, p, p, 0, p, None, None, 5, 1, 4, 2, 64, 256, 64, 128, 64, 128, 64, 0, 1, scale,
+                                    None) == -1
+    assert lib.aps_attention_packed_backward(p, p, p, p, p, p, p, p, 0, p, p, p, 5, 1, 4, 2, 64, 256, 64, 128, 64, 128, 64,
+                                             256, 64, 1, 1, scale, p, None) == -1
+    assert lib.aps_attention_paged(p, p, p, p, p, 0, p, 0, p, 5, 2, 4, 2, 64, 8, 16, 3, 3, 256, 64, 0, scale, 0, None,
+                                   None) == -1
