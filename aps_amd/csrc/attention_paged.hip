@@ -415,6 +415,11 @@ static bool paged_sizes_fit(int64_t total, int64_t N, int64_t Hq, int64_t Hkv, i
          (page & (page - 1)) == 0 && num_pages >= 1 && num_pages <= (int64_t)0x7fff0000 / page && width >= 1 && width <= (int64_t)0x7fff0000 / page;
 }
 
+static inline bool apart(const void* p, int64_t p_bytes, const void* q, int64_t q_bytes) {
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a + (uint64_t)p_bytes <= b || b + (uint64_t)q_bytes <= a;
+}
+
 extern "C" int64_t aps_attention_paged_workspace(int64_t total, int64_t N, int64_t Hq, int64_t Hkv,
                                                  int64_t head_dim, int64_t page, int64_t width, int32_t dtype) {
   if (!paged_sizes_fit(total, N, Hq, Hkv, 1, page, width)) return -1;
@@ -470,6 +475,13 @@ extern "C" int aps_paged_append(const void* k, const void* v, void* k_pages, voi
   const int64_t e = dtype == kTypeF32 ? 4 : 8;
   APS_CHECK_ARG(aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages));
   APS_CHECK_ARG(strides_fit(k_t, k_h, e) && strides_fit(v_t, v_h, e));
+  // (slots that one launch reads and writes, or writes twice, would hold what came last)
+  const int64_t bytes = 16 / e, held = num_pages * page * Hkv * head_dim * bytes;
+  const int64_t of_k = ((total - 1) * k_t + (Hkv - 1) * k_h + head_dim) * bytes;
+  const int64_t of_v = ((total - 1) * v_t + (Hkv - 1) * v_h + head_dim) * bytes;
+  APS_CHECK_ARG(apart(k_pages, held, v_pages, held));
+  APS_CHECK_ARG(apart(k, of_k, k_pages, held) && apart(k, of_k, v_pages, held));
+  APS_CHECK_ARG(apart(v, of_v, k_pages, held) && apart(v, of_v, v_pages, held));
   AppendArgs a{};
   a.k = k, a.v = v, a.k_pages = k_pages, a.v_pages = v_pages;
   a.cu = Index{cu_seqlens, cu_wide}, a.kv_lens = Index{kv_lens, kv_wide};

@@ -668,7 +668,8 @@ def paged_append(k: th.Tensor, v: th.Tensor, k_pages: th.Tensor, v_pages: th.Ten
     p of sequence n lies in page page_table[n, p // page]), kv_lens N: the positions of each sequence WITH its new
     tokens, which are the last of them.  Positions without a page (behind the table's W pages, or an entry outside
     0 .. P - 1) are not written.
-    Only the written slots change; two sequences must not write the same slot."""
+    Only the written slots change; two sequences must not write the same slot, and the two caches must not overlap each
+    other or k / v (refused)."""
     what = "paged_append"
     if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype or k.shape[2] not in PACKED_HEAD_DIMS or \
             k.dtype not in ELEMENT_TYPES:

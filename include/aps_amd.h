@@ -1089,7 +1089,8 @@ int aps_attention_packed_backward(const void* q, const void* k, const void* v, c
  * new tokens (its cu_seqlens range) being the last of them.  A position behind the table's width, or whose page is
  * outside [0, num_pages), is hidden from the attention and not written; one before 0 (more new tokens than positions)
  * sees nothing and is not written.
- * aps_paged_append: k / v [total, Hkv, dh] (by strides) of the new tokens into the cache. */
+ * aps_paged_append: k / v [total, Hkv, dh] (by strides) of the new tokens into the cache.  The two caches must not
+ * overlap each other, nor the extent of k or v. */
 int aps_paged_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
                      const void* cu_seqlens, int32_t cu_wide, const void* kv_lens, int32_t kv_wide,
                      int64_t total, int64_t N, int64_t Hkv, int64_t head_dim, int64_t num_pages, int64_t page,

@@ -34,3 +34,26 @@ def test_scales_that_f32_does_not_hold(scale):
                                              256, 64, 1, 1, scale, p, None) == -1
     assert lib.aps_attention_paged(p, p, p, p, p, 0, p, 0, p, 5, 2, 4, 2, 64, 8, 16, 3, 3, 256, 64, 0, scale, 0, None,
                                    None) == -1
+
+
+def test_append_refuses_a_cache_that_overlaps():
+    """slots read and written by one launch, in no order: the caches with each other, k or v with either; checked at the
+    C entry (no device here: a call that passes the checks fails at its launch instead)"""
+    lib = nat.load()
+    hold = C.create_string_buffer(1 << 17)
+    base = C.addressof(hold) + -C.addressof(hold) % 16
+    pages, page, heads, dim, total = 3, 4, 2, 64, 4
+    held, row = pages * page * heads * dim * 4, 2 * heads * dim * 4  # k and v as slices of rows twice as wide
+
+    def append(k, v, kc, vc, idx=base + 120000):
+        return lib.aps_paged_append(base + k, base + v, base + kc, base + vc, idx, idx, 0, idx, 0, total, 1, heads, dim, pages,
+                                    page, 3, 3, row // 4, dim, row // 4, dim, 0, None)
+
+    new = 2 * held
+    for k, v, kc, vc in ((new, new, 0, 0), (new, new, 0, held - 16), (new, new, held - 16, 0), (0, new, 0, held),
+                         (new, held - 16, 0, held), (new, 2 * held - 16, 0, held), (new, new, new, 0),
+                         (new, new, 0, new + total * row - row // 2 - 16)):
+        assert append(k, v, kc, vc) == -1, (k, v, kc, vc)
+    if not torch.cuda.is_available():
+        assert append(new, new + row // 2, 0, held) not in (0, -1)
+        assert append(new, new, 0, new + total * row) not in (0, -1)
