@@ -10,6 +10,7 @@ from ctypes import c_void_p as C_void_p
 from typing import List, Optional, Sequence
 
 import torch as th
+from torch.autograd import forward_ad
 
 from aps_amd import _native as nat
 
@@ -555,6 +556,13 @@ def _strided16(t: th.Tensor) -> th.Tensor:
     return t.clone(memory_format=th.contiguous_format)
 
 
+def _refuse_tangents(what: str, *tensors) -> None:
+    """forward-mode derivatives pass none of these kernels: dual tensors would lose their tangents without a word"""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and \
+            any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: no forward-mode derivative (torch.autograd.forward_ad)")
+
+
 def _index_array(t: th.Tensor, what: str, length: Optional[int] = None) -> th.Tensor:
     if t.dim() != 1 or t.dtype not in (th.int32, th.int64) or (length is not None and t.shape[0] != length):
         want = "" if length is None else f" of {length}"
@@ -605,6 +613,7 @@ def attention_packed(q: th.Tensor, k: th.Tensor, v: th.Tensor, cu_seqlens: th.Te
     if cu_seqlens.shape[0] < 2:
         raise RuntimeError(f"{what}: cu_seqlens holds the N + 1 bounds of N >= 1 sequences")
     scale = _softmax_scale(what, scale, q.shape[2])
+    _refuse_tangents(what, q, k, v)
     if nat.needs_grad(q, k, v):
         from aps_amd.grad_ops import AttentionPackedFn
         return AttentionPackedFn.apply(q, k, v, cu_seqlens, bool(causal), scale)
@@ -680,6 +689,7 @@ def paged_append(k: th.Tensor, v: th.Tensor, k_pages: th.Tensor, v_pages: th.Ten
             v_pages.dtype != k.dtype:
         raise RuntimeError(f"{what}: cache {tuple(k_pages.shape)} {k_pages.dtype} / {tuple(v_pages.shape)} does not fit "
                            f"k {tuple(k.shape)} {k.dtype}")
+    _refuse_tangents(what, k, v)
     nat.require_device(k, v, k_pages, v_pages, page_table, cu_seqlens, kv_lens)
     T, H, D = k.shape
     if not T or not H:
@@ -707,6 +717,7 @@ def attention_paged(q: th.Tensor, k_pages: th.Tensor, v_pages: th.Tensor, page_t
     page_table, cu_seqlens, kv_lens = _check_cache(what, q.shape[0], k_pages, v_pages, page_table, cu_seqlens, kv_lens)
     _check_heads(what, q, k_pages, v_pages)
     scale = _softmax_scale(what, scale, q.shape[2])
+    _refuse_tangents(what, q, k_pages, v_pages)
     nat.require_device(q, k_pages, v_pages, page_table, cu_seqlens, kv_lens, out)
     lib = nat.load()
     T, Hq, D = q.shape
@@ -777,6 +788,7 @@ def beam_select(logits: th.Tensor, scores: th.Tensor, eos: int, finished: Option
         raise RuntimeError(f"{what}: eos {eos} outside the vocabulary of {V}")
     if finished is not None and (finished.shape != scores.shape or finished.dtype != th.bool):
         raise RuntimeError(f"{what}: finished must be bool {tuple(scores.shape)}, got {tuple(finished.shape)} {finished.dtype}")
+    _refuse_tangents(what, logits, scores)
     dev = nat.require_device(logits, scores, finished)
     lib = nat.load()
     if len(shape) == 3:
@@ -814,6 +826,7 @@ def beam_reorder(states: Sequence[th.Tensor], parent: th.Tensor, dims: Optional[
         raise RuntimeError(f"{what}: {len(states)} states, {len(dims)} dims")
     if not states:
         return []
+    _refuse_tangents(what, *states)
     nat.require_device(parent, *states)
     N, K = parent.shape
     B, src, dst, outer, inner = 0, [], [], [], []

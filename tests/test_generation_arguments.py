@@ -57,3 +57,23 @@ def test_append_refuses_a_cache_that_overlaps():
     if not torch.cuda.is_available():
         assert append(new, new + row // 2, 0, held) not in (0, -1)
         assert append(new, new, 0, new + total * row) not in (0, -1)
+
+
+def test_forward_mode_is_refused():
+    """dual tensors (without requires_grad) would come out without their tangents"""
+    from torch.autograd import forward_ad
+    cu, idx = torch.tensor([0, 5], dtype=torch.int32), t(1, 3, dtype=torch.int32)
+    x, pages = t(5, 4, 64), t(3, 4, 4, 64)
+    parent = torch.zeros(1, 5, dtype=torch.int64)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        s = forward_ad.make_dual(t(1, 5), t(1, 5))
+        for call in (lambda: nn_ops.attention_packed(d, x, x, cu), lambda: nn_ops.attention_packed(x, x, d, cu),
+                     lambda: nn_ops.attention_packed(d.requires_grad_(), x, x, cu),
+                     lambda: nn_ops.attention_paged(d, pages, pages, idx, cu, cu[1:]),
+                     lambda: nn_ops.paged_append(x, d, pages, pages.clone(), idx, cu, cu[1:]),
+                     lambda: nn_ops.beam_select(t(5, 9), s, 1), lambda: nn_ops.beam_reorder([d], parent)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="GPU only"):  # (no tangent: the usual way)
+            nn_ops.attention_packed(x, x, x, cu)
