@@ -838,6 +838,8 @@ def beam_reorder(states: Sequence[th.Tensor], parent: th.Tensor, dims: Optional[
         if rows < N or rows % N or (B and rows != N * B):
             raise RuntimeError(f"{what}: axis {d} of {tuple(shape)} is not {N} x {B or 'hypotheses'}")
         B = rows // N
+        if t.is_conj() or t.is_neg():  # (a view whose memory holds something else)
+            t = t.resolve_conj().resolve_neg()
         t = t.contiguous()
         src.append(t)
         if B == K:

@@ -96,3 +96,16 @@ def test_tables_of_one_row_or_one_column():
             nn_ops.paged_append(k, v, *args)
             got.append([nn_ops.attention_paged(q, *args), *cache])
         assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@gpu
+def test_reordered_states_that_are_lazy_views():
+    """conjugated complex states and the imaginary part of one: their values, not their memory"""
+    from aps_amd import nn_ops
+    z = torch.randn(6, 5, dtype=torch.complex64, generator=torch.Generator().manual_seed(1)).to(DEV)
+    parent = torch.tensor([[2, 0, 0], [1, 1, 2]], device=DEV)
+    rows = (parent + 3 * torch.arange(2, device=DEV)[:, None]).reshape(-1)
+    states = [z, z.conj(), z.conj().imag, z.conj().t()]
+    out = nn_ops.beam_reorder(states, parent, dims=[0, 0, 0, 1])
+    for x, s, d in zip(out, states, (0, 0, 0, 1)):
+        assert torch.equal(x, s.index_select(d, rows)), s
