@@ -90,7 +90,9 @@ class XfmrASR(ASREncoderDecoderBase):
     @th.no_grad()
     def beam_search(self, x_pad: th.Tensor, x_len: NoneOrTensor = None, beam: int = 8, max_len: int = 100):
         """x_pad N x Ti x D | N x S -> (tokens N x beam x L, scores N x beam, lengths N x beam), best first:
-        TorchTransformerDecoder.beam_search behind `sos`"""
+        TorchTransformerDecoder.beam_search behind `sos`.  The model must be in eval() mode"""
+        if any(m.training for m in self.modules()):
+            raise RuntimeError("beam_search: put the model into eval() mode, all of its modules")
         enc_out, _, enc_len = self._training_prep(x_pad, x_len)
         prompt = th.full((enc_out.shape[0], 1), self.sos, dtype=th.int64, device=enc_out.device)
         return self.decoder.beam_search(enc_out, enc_len, prompt, self.eos, beam=beam, max_len=max_len)

@@ -191,8 +191,8 @@ class TorchTransformerDecoder(nn.Module):
         hypothesis: `paged_append`, `attention_paged`, `beam_select`, `beam_reorder`.  A page holds one token,
         so a hypothesis' past is a row of slot numbers: taking over another's past copies that row, no
         keys or values.  The module must be in eval() mode (no dropout)."""
-        if self.training:
-            raise RuntimeError("beam_search: put the decoder into eval() mode")
+        if any(m.training for m in self.modules()):
+            raise RuntimeError("beam_search: put the decoder into eval() mode, all of its modules")
         N, P = prompt.shape
         dev, dim = enc_out.device, self.vocab_embed.embedding_dim
         layers = list(self.decoder.layers)
