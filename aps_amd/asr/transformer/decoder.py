@@ -22,7 +22,7 @@ from torch.nn import MultiheadAttention
 from aps_amd.asr.transformer.impl import _check_activation, get_activation_fn
 from aps_amd.grad_ops import ScaleAddFn, dropout, dropout_active
 from aps_amd.asr.transformer.pose import get_xfmr_pose
-from aps_amd.nn_ops import (PACKED_HEAD_DIMS, attention_core, attention_cross, attention_packed,
+from aps_amd.nn_ops import (BEAM_MAX, PACKED_HEAD_DIMS, attention_core, attention_cross, attention_packed,
                             attention_paged, beam_reorder, beam_select, embedding_posenc, layernorm, linear,
                             paged_append, posenc_add)
 
@@ -193,6 +193,10 @@ class TorchTransformerDecoder(nn.Module):
         keys or values.  The module must be in eval() mode (no dropout)."""
         if any(m.training for m in self.modules()):
             raise RuntimeError("beam_search: put the decoder into eval() mode, all of its modules")
+        if prompt.dim() != 2 or enc_out.dim() != 3 or prompt.shape[0] != enc_out.shape[0] or \
+                (enc_len is not None and enc_len.shape != enc_out.shape[:1]):
+            raise RuntimeError(f"beam_search: enc_out {tuple(enc_out.shape)}, prompt {tuple(prompt.shape)}, enc_len "
+                               f"{None if enc_len is None else tuple(enc_len.shape)}: one prompt and one length an utterance")
         N, P = prompt.shape
         dev, dim = enc_out.device, self.vocab_embed.embedding_dim
         layers = list(self.decoder.layers)
@@ -200,8 +204,10 @@ class TorchTransformerDecoder(nn.Module):
         head_dim = dim // heads
         if head_dim not in PACKED_HEAD_DIMS:
             raise NotImplementedError(f"beam_search: heads of {head_dim}, the cache's attention takes {PACKED_HEAD_DIMS}")
-        if P < 1 or max_len < 1 or not 1 <= beam <= self.vocab_size:
-            raise RuntimeError(f"beam_search: prompt of {P} tokens, {max_len} more, {beam} of {self.vocab_size} tokens")
+        if N < 1 or P < 1 or max_len < 1 or not 1 <= beam <= min(self.vocab_size, BEAM_MAX) or \
+                not 0 <= eos < self.vocab_size:
+            raise RuntimeError(f"beam_search: {N} prompts of {P} tokens, {max_len} more, beam {beam} (1 .. {BEAM_MAX}), eos "
+                               f"{eos}, {self.vocab_size} tokens")
         pose = self.abs_pos_enc
         memory = enc_out.contiguous()
         kvs = [layer.memory_kv(memory) for layer in layers]

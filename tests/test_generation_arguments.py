@@ -105,3 +105,16 @@ def test_searches_refuse_modules_in_training():
     net.eval()
     with pytest.raises(RuntimeError, match="GPU only"):
         net.beam_search(t(2, 50, 40), torch.tensor([50, 40]))
+
+
+def test_search_arguments():
+    """what does not fit is refused by name, not somewhere inside the first step"""
+    from aps_amd.asr.transformer.decoder import TorchTransformerDecoder
+    dec = TorchTransformerDecoder(90, pose_kwargs={"dropout": 0}, num_layers=1, arch_kwargs=ARCH).eval()
+    enc, lens, prompt = t(3, 5, 64), torch.tensor([5, 4, 3]), torch.zeros(3, 1, dtype=torch.int64)
+    for args, kw in (((enc, lens, prompt[:1], 1), {}), ((enc, lens, prompt[:2], 1), {}), ((enc[0], lens, prompt, 1), {}),
+                     ((enc, lens, prompt[:, 0], 1), {}), ((enc, lens[:2], prompt, 1), {}),
+                     ((enc, lens[:, None], prompt, 1), {}), ((enc, lens, prompt, 90), {}), ((enc, lens, prompt, -1), {}),
+                     ((enc, lens, prompt, 1), {"beam": 65}), ((enc[:0], None, prompt[:0], 1), {})):
+        with pytest.raises(RuntimeError, match="beam_search:"):
+            dec.beam_search(*args, **kw)
