@@ -211,7 +211,8 @@ class TorchTransformerDecoder(nn.Module):
         pose = self.abs_pos_enc
         memory = enc_out.contiguous()
         kvs = [layer.memory_kv(memory) for layer in layers]
-        caches = [th.empty(2, N * P + N * beam * max_len, 1, heads, head_dim, device=dev) for _ in layers]
+        caches = [th.empty(2, N * P + N * beam * max_len, 1, heads, head_dim, device=dev, dtype=th.float32)
+                  for _ in layers]
 
         def forward(tokens: th.Tensor, at: int, table: th.Tensor, cu: th.Tensor, lens: th.Tensor) -> th.Tensor:
             """tokens N x rows x new (their positions at, at + 1, ...) -> logits of the last, N rows x V"""
@@ -235,7 +236,7 @@ class TorchTransformerDecoder(nn.Module):
         table[:, :P] = th.arange(N * P, dtype=th.int32, device=dev).view(N, P)
         cu = th.arange(0, N * P + 1, P, dtype=th.int32, device=dev)
         logits = forward(prompt.view(N, 1, P), 0, table, cu, th.full((N,), P, dtype=th.int32, device=dev))
-        scores, parent, token, done = beam_select(logits, th.zeros(N, 1, device=dev), eos, beam=beam)
+        scores, parent, token, done = beam_select(logits, th.zeros(N, 1, device=dev, dtype=th.float32), eos, beam=beam)
         (table,) = beam_reorder([table], parent)
         tokens = th.full((N * beam, max_len), eos, dtype=th.int64, device=dev)
         tokens[:, 0] = token.view(-1)

@@ -109,3 +109,127 @@ def test_reordered_states_that_are_lazy_views():
     out = nn_ops.beam_reorder(states, parent, dims=[0, 0, 0, 1])
     for x, s, d in zip(out, states, (0, 0, 0, 1)):
         assert torch.equal(x, s.index_select(d, rows)), s
+
+
+# ---- searches ------------------------------------------------------------------------------------
+
+def check_search(found, want, eos):
+    tokens, scores, lengths = found
+    for i, hyps in enumerate(want):
+        for b, (score, toks, _) in enumerate(hyps):
+            assert lengths[i, b].item() == len(toks), (i, b)
+            assert tokens[i, b, :len(toks)].tolist() == toks, (i, b)
+            assert (tokens[i, b, len(toks):] == eos).all()
+            assert abs(scores[i, b].item() - score) < 1e-4 * max(1.0, abs(score))
+    assert tokens.shape[2] == lengths.max()
+
+
+def small_decoder(V, seed):
+    from aps_amd.asr.transformer.decoder import TorchTransformerDecoder
+    torch.manual_seed(seed)
+    dec = TorchTransformerDecoder(V, pose_kwargs={"dropout": 0}, num_layers=2,
+                                  arch_kwargs={"att_dim": 64, "nhead": 2, "feedforward_dim": 128, "att_dropout": 0,
+                                               "ffn_dropout": 0}).eval().to(DEV)
+    with torch.no_grad():
+        dec.output.weight.mul_(4.0)
+    return dec
+
+
+@gpu
+def test_long_searches_and_their_early_end():
+    """more than 16 tokens; and a search whose hypotheses have all ended long before max_len, so that it stops: against a
+    search that runs the decoder over every prefix"""
+    from tests.test_gpu_generation import search_reference
+    V, n, beam = 23, 2, 3
+    dec = small_decoder(V, 17)
+    enc, enc_len = randn(n, 19, 64, seed=3), torch.tensor([19, 8], device=DEV)
+    prompt = torch.tensor([[5], [7]], device=DEV)
+
+    def step(toks, rows):
+        with torch.no_grad():
+            return dec(enc[rows], enc_len[rows], toks.to(DEV), None)[:, -1].double().cpu()
+
+    first = dec.beam_search(enc, enc_len, prompt, 0, beam=beam, max_len=20)
+    check_search(first, search_reference(step, n, prompt.tolist(), 0, beam, 20), 0)
+    assert first[2].max() > 16
+    # every token that opens a hypothesis a lot ends them early: take for eos what was used most
+    eos = int(torch.bincount(first[0].flatten(), minlength=V).argmax())
+    from aps_amd import nn_ops
+    from aps_amd.asr.transformer import decoder as module
+    count = [0]
+
+    def counted(*args, **kw):
+        count[0] += 1
+        return nn_ops.beam_select(*args, **kw)
+
+    module.beam_select = counted
+    try:
+        found = dec.beam_search(enc, enc_len, prompt, eos, beam=beam, max_len=60)
+    finally:
+        module.beam_select = nn_ops.beam_select
+    want = search_reference(step, n, prompt.tolist(), eos, beam, 60)
+    check_search(found, want, eos)
+    longest = int(found[2].max())
+    assert all(done for hyps in want for _, _, done in hyps) and longest < 50
+    assert longest <= count[0] <= (longest + 7) // 8 * 8  # (looked at every eighth step)
+
+
+@gpu
+def test_search_of_one_token_and_of_one_hypothesis():
+    from tests.test_gpu_generation import search_reference
+    dec = small_decoder(11, 23)
+    enc = randn(2, 6, 64, seed=4)
+    prompt = torch.tensor([[3, 4], [5, 1]], device=DEV)
+
+    def step(toks, rows):
+        with torch.no_grad():
+            return dec(enc[rows], None, toks.to(DEV), None)[:, -1].double().cpu()
+
+    for beam, max_len in ((1, 1), (1, 9), (11, 1), (11, 4)):
+        check_search(dec.beam_search(enc, None, prompt, 2, beam=beam, max_len=max_len),
+                     search_reference(step, 2, prompt.tolist(), 2, beam, max_len), 2)
+
+
+@gpu
+@pytest.mark.parametrize("ctc", [False, True])
+def test_xfmr_asr_beam_search(ctc):
+    """waveforms of different lengths -> features -> encoder -> search, against the model's own teacher-forced forward
+    over every prefix; with the CTC branch the decoder's vocabulary is one token shorter"""
+    from aps_amd.libs import aps_asr_nnet
+    from aps_amd.transform import AsrTransform
+    from tests.test_gpu_generation import search_reference
+    torch.manual_seed(31)
+    arch = {"att_dim": 64, "nhead": 2, "feedforward_dim": 128, "att_dropout": 0, "ffn_dropout": 0}
+    V = 21
+    net = aps_asr_nnet("asr@xfmr")(
+        40, V + 1 if ctc else V, sos=V - 1, eos=V - 1, ctc=ctc,
+        asr_transform=AsrTransform(feats="fbank-log-cmvn", frame_len=400, frame_hop=160, window="hamm", num_mels=40),
+        enc_type="xfmr",
+        enc_kwargs=dict(num_layers=2, proj="conv2d", proj_kwargs={"conv_channels": 8, "num_layers": 2}, pose="abs",
+                        pose_kwargs={"dropout": 0}, arch_kwargs=dict(arch)),
+        dec_kwargs=dict(num_layers=2, pose_kwargs={"dropout": 0}, arch_kwargs=dict(arch))).eval().to(DEV)
+    with torch.no_grad():
+        net.decoder.output.weight.mul_(4.0)
+    wav, wav_len = randn(3, 12000, seed=2, std=0.1), torch.tensor([12000, 9000, 7000], device=DEV)
+
+    def step(toks, rows):
+        with torch.no_grad():
+            out, _, _ = net(wav, wav_len, toks.to(DEV).expand(3, -1), None)
+            return out[rows, -1].double().cpu()
+
+    found = net.beam_search(wav, wav_len, beam=3, max_len=6)
+    assert found[0].shape[:2] == (3, 3) and int(found[0].max()) < V
+    check_search(found, search_reference(step, 3, [[V - 1]] * 3, V - 1, 3, 6), V - 1)
+
+
+@gpu
+def test_search_under_another_default_dtype():
+    dec = small_decoder(11, 29)
+    enc, prompt = randn(2, 6, 64, seed=4), torch.tensor([[3], [5]], device=DEV)
+    want = dec.beam_search(enc, None, prompt, 2, beam=3, max_len=5)
+    torch.set_default_dtype(torch.float64)
+    try:
+        got = dec.beam_search(enc, None, prompt, 2, beam=3, max_len=5)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
