@@ -364,10 +364,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 }
 
 // Which kernel and how many splits, from what the host knows (the lengths themselves are on the
-// device): form 1 / 2 = decode tiles of 16 / 32 rows, 0 = 128-row tiles.
+// device): form 1 / 2 = decode tiles of 16 / 32 rows, 0 = 128-row tiles, one for the whole call; the same for every type.
 struct PagedPlan { int form; int64_t tiles; int splits; };
 
-static PagedPlan paged_plan(int64_t total, int64_t N, int64_t G, int64_t Hkv, int64_t max_keys, int64_t dtype) {
+static PagedPlan paged_plan(int64_t total, int64_t N, int64_t G, int64_t Hkv, int64_t max_keys) {
   PagedPlan p;
   const int64_t mean = (total * G + N - 1) / N;  // rows of a sequence and key head
   // (16 x 2 000 keys, rows of 128: 32 rows of bf16 / f32 take 16 / 28 us in decode tiles and 20 / 42 in 128-row
@@ -421,9 +421,9 @@ static inline bool apart(const void* p, int64_t p_bytes, const void* q, int64_t 
 }
 
 extern "C" int64_t aps_attention_paged_workspace(int64_t total, int64_t N, int64_t Hq, int64_t Hkv,
-                                                 int64_t head_dim, int64_t page, int64_t width, int32_t dtype) {
+                                                 int64_t head_dim, int64_t page, int64_t width, int32_t) {
   if (!paged_sizes_fit(total, N, Hq, Hkv, 1, page, width)) return -1;
-  const PagedPlan p = paged_plan(total, N, Hq / Hkv, Hkv, width * page, dtype);
+  const PagedPlan p = paged_plan(total, N, Hq / Hkv, Hkv, width * page);
   return p.splits > 1 ? p.splits * total * Hq * (head_dim + 2) * (int64_t)sizeof(float) : 0;
 }
 
@@ -449,7 +449,7 @@ extern "C" int aps_attention_paged(const void* q, const void* k_pages, const voi
   a.k_t = a.v_t = Hkv * head_dim, a.k_h = a.v_h = head_dim;
   a.num_pages = num_pages, a.max_keys = width * page, a.page_shift = __builtin_ctzll((uint64_t)page);
   a.causal = 1, a.zero_tail = keep_tail == 0, a.c = scale * kLog2e;
-  const PagedPlan p = paged_plan(total, N, a.G, Hkv, a.max_keys, dtype);
+  const PagedPlan p = paged_plan(total, N, a.G, Hkv, a.max_keys);
   APS_CHECK_ARG(p.tiles * Hkv < 0x7fffffff);
   a.tiles = p.tiles, a.splits = p.splits;
   if (p.splits > 1) {

@@ -1098,7 +1098,7 @@ int aps_paged_append(const void* k, const void* v, void* k_pages, void* v_pages,
                      int32_t dtype, void* stream);
 /* the new tokens' attention over everything cached up to themselves; a row that sees nothing gives zeros.
  * keep_tail = 1: rows of no sequence are left as they are instead of cleared.
- * workspace: aps_attention_paged_workspace bytes (0: none needed). */
+ * workspace: aps_attention_paged_workspace bytes (0: none needed; partial results are f32 whatever `dtype` is). */
 int64_t aps_attention_paged_workspace(int64_t total, int64_t N, int64_t Hq, int64_t Hkv, int64_t head_dim,
                                       int64_t page, int64_t width, int32_t dtype);
 int aps_attention_paged(const void* q, const void* k_pages, const void* v_pages, const int32_t* page_table,
