@@ -233,3 +233,103 @@ def test_search_under_another_default_dtype():
     finally:
         torch.set_default_dtype(torch.float32)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- far offsets, rows of no sequence ------------------------------------------------------------
+
+@gpu
+@pytest.mark.parametrize("new", [1, 20, 100])
+def test_pages_behind_four_billion_elements(new):
+    """a cache of more than 2^32 elements whose last pages are the ones in use: offsets in 64 bits, in the append and in
+    the kernels for few and for many rows"""
+    from aps_amd import nn_ops
+    hq, hkv, d, page, count = 8, 4, 128, 64, (1 << 32) // (4 * 128 * 64) + 40
+    cache = [torch.zeros(count, page, hkv, d, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    kv = [1500, new + 3]
+    table = torch.stack([count - 1 - torch.arange(24), torch.arange(24) + count - 48]).int().to(DEV)
+    old = [[randn(n - new, hkv, d, dtype=torch.bfloat16, seed=10 * i + j) for j in range(2)] for i, n in enumerate(kv)]
+    for i, rows in enumerate(old):
+        at = torch.arange(rows[0].shape[0], device=DEV)
+        for c, r in zip(cache, rows):
+            c[table[i, at // page].long(), at % page] = r
+    q, k, v = (randn(2 * new, h, d, dtype=torch.bfloat16, seed=i) for i, h in ((1, hq), (2, hkv), (3, hkv)))
+    args = (*cache, table, cu_of([new, new]), torch.tensor(kv, device=DEV))
+    nn_ops.paged_append(k, v, *args)
+    out = nn_ops.attention_paged(q, *args)
+    for i in range(2):
+        cut = slice(i * new, (i + 1) * new)
+        ks, vs = (torch.cat([o, x[cut]]).double().cpu() for o, x in zip(old[i], (k, v)))
+        for h in range(hq):
+            want, bound = ref.attend(q[cut, h].double().cpu(), ks[:, h // 2], vs[:, h // 2], kv[i] - new, True, d**-0.5,
+                                     torch.bfloat16)
+            ref.check(out[cut, h], want, bound, f"sequence {i} head {h}")
+
+
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_rows_before_the_first_sequence(kind):
+    """cu_seqlens that begins behind 0: the rows ahead belong to none, like those behind the last"""
+    from aps_amd import nn_ops
+    lens, lead, tail = [40, 0, 77], 9, 5
+    t = lead + sum(lens) + tail
+    x = [randn(t, h, 64, dtype=TYPES[kind], seed=i).requires_grad_() for i, h in enumerate((4, 2, 2))]
+    g = randn(t, 4, 64, dtype=TYPES[kind], seed=5)
+    cu = cu_of(lens) + lead
+    out = nn_ops.attention_packed(*x, cu)
+    grads = torch.autograd.grad(out, x, g)
+    body = slice(lead, t - tail)
+    vals, bounds = ref.packed(*(y[body] for y in x), lens, True, g=g[body])
+    for name, got, want, bound in zip(("out", "gq", "gk", "gv"), (out,) + grads, vals, bounds):
+        ref.check(got[body], want, bound, name)
+        assert not got[:lead].any() and not got[t - tail:].any()
+    q, k, v = (y.detach() for y in x)
+    cache = [torch.zeros(40, 16, 2, 64, dtype=TYPES[kind], device=DEV) for _ in range(2)]
+    args = (*cache, torch.arange(39, device=DEV, dtype=torch.int32).view(3, 13) + 1, cu, torch.tensor(lens, device=DEV))
+    nn_ops.paged_append(k, v, *args)
+    paged = nn_ops.attention_paged(q, *args)
+    ref.check(paged[body], vals[0], bounds[0], "paged")
+    assert not paged[:lead].any() and not paged[t - tail:].any()
+    kept = torch.full_like(paged, 3.0)
+    nn_ops.attention_paged(q, *args, out=kept)
+    assert (kept[:lead] == 3).all() and (kept[t - tail:] == 3).all() and torch.equal(kept[body], paged[body])
+    assert not cache[0][0].any()  # (page 0 is in no table)
+
+
+@gpu
+def test_two_captured_steps_share_nothing():
+    """two captured decoding steps replayed in turn and on two streams at once: each its own partial results"""
+    from aps_amd import nn_ops
+    n, hq, hkv, d, page, width = 3, 8, 2, 64, 16, 200
+    sets = []
+    for s in range(2):
+        cache = [randn(n * width, page, hkv, d, dtype=torch.float16, seed=10 * s + i) for i in range(2)]
+        q, k, v = (randn(n, h, d, dtype=torch.float16, seed=10 * s + 3 + i) for i, h in enumerate((hq, hkv, hkv)))
+        args = (*cache, torch.arange(n * width, device=DEV, dtype=torch.int32).view(n, width), cu_of([1] * n),
+                torch.tensor([3000, 17, 2100], device=DEV))
+        x, sc = randn(2 * 4, 5001, seed=30 + s), -randn(2, 4, seed=40 + s).abs()
+
+        def step(q=q, k=k, v=v, args=args, x=x, sc=sc):
+            nn_ops.paged_append(k, v, *args)
+            return [nn_ops.attention_paged(q, *args), *nn_ops.beam_select(x, sc, 1)]
+
+        sets.append(step)
+    with torch.no_grad():
+        want = [s() for s in sets]
+        torch.cuda.synchronize()
+        graphs, held = [], []
+        for s in sets:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1]):
+                held.append(s())
+        streams = [torch.cuda.Stream() for _ in sets]
+        for _ in range(4):
+            for g, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    g.replay()
+            torch.cuda.synchronize()
+            for a, b in zip(held, want):
+                assert all(torch.equal(x, y) for x, y in zip(a, b))
+            eager = [s() for s in sets]
+            torch.cuda.synchronize()
+            for a, b in zip(eager, want):
+                assert all(torch.equal(x, y) for x, y in zip(a, b))
