@@ -14,10 +14,11 @@
 // P and dS are rounded to the tensors' type between the products (attention_tile.h: `pack`).  f16 has 30 binary
 // orders: dS, of the size of do / (row length), would fall below its normal numbers with upstream gradients of 1e-3 and
 // pass its largest with 1e4, and P of long rows is small too.  So f16 takes both times powers of two, which come out
-// again in f32 at the end: P times 2^14 where it is rounded (dv), dS times 2^(14 - e), 2^e > |do_r| |v_j|, so that
-// |dS| <= 2 |do_r| |v_j| becomes at most 2^15.  For dq, e goes by the row's own norm and the largest norm of its
-// sequence's values (a launch ahead leaves one for every 128 keys: 6 us of 620 on the 3 sequences named below); for
-// dk by the key tile's values and the rows that see it (the dq launch leaves a norm for every 32 rows).
+// again in f32 at the end: P times 2^14 where it is rounded (dv), dS times 2^(14 - e), 2^e > |do_r| |v| for the largest
+// v the row sees (o_r, in D_r, is a mean of them all), so that |dS| <= 2 |do_r| |v| becomes at most 2^15.  A launch
+// ahead leaves the largest norm of every 128 keys' values (6 us of 620 on the 3 sequences named below).  For dq, e goes
+// by the row's own norm; for dk by the largest of the rows that see the key tile (the dq launch leaves one for
+// every 32 rows).
 #include "attention_rows.h"
 
 namespace aps {
@@ -73,8 +74,8 @@ __global__ __launch_bounds__(256) void attention_value_norms_kernel(GradArgs a) 
 }
 
 // dq: the forward kernel's walk, with V as the left operand of dP^T = V dO^T beside S^T = K Q^T and K
-// read transposed for dq^T = K^T dS^T.  (The 12 sequences named at the next kernel: 101 us, 660 TFLOP/s; the 3:
-// 183 us, 810.)
+// read transposed for dq^T = K^T dS^T.  (The 12 sequences named at the next kernel: 99 - 107 us by card, 620 - 670
+// TFLOP/s; the 3: 183 - 188 us, 790 - 810.)
 template <typename T, int D>
 __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attention_rows_backward_kernel(GradArgs a) {
   constexpr int BK = key_tile<T, D>(), NS = D / 16, NKB = BK / 32, NDB = D / 32, PLANE = BK * D * 2, TILE = planes<T>() * PLANE;
@@ -235,9 +236,9 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attenti
 // keys of a causal sequence are seen by every row of the group and the longest tile is what the launch
 // waits for (12 sequences of 195 - 2 048 tokens, 16 heads over 4 of 128, bf16: 439 us with tiles of 128, 373 with
 // 64 when it was changed).  f32 with D = 128 has no registers for the larger row tile: four times 32 keys there.
-// That case takes 217 us now, 410 TFLOP/s: 604 tiles on 256 CUs whose longest walks 128 row tiles of 1.7 us, one
+// That case takes 198 - 218 us by card now, 410 - 450 TFLOP/s: 604 tiles on 256 CUs whose longest walks 128 row tiles of 1.7 us, one
 // wavefront a SIMD, LDS and the waits for it half of each; 3 sequences of 3 582 - 4 500, 16 heads of
-// 64, f16, two wavefronts a SIMD: 266 us, 740 TFLOP/s.
+// 64, f16, two wavefronts a SIMD: 267 - 271 us, 730 TFLOP/s.
 template <typename T, int D>
 constexpr int grad_rows() { return D * planes<T>() >= 384 ? 32 : 64; }
 template <typename T, int D>
@@ -368,16 +369,17 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
   };
   load(lo);
   if constexpr (narrow<T>()) {
-    static_assert(kNormKeys % grad_keys<T, D>() == 0, "a tile's keys share a norm");
-    float most = 0.f;
+    float most = 0.f, value = 0.f;
     const float* norms = a.row_norm + (h * a.total + t.start) * a.G;
     for (int r = (a.causal ? tile0 * a.G / 32 + (int)threadIdx.x : (int)threadIdx.x) * 32; r < t.len * a.G; r += 256 * 32)
       most = fmaxf(most, norms[r]);
+    for (int key = lane * kNormKeys; key < t.len; key += 64 * kNormKeys)
+      value = fmaxf(value, a.value_norm[h * a.total + t.start + key]);
     most = wave_max(most);
     if (lane == 0) s_most[wv] = most;
     __syncthreads();
     most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
-    const int order = order_of(most, a.value_norm[h * a.total + t.start + tile0 / kNormKeys * kNormKeys]);
+    const int order = order_of(most, wave_max(value));
     times = ldexpf(1.f, -order), back_k = ldexpf(a.scale, order - kOrders), back_v = ldexpf(1.f, -kOrders);
   }
   store(0);

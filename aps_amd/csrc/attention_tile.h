@@ -14,8 +14,9 @@
 // are formed, h h + (h m + m h) + (h l + l h + m m), smallest first, in f32; the three left out are below
 // 2^-22 |x y| together, as is usual of an f32 product sum.  Any exponent is kept (no scaling); an infinity
 // makes what it is multiplied into NaN.  Six 16-bit MFMAs of 32 cycles stand for eight f32 ones of 64 (32x32x2,
-// 16 deep): 8 sequences of 1 400 - 1 500 tokens, 8 heads of 64, causal, forward and gradients 775 us; with
-// the f32 instructions 1 160 (head size 128: 1 640 against 2 566).
+// 16 deep): 8 sequences of 1 400 - 1 500 tokens, 8 heads of 64, causal, forward and gradients 775 us where the f32
+// instructions took 1 160 (head size 128: 1 640 against 2 566).  Now 614 (1 166), the forward pass 140 (265): 122 - 129
+// TFLOP/s, where a sixth of the library's large bf16 product is 193 - 216; the rest is splitting P and the softmax.
 #ifndef APS_AMD_ATTENTION_TILE_H_
 #define APS_AMD_ATTENTION_TILE_H_
 
@@ -124,9 +125,12 @@ __device__ __forceinline__ f32x16 mma<float>(const Frag<float>& a, const Frag<fl
   return mma_bf16(a.p[0], b.p[0], c);
 }
 
-// 8 registers of a result as an operand (16-bit types: one rounding -- the weights lie in [0, 1] up to a common
-// factor, so it is 2^-9 / 2^-12 of each weight; sums over many keys average it out, and the softmax's own sum is
-// kept from the unrounded values)
+// 8 registers of a result as an operand.  16-bit types: one rounding, of at most 2^-8 (bf16) / 2^-11 (f16) of each number, as
+// the result's own.  A second plane for what it takes away would cost half as many products again.  The weights lie
+// in [0, 1] up to a common factor and their sum is kept from the unrounded values; over many keys the roundings average
+// out, but a result that one rounding alone would leave 1.7e-3 off (bf16, norm) is 2.0e-3 - 2.4e-3 off, and 2.1e-4
+// becomes 2.8e-4 - 3.0e-4 in f16.  f16 weights below 2^-14 of the reference (at most the row's largest) keep 2^-25 of it;
+// the gradients, whose size is the caller's, are scaled first (attention_packed.hip).
 template <typename T>
 __device__ __forceinline__ Frag<T> pack(const float* p) {
   if constexpr (sizeof(T) == 2) {

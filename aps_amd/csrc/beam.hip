@@ -468,7 +468,7 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderArgs a) {
 
 // Elements a thread of the rows kernel takes.  32: 2 048 workgroups read 512 rows of 32 000 f32 logits in 25 us
 // (2.6 TB/s; the 64-bit exponentials keep the vector pipe busy for about half of that).  8 for what would be fewer
-// than two workgroups a CU: 8 rows of 4 233 in 5.7 us, with 32 in 7.5; 45 of 10 007 (bf16) in 5.9, with 32 in 7.9.
+// than two workgroups a CU: 8 rows of 4 233 in 5.7 us, with 32 in 7.5; 45 of 10 007 (bf16) in 6.0, with 32 in 7.9.
 static int per_thread(int64_t rows, int64_t V) { return rows * ((V + 8191) / 8192) < 512 ? 8 : 32; }
 static int64_t splits_of(int64_t rows, int64_t V) {
   const int64_t tile = kThreads * per_thread(rows, V);

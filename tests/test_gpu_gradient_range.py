@@ -155,3 +155,17 @@ def test_captured_gradients_of_a_fused_projection():
         assert torch.equal(first, step())
         q, k, v = leaf.detach().cpu().view(t, 3, h, d).unbind(1)
         check(q, k, v, g.cpu(), lens, True)
+
+
+@gpu
+@pytest.mark.parametrize("causal", [True, False])
+def test_values_whose_size_changes_within_a_sequence(causal):
+    """keys with small values beside keys with large ones: do . o, which all of a row's values are in, is in every dS"""
+    lens = [600, 300]
+    t = sum(lens)
+    at = torch.cat([torch.arange(n) for n in lens])
+    q, k = (half(t, 2, 64, seed=i) for i in range(2))
+    for size in (10.0**(3 - at / 100), 10.0**(at / 100 - 3), torch.where(at < 200, 1000.0, 1e-3), torch.where(at < 256, 0.0, 500.0),
+                 torch.where(at < 256, 500.0, 0.0)):
+        v = (torch.randn(t, 2, 64, generator=torch.Generator().manual_seed(2)) * size[:, None, None]).clamp(-6e4, 6e4).half()
+        check(q, k, v, half(t, 2, 64, seed=4, std=0.2), lens, causal)
