@@ -16,7 +16,8 @@
 // pass its largest with 1e4, and P of long rows is small too.  So f16 takes both times powers of two, which come out
 // again in f32 at the end: P times 2^14 where it is rounded (dv), dS times 2^(14 - e), 2^e > |do_r| |v| for the largest
 // v the row sees (o_r, in D_r, is a mean of them all), so that |dS| <= 2 |do_r| |v| becomes at most 2^15.  A launch
-// ahead leaves the largest norm of every 128 keys' values (6 us of 620 on the 3 sequences named below).  For dq, e goes
+// ahead leaves the largest norm of every 128 keys' values.  (On the 3 sequences named below that launch takes 6 us, dq
+// goes from 184 to 187 us and dk / dv from 269 to 273; maxima by atomics in LDS: 291.)  For dq, e goes
 // by the row's own norm; for dk by the largest of the rows that see the key tile (the dq launch leaves one for
 // every 32 rows).
 #include "attention_rows.h"
@@ -75,7 +76,7 @@ __global__ __launch_bounds__(256) void attention_value_norms_kernel(GradArgs a) 
 
 // dq: the forward kernel's walk, with V as the left operand of dP^T = V dO^T beside S^T = K Q^T and K
 // read transposed for dq^T = K^T dS^T.  (The 12 sequences named at the next kernel: 99 - 107 us by card, 620 - 670
-// TFLOP/s; the 3: 183 - 188 us, 790 - 810.)
+// TFLOP/s; the 3: 187 us, 790.)
 template <typename T, int D>
 __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attention_rows_backward_kernel(GradArgs a) {
   constexpr int BK = key_tile<T, D>(), NS = D / 16, NKB = BK / 32, NDB = D / 32, PLANE = BK * D * 2, TILE = planes<T>() * PLANE;
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attenti
 // 64 when it was changed).  f32 with D = 128 has no registers for the larger row tile: four times 32 keys there.
 // That case takes 198 - 218 us by card now, 410 - 450 TFLOP/s: 604 tiles on 256 CUs whose longest walks 128 row tiles of 1.7 us, one
 // wavefront a SIMD, LDS and the waits for it half of each; 3 sequences of 3 582 - 4 500, 16 heads of
-// 64, f16, two wavefronts a SIMD: 267 - 271 us, 730 TFLOP/s.
+// 64, f16, two wavefronts a SIMD: 268 - 274 us, 720 TFLOP/s.
 template <typename T, int D>
 constexpr int grad_rows() { return D * planes<T>() >= 384 ? 32 : 64; }
 template <typename T, int D>

@@ -333,3 +333,39 @@ def test_two_captured_steps_share_nothing():
             torch.cuda.synchronize()
             for a, b in zip(eager, want):
                 assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_rows_and_no_tokens(kind):
+    """sequences without tokens over a tensor of rows: zeros, or what `out` held"""
+    from aps_amd import nn_ops
+    x = [randn(10, h, 32, dtype=TYPES[kind], seed=i).requires_grad_() for i, h in enumerate((4, 2, 2))]
+    cu = torch.zeros(4, dtype=torch.int32, device=DEV)
+    out = nn_ops.attention_packed(*x, cu)
+    grads = torch.autograd.grad(out, x, torch.ones_like(out))
+    assert not out.any() and not any(g.any() for g in grads)
+    q, k, v = (t.detach() for t in x)
+    for width in (2, 4096):  # (one launch, split keys)
+        cache = [torch.full((5, 4, 2, 32), 2.0, dtype=TYPES[kind], device=DEV) for _ in range(2)]
+        args = (*cache, torch.ones(3, width, dtype=torch.int32, device=DEV), cu, torch.tensor([3, 0, 8], device=DEV))
+        nn_ops.paged_append(k, v, *args)
+        assert (cache[0] == 2).all() and (cache[1] == 2).all()
+        assert not nn_ops.attention_paged(q, *args).any()
+        kept = torch.full((10, 4, 32), 5.0, dtype=TYPES[kind], device=DEV)
+        assert (nn_ops.attention_paged(q, *args, out=kept) == 5).all()
+
+
+@gpu
+def test_largest_vocabulary():
+    from aps_amd import nn_ops
+    v = 1 << 24
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn(2, v, generator=g, device=DEV)
+    x[0, v - 1], x[1, 0], x[1, v // 2] = 9.0, 8.5, 8.0
+    scores, parent, token, done = nn_ops.beam_select(x, torch.tensor([[-1.0, -1.25]], device=DEV), v - 1, beam=64)
+    total = torch.log_softmax(x.double(), 1) + torch.tensor([[-1.0], [-1.25]], device=DEV)
+    best, at = torch.sort(total.flatten(), descending=True, stable=True)
+    assert torch.equal(parent[0], at[:64] // v) and torch.equal(token[0], at[:64] % v)
+    assert ((scores[0].double() - best[:64]).abs() <= 2**-24 * best[:64].abs() + 1e-10).all()
+    assert torch.equal(done[0], token[0] == v - 1)
