@@ -237,9 +237,9 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 192 ? 1 : 2)) void attenti
 // keys of a causal sequence are seen by every row of the group and the longest tile is what the launch
 // waits for (12 sequences of 195 - 2 048 tokens, 16 heads over 4 of 128, bf16: 439 us with tiles of 128, 373 with
 // 64 when it was changed).  f32 with D = 128 has no registers for the larger row tile: four times 32 keys there.
-// That case takes 198 - 218 us by card now, 410 - 450 TFLOP/s: 604 tiles on 256 CUs whose longest walks 128 row tiles of 1.7 us, one
-// wavefront a SIMD, LDS and the waits for it half of each; 3 sequences of 3 582 - 4 500, 16 heads of
-// 64, f16, two wavefronts a SIMD: 268 - 274 us, 720 TFLOP/s.
+// The 12 sequences take 198 - 218 us by card now, 410 - 450 TFLOP/s: 604 tiles on 256 CUs whose longest walks 128
+// row tiles of 1.6 us, one wavefront a SIMD, LDS and the waits for it half of each; 3 sequences of 3 582 - 4 500,
+// 16 heads of 64, f16, two wavefronts a SIMD: 268 - 274 us, 720 TFLOP/s.
 template <typename T, int D>
 constexpr int grad_rows() { return D * planes<T>() >= 384 ? 32 : 64; }
 template <typename T, int D>
@@ -331,7 +331,8 @@ __global__ __launch_bounds__(256, (D * planes<T>() >= 128 ? 1 : 2)) void attenti
       }
     } else {
       // An empty row reads the tile's last token's, which lies in the tile anyway (32-bit offsets hold within a tile, not
-      // to the end of a long sequence), and gets the weight 0 by lse = inf: only offsets lie behind the branch.  (With loads on both of its ways, those met in a wait for all but the
+      // to the end of a long sequence), and gets the weight 0 by lse = inf: only offsets lie behind the branch.
+      // (With loads on both of its ways, those met in a wait for all but the
       // last pair: 253 us against 217 on the 12 sequences.)
       uint32_t qo[PER], go[PER];
 #pragma unroll

@@ -364,7 +364,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 }
 
 // Which kernel and how many splits, from what the host knows (the lengths themselves are on the
-// device): form 1 / 2 = decode tiles of 16 / 32 rows, 0 = 128-row tiles, one for the whole call; the same for every type.
+// device): form 1 / 2 = decode tiles of 16 / 32 rows, 0 = 128-row tiles; one for the whole call, the same for every
+// type.
 struct PagedPlan { int form; int64_t tiles; int splits; };
 
 static PagedPlan paged_plan(int64_t total, int64_t N, int64_t G, int64_t Hkv, int64_t max_keys) {

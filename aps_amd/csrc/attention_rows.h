@@ -52,7 +52,7 @@ struct RowsArgs {
 // page of its own, and one before 0 sees nothing.
 __device__ __forceinline__ int first_position(const Index& kv_lens, int64_t n, int len, int64_t max_keys) {
   const int64_t kv = kv_lens.at(n);
-  return (int)(kv < 0 ? 0 : (kv > max_keys + len ? max_keys + len : kv)) - len;
+  return (int)((kv < 0 ? 0 : (kv > max_keys + len ? max_keys + len : kv)) - len);
 }
 
 // off + i, at most `most`
