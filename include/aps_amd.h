@@ -1055,6 +1055,8 @@ int aps_conformer_stack(float* x, const int64_t* lens, const ApsMegaLayer* layer
  *     axis are sequence n; from 0, non-decreasing, at most `total`.  Values outside that are clamped on
  *     the device.  Rows behind the last sequence belong to none: their outputs / gradients are zeros.
  *   scale: positive; with log2(e) a normal finite f32.
+ *   Non-finite values reach only the rows that see them (forward).  f32: an infinity in q or k makes NaN of the scores
+ *     it takes part in, of those too that would be -infinity.
  *   strides q_t, q_h, ... in elements (token, head; the last axis is contiguous); pointers 16-byte
  *     aligned, strides multiples of 16 bytes.
  * ------------------------------------------------------------------------------------------- */
